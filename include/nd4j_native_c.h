@@ -253,6 +253,125 @@ void nd4j_amd_setSlotTicket(Nd4jPointer *extraPointers, unsigned int value);
 void nd4j_amd_execReduceFloatNoAlloc(Nd4jPointer *extraPointers, int opNum, float *x, Nd4jLong *xShapeInfo,
                                      float *extraParams, float *result);
 
+/* ---- operators around a language model's matrix products: no counterpart in the reference ---------------
+ * Layer norm, embedding, log probabilities of tokens and clipping by the global norm, forward and backward.
+ *
+ * Arguments.  Data pointers are device pointers of the current device, as everywhere; tokens, indexes and offsets
+ * are 64-bit.  A shapeInfo argument describes rows: its last dimension holds a row's elements (any stride), the
+ * leading dimensions merge into rows a common distance apart (a matrix of either order, a padded or sliced matrix,
+ * a dense array of any rank; a rank-1 array is one row).  Host copies travel in extraPointers as usual - [0] for the
+ * first shapeInfo argument, [8] for the last, [7] for the one between - or the argument itself is a host pointer;
+ * otherwise the shapeInfo is read back from the device, which synchronises the stream.  Gains, biases and per-row
+ * values are dense vectors.  Per-row statistics, log probabilities and norms have the compute type: float for Half.
+ *
+ * Execution.  Every call is enqueued on the stream of extraPointers[1], returns without waiting, allocates nothing
+ * but scratch, gives the same bits for the same inputs, and may be captured into a graph.  Calls with a `scratch`
+ * argument take null for it (the library then keeps a block per device and stream, freed by
+ * nd4j_amd_releaseStream) or scratchBytes bytes of the caller's at a 16-byte boundary, at least what the
+ * nd4j_amd_scratch... function of that call says for the sizes.  On a stream under capture null is refused: a graph
+ * needs scratch that no other graph and no other stream uses while it runs.  Arguments that do not fit are refused
+ * (nd4j_lastError) before anything is enqueued; results are then left untouched.  Results must not overlap inputs
+ * unless a call says so. */
+
+/* z = (x - mean) / sqrt(variance + epsilon) * gain + bias, mean and variance (divided by the length) of every row.
+ * gain and bias may be null.  mean and invStd (1 / sqrt(variance + epsilon)) receive a value per row for the
+ * backward call; either may be null.  z may be x (the same view). */
+void nd4j_amd_execLayerNormFloat(Nd4jPointer *extraPointers, float *x, Nd4jLong *xShapeInfo, float *gain,
+                                 float *bias, float *z, Nd4jLong *zShapeInfo, float *mean, float *invStd,
+                                 double epsilon);
+void nd4j_amd_execLayerNormHalf(Nd4jPointer *extraPointers, float16 *x, Nd4jLong *xShapeInfo, float16 *gain,
+                                float16 *bias, float16 *z, Nd4jLong *zShapeInfo, float *mean, float *invStd,
+                                double epsilon);
+void nd4j_amd_execLayerNormDouble(Nd4jPointer *extraPointers, double *x, Nd4jLong *xShapeInfo, double *gain,
+                                  double *bias, double *z, Nd4jLong *zShapeInfo, double *mean, double *invStd,
+                                  double epsilon);
+/* The gradients for dz, the gradient of z: dx, dGain (also without a gain: that of one left out), dBias; each may be
+ * null, not all.  mean and invStd are those of the forward call.  dx may be dz or x (the same view).  Without rows
+ * dGain and dBias become zero. */
+void nd4j_amd_execLayerNormBpFloat(Nd4jPointer *extraPointers, float *x, Nd4jLong *xShapeInfo, float *gain,
+                                   float *mean, float *invStd, float *dz, Nd4jLong *dzShapeInfo, float *dx,
+                                   Nd4jLong *dxShapeInfo, float *dGain, float *dBias, Nd4jPointer scratch,
+                                   Nd4jLong scratchBytes);
+void nd4j_amd_execLayerNormBpHalf(Nd4jPointer *extraPointers, float16 *x, Nd4jLong *xShapeInfo, float16 *gain,
+                                  float *mean, float *invStd, float16 *dz, Nd4jLong *dzShapeInfo, float16 *dx,
+                                  Nd4jLong *dxShapeInfo, float16 *dGain, float16 *dBias, Nd4jPointer scratch,
+                                  Nd4jLong scratchBytes);
+void nd4j_amd_execLayerNormBpDouble(Nd4jPointer *extraPointers, double *x, Nd4jLong *xShapeInfo, double *gain,
+                                    double *mean, double *invStd, double *dz, Nd4jLong *dzShapeInfo, double *dx,
+                                    Nd4jLong *dxShapeInfo, double *dGain, double *dBias, Nd4jPointer scratch,
+                                    Nd4jLong scratchBytes);
+Nd4jLong nd4j_amd_scratchLayerNormBp(Nd4jLong rows, Nd4jLong length);
+
+/* z[i] = scale * table[tokens[i]] for n tokens (rows of z).  A negative token is padding: its row of z is zero.  A
+ * token that the table has no row for makes its row of z NaN. */
+void nd4j_amd_execEmbeddingFloat(Nd4jPointer *extraPointers, float *table, Nd4jLong *tableShapeInfo,
+                                 Nd4jLong *tokens, Nd4jLong n, float *z, Nd4jLong *zShapeInfo, double scale);
+void nd4j_amd_execEmbeddingHalf(Nd4jPointer *extraPointers, float16 *table, Nd4jLong *tableShapeInfo,
+                                Nd4jLong *tokens, Nd4jLong n, float16 *z, Nd4jLong *zShapeInfo, double scale);
+void nd4j_amd_execEmbeddingDouble(Nd4jPointer *extraPointers, double *table, Nd4jLong *tableShapeInfo,
+                                  Nd4jLong *tokens, Nd4jLong n, double *z, Nd4jLong *zShapeInfo, double scale);
+/* dTable[v] = scale * the sum of dz[i] over the i with tokens[i] == v, added onto what dTable holds when accumulate
+ * is not 0 (rows without a token then stay as they are; otherwise they become zero).  Tokens without a row of the table
+ * have no part.  The sum is taken in the compute type, in an order that depends on the tokens alone, and rounded once. */
+void nd4j_amd_execEmbeddingBpFloat(Nd4jPointer *extraPointers, float *dz, Nd4jLong *dzShapeInfo, Nd4jLong *tokens,
+                                   Nd4jLong n, float *dTable, Nd4jLong *dTableShapeInfo, double scale,
+                                   int accumulate, Nd4jPointer scratch, Nd4jLong scratchBytes);
+void nd4j_amd_execEmbeddingBpHalf(Nd4jPointer *extraPointers, float16 *dz, Nd4jLong *dzShapeInfo, Nd4jLong *tokens,
+                                  Nd4jLong n, float16 *dTable, Nd4jLong *dTableShapeInfo, double scale,
+                                  int accumulate, Nd4jPointer scratch, Nd4jLong scratchBytes);
+void nd4j_amd_execEmbeddingBpDouble(Nd4jPointer *extraPointers, double *dz, Nd4jLong *dzShapeInfo, Nd4jLong *tokens,
+                                    Nd4jLong n, double *dTable, Nd4jLong *dTableShapeInfo, double scale,
+                                    int accumulate, Nd4jPointer scratch, Nd4jLong scratchBytes);
+Nd4jLong nd4j_amd_scratchEmbeddingBp(Nd4jLong n, Nd4jLong vocabulary, Nd4jLong length);
+
+/* Per row of logits x: logSum = log(sum of exp(x)), logProbs = x[tokens[row]] - logSum, entropy = -sum p log p of
+ * p = exp(x - logSum), and the k (0 to 64, at most the length) likeliest tokens with their log probabilities, largest
+ * first, the lower token first among equals: rows of k in topTokens and topLogProbs.  Every result may be null (topTokens
+ * only with k = 0), tokens too when logProbs is.  A negative token is padding: its log probability is 0; a token behind
+ * the row's end gives NaN.  Elements of -infinity have probability 0; a row of nothing else has logSum -infinity, log
+ * probabilities -infinity (padding: 0) and entropy 0.  NaN or +infinity in a row makes its results NaN; NaN is never
+ * among the alternatives, and where fewer than k elements are numbers the rest of topTokens is -1. */
+void nd4j_amd_execTokenLogProbsFloat(Nd4jPointer *extraPointers, float *x, Nd4jLong *xShapeInfo, Nd4jLong *tokens,
+                                     float *logProbs, float *logSum, float *entropy, int k, Nd4jLong *topTokens,
+                                     float *topLogProbs, Nd4jPointer scratch, Nd4jLong scratchBytes);
+void nd4j_amd_execTokenLogProbsHalf(Nd4jPointer *extraPointers, float16 *x, Nd4jLong *xShapeInfo, Nd4jLong *tokens,
+                                    float *logProbs, float *logSum, float *entropy, int k, Nd4jLong *topTokens,
+                                    float *topLogProbs, Nd4jPointer scratch, Nd4jLong scratchBytes);
+void nd4j_amd_execTokenLogProbsDouble(Nd4jPointer *extraPointers, double *x, Nd4jLong *xShapeInfo, Nd4jLong *tokens,
+                                      double *logProbs, double *logSum, double *entropy, int k, Nd4jLong *topTokens,
+                                      double *topLogProbs, Nd4jPointer scratch, Nd4jLong scratchBytes);
+Nd4jLong nd4j_amd_scratchTokenLogProbs(Nd4jLong rows, Nd4jLong length, int k);
+/* dx = dLogProbs (delta(token) - p) - dEntropy p (log p + entropy) with the logSum and entropy of the forward call.
+ * dLogProbs or dEntropy may be null (tokens and entropy then too).  A negative token's dLogProbs counts as 0, a token
+ * behind the row's end makes the row of dx NaN, a row without a distribution (logSum -infinity) gets zeros.  The
+ * alternatives are not differentiated.  dx may be x (the same view). */
+void nd4j_amd_execTokenLogProbsBpFloat(Nd4jPointer *extraPointers, float *x, Nd4jLong *xShapeInfo, Nd4jLong *tokens,
+                                       float *logSum, float *entropy, float *dLogProbs, float *dEntropy, float *dx,
+                                       Nd4jLong *dxShapeInfo);
+void nd4j_amd_execTokenLogProbsBpHalf(Nd4jPointer *extraPointers, float16 *x, Nd4jLong *xShapeInfo, Nd4jLong *tokens,
+                                      float *logSum, float *entropy, float *dLogProbs, float *dEntropy, float16 *dx,
+                                      Nd4jLong *dxShapeInfo);
+void nd4j_amd_execTokenLogProbsBpDouble(Nd4jPointer *extraPointers, double *x, Nd4jLong *xShapeInfo,
+                                        Nd4jLong *tokens, double *logSum, double *entropy, double *dLogProbs,
+                                        double *dEntropy, double *dx, Nd4jLong *dxShapeInfo);
+
+/* norm[0] = the square root of the sum of the squares of all elements of n tensors, and dz = dx * maxNorm / norm where
+ * the norm is finite and greater than maxNorm, dz = dx otherwise (a norm of infinity or NaN changes nothing, so that the
+ * caller can look at it and skip the step).  dx and dz are device tables of n device pointers, dense tensors of
+ * offsets[i + 1] - offsets[i] elements (offsets: n + 1 entries on the device, from 0, ascending); dz may be the table dx,
+ * or name the same tensors: clipping in place.  total is offsets[n], known to the host.  norm may be null; with dz null
+ * the norm alone is computed and maxNorm is not looked at. */
+void nd4j_amd_execClipByGlobalNormFloat(Nd4jPointer *extraPointers, Nd4jPointer *dx, Nd4jPointer *dz,
+                                        Nd4jLong *offsets, int n, Nd4jLong total, double maxNorm, float *norm,
+                                        Nd4jPointer scratch, Nd4jLong scratchBytes);
+void nd4j_amd_execClipByGlobalNormHalf(Nd4jPointer *extraPointers, Nd4jPointer *dx, Nd4jPointer *dz,
+                                       Nd4jLong *offsets, int n, Nd4jLong total, double maxNorm, float *norm,
+                                       Nd4jPointer scratch, Nd4jLong scratchBytes);
+void nd4j_amd_execClipByGlobalNormDouble(Nd4jPointer *extraPointers, Nd4jPointer *dx, Nd4jPointer *dz,
+                                         Nd4jLong *offsets, int n, Nd4jLong total, double maxNorm, double *norm,
+                                         Nd4jPointer scratch, Nd4jLong scratchBytes);
+Nd4jLong nd4j_amd_scratchClipByGlobalNorm(Nd4jLong total);
+
 #if defined(__GNUC__)
 #pragma GCC visibility pop
 #endif

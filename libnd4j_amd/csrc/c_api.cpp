@@ -6,6 +6,7 @@
 
 #include "../../include/NativeOps.h"
 #include "../../include/nd4j_native_c.h"
+#include "native_training.h"
 #include "rng.h"
 #include "runtime.h"
 
@@ -294,6 +295,51 @@ void nd4j_amd_copyKernel(Nd4jPointer *extraPointers, void *dst, const void *src,
         nd4j_amd::launchCopy(s, dst, src, bytes);
         nd4j_amd::checkLaunch("copyKernel", s);
     });
+}
+
+// ---- the operators around a language model's matrix products ----------------------------------------------------------
+#define ND4J_C_TRAINING(SUFFIX, T, C)                                                                                             \
+    void nd4j_amd_execLayerNorm##SUFFIX(Nd4jPointer *e, T *x, Nd4jLong *xs, T *g, T *b, T *z, Nd4jLong *zs, C *m, C *i, double eps) { \
+        guardVoid([&] { nd4j_amd::layerNorm<T>(e, x, xs, g, b, z, zs, m, i, eps); });                                             \
+    }                                                                                                                             \
+    void nd4j_amd_execLayerNormBp##SUFFIX(Nd4jPointer *e, T *x, Nd4jLong *xs, T *g, C *m, C *i, T *dz, Nd4jLong *dzs, T *dx,       \
+                                          Nd4jLong *dxs, T *dg, T *db, Nd4jPointer w, Nd4jLong wb) {                              \
+        guardVoid([&] { nd4j_amd::layerNormBp<T>(e, x, xs, g, m, i, dz, dzs, dx, dxs, dg, db, w, wb); });                         \
+    }                                                                                                                             \
+    void nd4j_amd_execEmbedding##SUFFIX(Nd4jPointer *e, T *t, Nd4jLong *ts, Nd4jLong *k, Nd4jLong n, T *z, Nd4jLong *zs, double s) { \
+        guardVoid([&] { nd4j_amd::embedding<T>(e, t, ts, k, n, z, zs, s); });                                                     \
+    }                                                                                                                             \
+    void nd4j_amd_execEmbeddingBp##SUFFIX(Nd4jPointer *e, T *dz, Nd4jLong *dzs, Nd4jLong *k, Nd4jLong n, T *dt, Nd4jLong *dts,     \
+                                          double s, int acc, Nd4jPointer w, Nd4jLong wb) {                                        \
+        guardVoid([&] { nd4j_amd::embeddingBp<T>(e, dz, dzs, k, n, dt, dts, s, acc, w, wb); });                                   \
+    }                                                                                                                             \
+    void nd4j_amd_execTokenLogProbs##SUFFIX(Nd4jPointer *e, T *x, Nd4jLong *xs, Nd4jLong *t, C *lp, C *ls, C *h, int k,            \
+                                            Nd4jLong *top, C *tlp, Nd4jPointer w, Nd4jLong wb) {                                  \
+        guardVoid([&] { nd4j_amd::tokenLogProbs<T>(e, x, xs, t, lp, ls, h, k, top, tlp, w, wb); });                               \
+    }                                                                                                                             \
+    void nd4j_amd_execTokenLogProbsBp##SUFFIX(Nd4jPointer *e, T *x, Nd4jLong *xs, Nd4jLong *t, C *ls, C *h, C *dlp, C *dh, T *dx,  \
+                                              Nd4jLong *dxs) {                                                                    \
+        guardVoid([&] { nd4j_amd::tokenLogProbsBp<T>(e, x, xs, t, ls, h, dlp, dh, dx, dxs); });                                   \
+    }                                                                                                                             \
+    void nd4j_amd_execClipByGlobalNorm##SUFFIX(Nd4jPointer *e, Nd4jPointer *dx, Nd4jPointer *dz, Nd4jLong *o, int n, Nd4jLong t,   \
+                                               double most, C *norm, Nd4jPointer w, Nd4jLong wb) {                                \
+        guardVoid([&] { nd4j_amd::clipByGlobalNorm<T>(e, dx, dz, o, n, t, most, norm, w, wb); });                                 \
+    }
+ND4J_C_TRAINING(Float, float, float)
+ND4J_C_TRAINING(Half, float16, float)
+ND4J_C_TRAINING(Double, double, double)
+#undef ND4J_C_TRAINING
+Nd4jLong nd4j_amd_scratchLayerNormBp(Nd4jLong rows, Nd4jLong length) {
+    return guardRet<Nd4jLong>(0, [&] { return nd4j_amd::layerNormBpScratchBytes(rows, length); });
+}
+Nd4jLong nd4j_amd_scratchEmbeddingBp(Nd4jLong n, Nd4jLong vocabulary, Nd4jLong length) {
+    return guardRet<Nd4jLong>(0, [&] { return nd4j_amd::embeddingBpScratchBytes(n, vocabulary, length); });
+}
+Nd4jLong nd4j_amd_scratchTokenLogProbs(Nd4jLong rows, Nd4jLong length, int k) {
+    return guardRet<Nd4jLong>(0, [&] { return nd4j_amd::tokenLogProbsScratchBytes(rows, length, k); });
+}
+Nd4jLong nd4j_amd_scratchClipByGlobalNorm(Nd4jLong total) {
+    return guardRet<Nd4jLong>(0, [&] { return nd4j_amd::clipByGlobalNormScratchBytes(total); });
 }
 
 }  // extern "C"

@@ -1,0 +1,430 @@
+// Rows of a table looked up by token and scaled, and the table's gradient.
+//
+//   z[i] = scale * table[tokens[i]],   dTable[v] = scale * sum of dz[i] over the i with tokens[i] == v
+//
+// The gradient sorts the tokens (stably, so that equal tokens stay in the order of their positions), cuts the sorted list
+// into chunks of equal length, sums every run of equal tokens inside a chunk in a wave's registers, and joins the runs that
+// cross chunks in the chunks' order: no atomics on values, the same bits from every run, and a token that comes a hundred
+// thousand times is shared by many waves.  Sums are held in the compute type and rounded to the storage type once.
+#include "launch.h"
+#include "training.cuh"
+
+namespace nd4j_amd {
+namespace {
+
+using namespace tr;
+
+constexpr int kThreads = 256;
+
+// Any view: a thread per element.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) embeddingAnyKernel(const T *table, RowView tv, const Long *tokens, T *z, RowView zv,
+                                                               typename Compute<T>::type scale) {
+    typedef typename Compute<T>::type C;
+    const Long total = zv.rows * zv.length;
+    for (Long i = (Long)blockIdx.x * kThreads + threadIdx.x; i < total; i += (Long)gridDim.x * kThreads) {
+        const Long r = i / zv.length, c = i - r * zv.length, t = tokens[r];
+        C v = t < 0 ? (C)0 : notANumber<C>();
+        if (t >= 0 && t < tv.rows) v = toCompute(table[t * tv.row + c * tv.el]) * scale;
+        z[r * zv.row + c * zv.el] = fromCompute<T>(v);
+    }
+}
+
+// ---- sorting the tokens ----------------------------------------------------------------------------------------------
+// Least significant digit first, 8 bits a pass.  A block counts the digits of its tile (a multiple of kSubTile tokens), a
+// second launch places the tile's tokens behind those of lower digits and of the blocks before it.  At most kSortBlocks
+// tiles, so that the placing block can add up the counts of all blocks itself.
+constexpr int kSortBits = 8, kDigits = 1 << kSortBits;
+constexpr int kSortRounds = 4, kSubTile = kThreads * kSortRounds;
+constexpr int kSortBlocks = 256;
+
+// the sort key of token t: tokens outside the table come last, under the key `vocabulary`
+__device__ __forceinline__ unsigned keyOf(Long t, unsigned vocabulary) { return t >= 0 && t < (Long)vocabulary ? (unsigned)t : vocabulary; }
+
+__global__ void __launch_bounds__(kThreads) sortCountKernel(const Long *tokens, const unsigned *keys, unsigned n, unsigned vocabulary,
+                                                            unsigned tile, int shift, unsigned *counts, unsigned char *present) {
+    __shared__ unsigned local[kDigits];
+    local[threadIdx.x] = 0;
+    // the first pass clears the table of the tokens that occur (a whole number of words, see sortScratch)
+    if (present != nullptr)
+        for (size_t i = (size_t)blockIdx.x * kThreads + threadIdx.x; i < ((size_t)vocabulary + 4) / 4; i += (size_t)gridDim.x * kThreads)
+            reinterpret_cast<unsigned *>(present)[i] = 0u;
+    __syncthreads();
+    const unsigned long long first = (unsigned long long)blockIdx.x * tile;
+    const unsigned end = (unsigned)(first + tile < n ? first + tile : n);
+    for (unsigned i = (unsigned)first + threadIdx.x; i < end; i += kThreads) {
+        const unsigned key = keys != nullptr ? keys[i] : keyOf(tokens[i], vocabulary);
+        atomicAdd(&local[(key >> shift) & (kDigits - 1)], 1u);
+    }
+    __syncthreads();
+    counts[(size_t)blockIdx.x * kDigits + threadIdx.x] = local[threadIdx.x];
+}
+
+__global__ void __launch_bounds__(kThreads) sortPlaceKernel(const Long *tokens, const unsigned *keys, const unsigned *positions, unsigned n,
+                                                            unsigned vocabulary, unsigned tile, int shift, const unsigned *counts,
+                                                            unsigned *keysOut, unsigned *positionsOut, unsigned char *present) {
+    constexpr int WAVES = kThreads / kWaveLanes;
+    __shared__ unsigned starts[kDigits];
+    __shared__ unsigned waveCounts[WAVES][kDigits];
+    const int d = threadIdx.x, lane = threadIdx.x % kWaveLanes, wave = threadIdx.x / kWaveLanes;
+    // where this block's tokens of digit d begin: all tokens of lower digits, then those of digit d in the blocks before
+    unsigned before = 0, whole = 0;
+#pragma unroll 8
+    for (unsigned b = 0; b < gridDim.x; b++) {
+        const unsigned c = counts[(size_t)b * kDigits + d];
+        whole += c;
+        if (b < blockIdx.x) before += c;
+    }
+    starts[d] = whole;
+    __syncthreads();
+    for (int step = 1; step < kDigits; step <<= 1) {
+        const unsigned v = d >= step ? starts[d - step] : 0u;
+        __syncthreads();
+        starts[d] += v;
+        __syncthreads();
+    }
+    const unsigned mine = starts[d] - whole + before;
+    __syncthreads();
+    starts[d] = mine;
+    const unsigned long long first = (unsigned long long)blockIdx.x * tile;
+    const unsigned long long end = first + tile < n ? first + tile : n;
+    for (unsigned long long at = first; at < end; at += kSubTile) {
+#pragma unroll
+        for (int w = 0; w < WAVES; w++) waveCounts[w][d] = 0;
+        __syncthreads();
+        // a wave ranks kSortRounds x 64 consecutive tokens: behind the equal digits of its earlier rounds and lower lanes
+        unsigned key[kSortRounds], position[kSortRounds], rank[kSortRounds];
+        volatile unsigned *mineCounts = waveCounts[wave];
+#pragma unroll
+        for (int k = 0; k < kSortRounds; k++) {
+            const unsigned long long i = at + (unsigned)(wave * kSortRounds + k) * kWaveLanes + lane;
+            const bool live = i < end;
+            key[k] = 0;
+            position[k] = 0;
+            if (live) {
+                key[k] = keys != nullptr ? keys[i] : keyOf(tokens[i], vocabulary);
+                position[k] = positions != nullptr ? positions[i] : (unsigned)i;
+            }
+            const unsigned digit = (key[k] >> shift) & (kDigits - 1);
+            unsigned long long equal = __ballot(live);
+#pragma unroll
+            for (int bit = 0; bit < kSortBits; bit++) {
+                const unsigned long long set = __ballot((digit >> bit) & 1);
+                equal &= (digit >> bit) & 1 ? set : ~set;
+            }
+            const unsigned lower = __popcll(equal & ((1ull << lane) - 1));
+            rank[k] = 0;
+            if (live) {
+                const unsigned seen = mineCounts[digit];
+                rank[k] = seen + lower;
+                if (lower == 0) mineCounts[digit] = seen + (unsigned)__popcll(equal);
+            }
+            __builtin_amdgcn_wave_barrier();
+        }
+        __syncthreads();
+        unsigned running = starts[d];
+#pragma unroll
+        for (int w = 0; w < WAVES; w++) {
+            const unsigned c = waveCounts[w][d];
+            waveCounts[w][d] = running;
+            running += c;
+        }
+        starts[d] = running;
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kSortRounds; k++) {
+            const unsigned long long i = at + (unsigned)(wave * kSortRounds + k) * kWaveLanes + lane;
+            if (i < end) {
+                const unsigned to = waveCounts[wave][(key[k] >> shift) & (kDigits - 1)] + rank[k];
+                keysOut[to] = key[k];
+                positionsOut[to] = position[k];
+                if (present != nullptr) present[key[k]] = 1;  // (the table has a place for the key `vocabulary` too)
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// ---- summing ---------------------------------------------------------------------------------------------------------
+constexpr int kMostChunk = 64;   // a wave holds its chunk's keys and positions one a lane
+constexpr int kRowsInFlight = 8;
+
+// How the sorted list is cut, and where the columns are
+struct SumPlan {
+    unsigned n, vocabulary;
+    int chunk;
+    unsigned chunks;
+    Long length;
+    unsigned tiles;  // tiles of 64 vectors of columns
+};
+
+template <typename T, bool UNIT>
+__device__ __forceinline__ void loadColumns(const T *row, Long el, Long c0, Long length, Pack<T> &v) {
+    constexpr int N = Pack<T>::N;
+    if (UNIT && c0 + N <= length) {
+        v = loadPackAnywhere(row + c0);
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < N; e++) v.v[e] = fromCompute<T>((typename Compute<T>::type)0);
+#pragma unroll
+    for (int e = 0; e < N; e++)
+        if (c0 + e < length) v.v[e] = row[(c0 + e) * el];
+}
+
+template <typename T, bool UNIT>
+__device__ __forceinline__ void storeSum(T *row, Long el, Long c0, Long length, const typename Compute<T>::type *acc,
+                                         typename Compute<T>::type scale, bool accumulate) {
+    typedef typename Compute<T>::type C;
+    constexpr int N = Pack<T>::N;
+    if (UNIT && c0 + N <= length) {
+        Pack<T> o;
+        if (accumulate) o = loadPackAnywhere(row + c0);
+#pragma unroll
+        for (int e = 0; e < N; e++) o.v[e] = fromCompute<T>(acc[e] * scale + (accumulate ? toCompute(o.v[e]) : (C)0));
+        storePackAnywhere(row + c0, o);
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < N; e++)
+        if (c0 + e < length) {
+            T *p = row + (c0 + e) * el;
+            *p = fromCompute<T>(acc[e] * scale + (accumulate ? toCompute(*p) : (C)0));
+        }
+}
+
+// the row of partial sums of a chunk: which = 0 for a run that began in an earlier chunk, 1 for one that goes on behind it
+template <typename C> __device__ __forceinline__ C *partialRow(C *partial, unsigned chunk, int which, Long length) {
+    return partial + ((size_t)chunk * 2 + which) * length;
+}
+
+// A wave takes one chunk and one tile of columns.  The blocks behind those clear the rows of tokens that do not occur.
+template <typename T, bool UNIT>
+__global__ void __launch_bounds__(kThreads) embeddingBpSumKernel(const T *dz, RowView dzv, const unsigned *keys, const unsigned *positions,
+                                                                 SumPlan plan, T *dTable, RowView tv, typename Compute<T>::type scale,
+                                                                 int accumulate, typename Compute<T>::type *partial,
+                                                                 const unsigned char *present, unsigned sumBlocks) {
+    typedef typename Compute<T>::type C;
+    constexpr int N = Pack<T>::N, WAVES = kThreads / kWaveLanes;
+    const int lane = threadIdx.x % kWaveLanes, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWaveLanes);
+    if (blockIdx.x >= sumBlocks) {
+        C zero[N];
+#pragma unroll
+        for (int e = 0; e < N; e++) zero[e] = (C)0;
+        for (Long v = (Long)(blockIdx.x - sumBlocks) * WAVES + wave; v < (Long)plan.vocabulary; v += (Long)(gridDim.x - sumBlocks) * WAVES) {
+            if (present[v]) continue;
+            for (Long c = (Long)lane * N; c < plan.length; c += kWaveLanes * N)
+                storeSum<T, UNIT>(dTable + v * tv.row, tv.el, c, plan.length, zero, (C)0, false);
+        }
+        return;
+    }
+    const unsigned long long work = (unsigned long long)blockIdx.x * WAVES + wave;
+    if (work >= (unsigned long long)plan.chunks * plan.tiles) return;
+    const unsigned chunk = (unsigned)(work / plan.tiles), tile = (unsigned)(work % plan.tiles);
+    const Long c0 = ((Long)tile * kWaveLanes + lane) * N;
+    const unsigned long long first = (unsigned long long)chunk * plan.chunk;
+    const int count = (int)(first + plan.chunk <= plan.n ? plan.chunk : plan.n - first);
+    const int mineAt = lane < count ? lane : count - 1;
+    const unsigned myKey = keys[first + mineAt], myPosition = positions[first + mineAt];
+    const unsigned keyBefore = first > 0 ? keys[first - 1] : 0xffffffffu;
+    const unsigned keyBehind = first + count < plan.n ? keys[first + count] : 0xffffffffu;
+    C acc[N];
+#pragma unroll
+    for (int e = 0; e < N; e++) acc[e] = (C)0;
+    unsigned current = __builtin_amdgcn_readlane(myKey, 0);
+    bool fromBefore = current == keyBefore;
+    auto finish = [&](bool goesOn) {
+        if (current < plan.vocabulary && c0 < plan.length) {
+            if (fromBefore || goesOn) {
+                C *row = partialRow(partial, chunk, fromBefore ? 0 : 1, plan.length);
+#pragma unroll
+                for (int e = 0; e < N; e++)
+                    if (c0 + e < plan.length) row[c0 + e] = acc[e];
+            } else {
+                storeSum<T, UNIT>(dTable + (Long)current * tv.row, tv.el, c0, plan.length, acc, scale, accumulate != 0);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < N; e++) acc[e] = (C)0;
+        fromBefore = false;
+    };
+    for (int i = 0; i < count; i += kRowsInFlight) {
+        Pack<T> v[kRowsInFlight];
+#pragma unroll
+        for (int u = 0; u < kRowsInFlight; u++) {
+            const int at = i + u < count ? i + u : count - 1;
+            const unsigned p = __builtin_amdgcn_readlane(myPosition, at);
+            loadColumns<T, UNIT>(dz + (Long)p * dzv.row, dzv.el, c0, plan.length, v[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < kRowsInFlight; u++) {
+            if (i + u < count) {
+                const unsigned key = __builtin_amdgcn_readlane(myKey, i + u);
+                if (key != current) {
+                    finish(false);
+                    current = key;
+                }
+#pragma unroll
+                for (int e = 0; e < N; e++) acc[e] += toCompute(v[u].v[e]);
+            }
+        }
+    }
+    finish(current == keyBehind);
+}
+
+// A block takes one chunk and one tile: where a run begins in the chunk and goes on behind it, the run's partial sums are
+// added up in the order of the chunks (each wave every fourth of them, then the waves in order).
+template <typename T, bool UNIT>
+__global__ void __launch_bounds__(kThreads) embeddingBpJoinKernel(const unsigned *keys, SumPlan plan, T *dTable, RowView tv,
+                                                                  typename Compute<T>::type scale, int accumulate,
+                                                                  const typename Compute<T>::type *partial) {
+    typedef typename Compute<T>::type C;
+    constexpr int N = Pack<T>::N, WAVES = kThreads / kWaveLanes;
+    __shared__ C smem[WAVES][kWaveLanes][N];
+    const int lane = threadIdx.x % kWaveLanes, wave = threadIdx.x / kWaveLanes;
+    const unsigned chunk = (unsigned)(blockIdx.x / plan.tiles), tile = (unsigned)(blockIdx.x % plan.tiles);
+    const unsigned long long first = (unsigned long long)chunk * plan.chunk, behind = first + plan.chunk;
+    if (behind >= plan.n) return;
+    const unsigned key = keys[behind - 1];
+    if (key >= plan.vocabulary || keys[behind] != key) return;
+    if (first > 0 && keys[first] == key && keys[first - 1] == key) return;  // began earlier
+    unsigned long long low = behind + 1, high = plan.n;                     // the run ends in [low, high]
+    while (low < high) {
+        const unsigned long long mid = (low + high) >> 1;
+        if (keys[mid] == key) low = mid + 1;
+        else high = mid;
+    }
+    const unsigned lastChunk = (unsigned)((low - 1) / plan.chunk);
+    const Long c0 = ((Long)tile * kWaveLanes + lane) * N;
+    C acc[N];
+#pragma unroll
+    for (int e = 0; e < N; e++) acc[e] = (C)0;
+    for (unsigned c = chunk + wave; c <= lastChunk; c += WAVES) {
+        const C *row = partialRow(partial, c, c == chunk ? 1 : 0, plan.length);
+#pragma unroll
+        for (int e = 0; e < N; e++)
+            if (c0 + e < plan.length) acc[e] += row[c0 + e];
+    }
+#pragma unroll
+    for (int e = 0; e < N; e++) smem[wave][lane][e] = acc[e];
+    __syncthreads();
+    if (wave != 0 || c0 >= plan.length) return;
+#pragma unroll
+    for (int w = 1; w < WAVES; w++)
+#pragma unroll
+        for (int e = 0; e < N; e++) acc[e] += smem[w][lane][e];
+    storeSum<T, UNIT>(dTable + (Long)key * tv.row, tv.el, c0, plan.length, acc, scale, accumulate != 0);
+}
+
+// the chunk's length: long enough that few runs cross chunks, short enough that a few thousand waves share a small batch
+int chunkOf(Long n) { return n >= (1 << 18) ? kMostChunk : (n >= (1 << 14) ? 32 : 16); }
+
+size_t aligned(size_t bytes) { return (bytes + 255) & ~(size_t)255; }
+
+// the scratch's parts, in bytes from its start
+struct Layout {
+    size_t keys[2], positions[2], counts, present, partial, bytes;
+};
+Layout layoutOf(Long n, Long vocabulary, Long length) {
+    Layout l;
+    size_t at = 0;
+    auto take = [&](size_t bytes) { const size_t here = at; at += aligned(bytes); return here; };
+    for (int i = 0; i < 2; i++) {
+        l.keys[i] = take((size_t)n * 4);
+        l.positions[i] = take((size_t)n * 4);
+    }
+    l.counts = take((size_t)kSortBlocks * kDigits * 4);
+    l.present = take((size_t)vocabulary + 8);
+    const Long chunk = chunkOf(n), chunks = (n + chunk - 1) / chunk;
+    l.partial = take((size_t)chunks * 2 * length * sizeof(double));
+    l.bytes = at;
+    return l;
+}
+
+}  // namespace
+
+bool embeddingBpFits(Long n, Long length) {
+    const Long chunk = chunkOf(n), tiles = length / (kWaveLanes * Pack<double>::N) + 1;
+    return n / chunk + 1 < ((Long)1 << 30) / tiles;
+}
+size_t embeddingBpScratch(Long n, Long vocabulary, Long length) { return layoutOf(n, vocabulary, length).bytes; }
+
+template <typename T>
+void launchEmbedding(hipStream_t s, const T *table, const RowView &tv, const Long *tokens, T *z, const RowView &zv, double scale) {
+    typedef typename Compute<T>::type C;
+    ND4J_LAUNCH((embeddingAnyKernel<T>), dim3(gridFor(zv.rows * zv.length, kThreads, kGridCap)), dim3(kThreads), 0, s, table, tv, tokens, z, zv,
+                (C)scale);
+}
+
+template <typename T>
+void launchEmbeddingBp(hipStream_t s, const T *dz, const RowView &dzv, const Long *tokens, T *dTable, const RowView &tv, double scale,
+                       bool accumulate, void *scratch) {
+    typedef typename Compute<T>::type C;
+    const unsigned n = (unsigned)dzv.rows, vocabulary = (unsigned)tv.rows;
+    const Layout l = layoutOf(n, vocabulary, tv.length);
+    char *base = reinterpret_cast<char *>(scratch);
+    unsigned *keys[2], *positions[2];
+    for (int i = 0; i < 2; i++) {
+        keys[i] = reinterpret_cast<unsigned *>(base + l.keys[i]);
+        positions[i] = reinterpret_cast<unsigned *>(base + l.positions[i]);
+    }
+    unsigned *counts = reinterpret_cast<unsigned *>(base + l.counts);
+    unsigned char *present = reinterpret_cast<unsigned char *>(base + l.present);
+    C *partial = reinterpret_cast<C *>(base + l.partial);
+    int bits = 1;
+    while (bits < 32 && ((unsigned long long)1 << bits) <= vocabulary) bits++;  // the key `vocabulary` occurs too
+    // (a grid of no blocks is not a launch: without tokens one block clears the table of those that occur)
+    const unsigned tile = (unsigned)(((n + (unsigned long long)kSortBlocks * kSubTile - 1) / ((unsigned long long)kSortBlocks * kSubTile)) *
+                                     kSubTile);
+    const unsigned blocks = n == 0 ? 1 : (unsigned)(((unsigned long long)n + tile - 1) / tile);
+    const unsigned *from = nullptr, *fromPositions = nullptr;
+    int to = 0;
+    for (int shift = 0; shift < bits; shift += kSortBits) {
+        ND4J_LAUNCH(sortCountKernel, dim3(blocks), dim3(kThreads), 0, s, tokens, from, n, vocabulary, tile, shift, counts,
+                    shift == 0 ? present : nullptr);
+        if (n == 0) break;
+        ND4J_LAUNCH(sortPlaceKernel, dim3(blocks), dim3(kThreads), 0, s, tokens, from, fromPositions, n, vocabulary, tile, shift, counts,
+                    keys[to], positions[to], shift == 0 ? present : nullptr);
+        from = keys[to];
+        fromPositions = positions[to];
+        to ^= 1;
+    }
+    SumPlan plan;
+    plan.n = n;
+    plan.vocabulary = vocabulary;
+    plan.chunk = chunkOf(n);
+    plan.chunks = (unsigned)(((unsigned long long)n + plan.chunk - 1) / plan.chunk);
+    plan.length = tv.length;
+    plan.tiles = (unsigned)((tv.length + kWaveLanes * Pack<T>::N - 1) / (kWaveLanes * Pack<T>::N));
+    constexpr int WAVES = kThreads / kWaveLanes;
+    const unsigned sumBlocks = (unsigned)(((unsigned long long)plan.chunks * plan.tiles + WAVES - 1) / WAVES);
+    const unsigned clearBlocks = accumulate ? 0 : (unsigned)gridFor(vocabulary, WAVES, 1 << 16);
+    const bool unit = dzv.el == 1 && tv.el == 1;
+    if (sumBlocks + clearBlocks > 0) {
+        if (unit)
+            ND4J_LAUNCH((embeddingBpSumKernel<T, true>), dim3(sumBlocks + clearBlocks), dim3(kThreads), 0, s, dz, dzv, from, fromPositions, plan,
+                        dTable, tv, (C)scale, accumulate ? 1 : 0, partial, present, sumBlocks);
+        else
+            ND4J_LAUNCH((embeddingBpSumKernel<T, false>), dim3(sumBlocks + clearBlocks), dim3(kThreads), 0, s, dz, dzv, from, fromPositions, plan,
+                        dTable, tv, (C)scale, accumulate ? 1 : 0, partial, present, sumBlocks);
+    }
+    if (plan.chunks > 1) {
+        const unsigned joinBlocks = (plan.chunks - 1) * plan.tiles;
+        if (unit)
+            ND4J_LAUNCH((embeddingBpJoinKernel<T, true>), dim3(joinBlocks), dim3(kThreads), 0, s, from, plan, dTable, tv, (C)scale,
+                        accumulate ? 1 : 0, partial);
+        else
+            ND4J_LAUNCH((embeddingBpJoinKernel<T, false>), dim3(joinBlocks), dim3(kThreads), 0, s, from, plan, dTable, tv, (C)scale,
+                        accumulate ? 1 : 0, partial);
+    }
+}
+
+#define INST(T)                                                                                                                    \
+    template void launchEmbedding<T>(hipStream_t, const T *, const RowView &, const Long *, T *, const RowView &, double);           \
+    template void launchEmbeddingBp<T>(hipStream_t, const T *, const RowView &, const Long *, T *, const RowView &, double, bool, void *);
+INST(float)
+INST(float16)
+INST(double)
+#undef INST
+
+}  // namespace nd4j_amd

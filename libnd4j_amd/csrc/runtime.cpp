@@ -173,6 +173,33 @@ Workspace workspaceFor(hipStream_t s, size_t minBytes) {
 }
 
 namespace {
+std::map<std::pair<int, hipStream_t>, std::pair<void *, size_t> > gOperatorScratch;
+}  // namespace
+
+void *operatorScratchFor(hipStream_t s, size_t bytes) {
+    int dev = 0;
+    (void)hipGetDevice(&dev);
+    std::lock_guard<std::mutex> lock(gMutex);
+    std::pair<void *, size_t> &block = gOperatorScratch[std::make_pair(dev, s)];
+    if (block.first != nullptr && block.second >= bytes) return block.first;
+    size_t want = (size_t)1 << 20;  // powers of two, so that a growing batch does not allocate at every step
+    while (want < bytes) want <<= 1;
+    if (block.first != nullptr) {
+        (void)hipStreamSynchronize(s);  // earlier work on this stream may still use the old block
+        (void)hipFree(block.first);
+        block = std::pair<void *, size_t>(nullptr, 0);
+    }
+    void *p = nullptr;
+    hipError_t e = hipMalloc(&p, want);
+    if (e != hipSuccess) {
+        (void)hipGetLastError();
+        throwHip("operator scratch allocation", e);
+    }
+    block = std::make_pair(p, want);
+    return p;
+}
+
+namespace {
 struct PinnedSlot {
     void *block = nullptr;  // 256 bytes: value at 0, tagged words at 128, fault word at kPinnedFaultOffset
     unsigned ticket = 0;
@@ -326,21 +353,24 @@ void releaseStreamResources(hipStream_t s) {
     const auto key = std::make_pair(dev, s);
     Workspace w;
     w.ptr = nullptr;
-    void *slots = nullptr, *pinned = nullptr;
+    void *slots = nullptr, *pinned = nullptr, *scratch = nullptr;
     {
         std::lock_guard<std::mutex> lock(gMutex);
         auto wi = gWorkspaces.find(key);
         if (wi != gWorkspaces.end()) { w = wi->second; gWorkspaces.erase(wi); }
         auto fi = gFlatSlots.find(key);
         if (fi != gFlatSlots.end()) { slots = fi->second.block; gFlatSlots.erase(fi); }
+        auto si = gOperatorScratch.find(key);
+        if (si != gOperatorScratch.end()) { scratch = si->second.first; gOperatorScratch.erase(si); }
         auto pi = gPinnedSlots.find(key);
         if (pi != gPinnedSlots.end()) { pinned = pi->second.block; gPinnedSlots.erase(pi); }
     }
-    if (w.ptr == nullptr && slots == nullptr && pinned == nullptr) return;
+    if (w.ptr == nullptr && slots == nullptr && pinned == nullptr && scratch == nullptr) return;
     hipError_t e = hipStreamSynchronize(s);  // what is queued on the stream may still use them
     if (e != hipSuccess) throwHip("releaseStreamResources", e);
     if (w.ptr != nullptr) (void)hipFree(w.ptr);
     if (slots != nullptr) (void)hipFree(slots);
+    if (scratch != nullptr) (void)hipFree(scratch);
     if (pinned != nullptr) (void)hipHostFree(pinned);
 }
 

@@ -74,6 +74,9 @@ void reportUnknownOp(const char *family, int opNum);
 
 // Device scratch owned by the library, one per (device, stream), allocated on first use and kept.
 Workspace workspaceFor(hipStream_t s, size_t minBytes);
+// Device scratch of the operators of training.h, one block per (device, stream) beside the workspace above, so that
+// growing it never frees what a captured graph of another call holds.  Not for streams under capture.
+void *operatorScratchFor(hipStream_t s, size_t bytes);
 // Adds the slots, counter and ticket of the one-launch whole-array reduction to `w`: a block of device memory per
 // (device, stream) that only those reductions use, cleared when it is allocated.  Calls on one stream run one after the
 // other, so they may share it (one host thread per stream: the ticket source is not synchronised).

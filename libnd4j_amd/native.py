@@ -17,6 +17,7 @@ LIBRARY_PATH = os.path.join(_HERE, "libnd4j_amd.so")
 c_void_p = ctypes.c_void_p
 c_ll = ctypes.c_longlong
 c_int = ctypes.c_int
+c_double = ctypes.c_double
 
 _SUFFIX_RET = {"Float": ctypes.c_float, "Half": ctypes.c_float, "Double": ctypes.c_double}
 
@@ -58,6 +59,14 @@ _EXEC_SIGNATURES = {
     "nd4j_shuffle{S}": ([_P, _P, _P, _P, _P, c_int, _P, _P, _P], False),
     "nd4j_average{S}": ([_P, _P, _P, c_int, c_ll, c_int], False),
     "nd4j_accumulate{S}": ([_P, _P, _P, c_int, c_ll], False),
+    # operators around a language model's matrix products
+    "nd4j_amd_execLayerNorm{S}": ([_P, _P, _P, _P, _P, _P, _P, _P, _P, c_double], False),
+    "nd4j_amd_execLayerNormBp{S}": ([_P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P, c_ll], False),
+    "nd4j_amd_execEmbedding{S}": ([_P, _P, _P, _P, c_ll, _P, _P, c_double], False),
+    "nd4j_amd_execEmbeddingBp{S}": ([_P, _P, _P, _P, c_ll, _P, _P, c_double, c_int, _P, c_ll], False),
+    "nd4j_amd_execTokenLogProbs{S}": ([_P, _P, _P, _P, _P, _P, _P, c_int, _P, _P, _P, c_ll], False),
+    "nd4j_amd_execTokenLogProbsBp{S}": ([_P, _P, _P, _P, _P, _P, _P, _P, _P, _P], False),
+    "nd4j_amd_execClipByGlobalNorm{S}": ([_P, _P, _P, _P, c_int, c_ll, c_double, _P, _P, c_ll], False),
 }
 
 _PLAIN_SIGNATURES = {
@@ -116,6 +125,10 @@ _PLAIN_SIGNATURES = {
     "nd4j_amd_releaseStream": ([_P], None),
     "nd4j_amd_setSlotTicket": ([_P, ctypes.c_uint], None),
     "nd4j_amd_execReduceFloatNoAlloc": ([_P, c_int, _P, _P, _P, _P], None),
+    "nd4j_amd_scratchLayerNormBp": ([c_ll, c_ll], c_ll),
+    "nd4j_amd_scratchEmbeddingBp": ([c_ll, c_ll, c_ll], c_ll),
+    "nd4j_amd_scratchTokenLogProbs": ([c_ll, c_ll, c_int], c_ll),
+    "nd4j_amd_scratchClipByGlobalNorm": ([c_ll], c_ll),
 }
 
 
@@ -264,6 +277,15 @@ def _install_overloads():
         setattr(NativeOps, "execRandom" + S, mk("_random"))
         setattr(NativeOps, "execScalar" + S, mk("_scalar"))
         setattr(NativeOps, "execReduce3" + S, mk("_reduce3"))
+
+        # (these have one form each: looked up here once instead of by __getattr__ at every call, which takes longer than
+        # a small call does)
+        for template in _EXEC_SIGNATURES:
+            if template.startswith("nd4j_amd_"):
+                def direct(self, *args, _c=template.format(S=S)):
+                    return self._call(_c, *args)
+                direct.__name__ = template.format(S=S)[len("nd4j_"):]
+                setattr(NativeOps, direct.__name__, direct)
 
 
 _install_overloads()
