@@ -47,6 +47,93 @@ __global__ void __launch_bounds__(kRowThreads) layerNormAnyKernel(const T *x, Ro
     }
 }
 
+// Rows of contiguous elements that a team of TEAM lanes holds in its registers: PACKS vectors of 16 bytes a lane, and the
+// elements behind the last whole vector one a lane.  One read of x, one write of z; gain and bias stay in registers over
+// the team's rows (HELD).  Loads are unconditional (a vector that is not there re-reads the lane's first place, see `at`).
+template <typename T, int TEAM, int PACKS>
+__global__ void __launch_bounds__(TEAM > kRowThreads ? TEAM : kRowThreads)
+    layerNormRowsKernel(const T *x, RowView xv, const T *gain, const T *bias, T *z, RowView zv, typename Compute<T>::type *mean,
+                        typename Compute<T>::type *invStd, typename Compute<T>::type epsilon) {
+    typedef typename Compute<T>::type C;
+    constexpr int N = Pack<T>::N, THREADS = TEAM > kRowThreads ? TEAM : kRowThreads, TEAMS = THREADS / TEAM;
+    constexpr bool HELD = TEAM < 1024;  // a lane of a block of 1024 has 128 registers, which the row itself needs
+    __shared__ C smem[THREADS / kWaveLanes];
+    const int lane = threadIdx.x % TEAM;
+    const int length = (int)xv.length, vectors = length / N, rest = vectors * N + lane;
+    const C perLength = (C)1 / (C)length;
+    int at[PACKS];
+    Pack<T> g[PACKS], b[PACKS];
+    C gRest = (C)1, bRest = (C)0;
+#pragma unroll
+    for (int j = 0; j < PACKS; j++) {
+        at[j] = lane + j * TEAM < vectors ? (lane + j * TEAM) * N : 0;
+        if (HELD && vectors > 0 && gain != nullptr) g[j] = loadPackAnywhere(gain + at[j]);
+        if (HELD && vectors > 0 && bias != nullptr) b[j] = loadPackAnywhere(bias + at[j]);
+    }
+    if (rest < length) {
+        if (gain != nullptr) gRest = toCompute(gain[rest]);
+        if (bias != nullptr) bRest = toCompute(bias[rest]);
+    }
+    for (Long r0 = (Long)blockIdx.x * TEAMS; r0 < xv.rows; r0 += (Long)gridDim.x * TEAMS) {
+        const Long r = r0 + threadIdx.x / TEAM;
+        const bool live = r < xv.rows;
+        const T *xr = x + (live ? r : r0) * xv.row;
+        Pack<T> v[PACKS];
+        C vRest = (C)0;
+        if (vectors > 0) {
+#pragma unroll
+            for (int j = 0; j < PACKS; j++) v[j] = loadPackAnywhere(xr + at[j]);
+        }
+        if (rest < length) vRest = toCompute(xr[rest]);
+        C sum = vRest;
+#pragma unroll
+        for (int j = 0; j < PACKS; j++)
+            if (lane + j * TEAM < vectors) {
+#pragma unroll
+                for (int e = 0; e < N; e++) sum += toCompute(v[j].v[e]);
+            }
+        const C mu = teamAll<TEAM>(sum, Add(), smem) * perLength;
+        C squares = rest < length ? (vRest - mu) * (vRest - mu) : (C)0;
+#pragma unroll
+        for (int j = 0; j < PACKS; j++)
+            if (lane + j * TEAM < vectors) {
+#pragma unroll
+                for (int e = 0; e < N; e++) {
+                    const C d = toCompute(v[j].v[e]) - mu;
+                    squares += d * d;
+                }
+            }
+        const C s = (C)1 / sqrtOf(teamAll<TEAM>(squares, Add(), smem) * perLength + epsilon);
+        if (!live) continue;
+        if (lane == 0) {
+            if (mean != nullptr) mean[r] = mu;
+            if (invStd != nullptr) invStd[r] = s;
+        }
+        T *zr = z + r * zv.row;
+#pragma unroll
+        for (int j = 0; j < PACKS; j++)
+            if (lane + j * TEAM < vectors) {
+                Pack<T> o;
+                if (!HELD && gain != nullptr) g[j] = loadPackAnywhere(gain + at[j]);
+                if (!HELD && bias != nullptr) b[j] = loadPackAnywhere(bias + at[j]);
+#pragma unroll
+                for (int e = 0; e < N; e++) {
+                    C h = (toCompute(v[j].v[e]) - mu) * s;
+                    if (gain != nullptr) h *= toCompute(g[j].v[e]);
+                    if (bias != nullptr) h += toCompute(b[j].v[e]);
+                    o.v[e] = fromCompute<T>(h);
+                }
+                storePackAnywhere(zr + at[j], o);
+            }
+        if (rest < length) {
+            C h = (vRest - mu) * s;
+            if (gain != nullptr) h *= gRest;
+            if (bias != nullptr) h += bRest;
+            zr[rest] = fromCompute<T>(h);
+        }
+    }
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kRowThreads) layerNormBpAnyKernel(const T *x, RowView xv, const T *gain,
                                                                     const typename Compute<T>::type *mean,
@@ -73,6 +160,134 @@ __global__ void __launch_bounds__(kRowThreads) layerNormBpAnyKernel(const T *x, 
             const C h = (toCompute(xr[c * xv.el]) - mu) * s;
             dxr[c * dxv.el] = fromCompute<T>(s * (a - meanA - h * meanAH));
         }
+    }
+}
+
+// The backward pass of rows that a team holds in its registers (as in layerNormRowsKernel): dx, and the row's share of the
+// gain's and bias's gradients added onto sums that a lane keeps for its own columns over all rows of its team.  At the end
+// the teams of a block add theirs up in LDS, and partial[0 / 1][block][column] receives the block's sums (null: not wanted).
+template <int TEAM> constexpr int bpThreads() { return TEAM > 512 ? TEAM : 512; }
+template <typename T, int TEAM, int PACKS>
+__global__ void __launch_bounds__(bpThreads<TEAM>())
+    layerNormBpRowsKernel(const T *x, RowView xv, const T *gain, const typename Compute<T>::type *mean, const typename Compute<T>::type *invStd,
+                          const T *dz, RowView dzv, T *dx, RowView dxv, typename Compute<T>::type *partial) {
+    typedef typename Compute<T>::type C;
+    constexpr int N = Pack<T>::N, THREADS = bpThreads<TEAM>(), TEAMS = THREADS / TEAM;
+    extern __shared__ __align__(16) char dynamicLds[];
+    C *columns = reinterpret_cast<C *>(dynamicLds);  // [TEAMS / 2][columns of a row]
+    __shared__ C sums[2][THREADS / kWaveLanes];
+    const int lane = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
+    C *smem = sums[0] + threadIdx.x / TEAM * (TEAM / kWaveLanes), *smem2 = smem + THREADS / kWaveLanes;
+    const int length = (int)xv.length, vectors = length / N, rest = vectors * N + lane;
+    const C perLength = (C)1 / (C)length;
+    int at[PACKS];
+    Pack<T> g[PACKS];
+    C gainSum[PACKS][N], biasSum[PACKS][N], gainRest = (C)0, biasRest = (C)0, gRest = (C)1;
+#pragma unroll
+    for (int j = 0; j < PACKS; j++) {
+        at[j] = lane + j * TEAM < vectors ? (lane + j * TEAM) * N : 0;
+        if (vectors > 0 && gain != nullptr) g[j] = loadPackAnywhere(gain + at[j]);
+#pragma unroll
+        for (int e = 0; e < N; e++) gainSum[j][e] = biasSum[j][e] = (C)0;
+    }
+    if (rest < length && gain != nullptr) gRest = toCompute(gain[rest]);
+    for (Long r0 = (Long)blockIdx.x * TEAMS; r0 < xv.rows; r0 += (Long)gridDim.x * TEAMS) {
+        const bool live = r0 + team < xv.rows;
+        const Long r = live ? r0 + team : r0;
+        const T *xr = x + r * xv.row, *dzr = dz + r * dzv.row;
+        Pack<T> v[PACKS], d[PACKS];
+        C vRest = (C)0, dRest = (C)0;
+        if (vectors > 0) {
+#pragma unroll
+            for (int j = 0; j < PACKS; j++) {
+                v[j] = loadPackAnywhere(xr + at[j]);
+                d[j] = loadPackAnywhere(dzr + at[j]);
+            }
+        }
+        const C mu = mean[r], s = invStd[r];
+        if (rest < length) {
+            vRest = toCompute(xr[rest]);
+            dRest = toCompute(dzr[rest]);
+        }
+        C sumA = (C)0, sumAH = (C)0;
+        if (live) {
+#pragma unroll
+            for (int j = 0; j < PACKS; j++)
+                if (lane + j * TEAM < vectors) {
+#pragma unroll
+                    for (int e = 0; e < N; e++) {
+                        const C dd = toCompute(d[j].v[e]), h = (toCompute(v[j].v[e]) - mu) * s;
+                        const C a = gain != nullptr ? dd * toCompute(g[j].v[e]) : dd;
+                        sumA += a;
+                        sumAH += a * h;
+                        gainSum[j][e] += dd * h;
+                        biasSum[j][e] += dd;
+                    }
+                }
+            if (rest < length) {
+                const C h = (vRest - mu) * s, a = dRest * gRest;
+                sumA += a;
+                sumAH += a * h;
+                gainRest += dRest * h;
+                biasRest += dRest;
+            }
+        }
+        if (dx == nullptr) continue;
+        const C meanA = teamAll<TEAM>(sumA, Add(), smem) * perLength, meanAH = teamAll<TEAM>(sumAH, Add(), smem2) * perLength;
+        if (!live) continue;
+        T *dxr = dx + r * dxv.row;
+#pragma unroll
+        for (int j = 0; j < PACKS; j++)
+            if (lane + j * TEAM < vectors) {
+                Pack<T> o;
+#pragma unroll
+                for (int e = 0; e < N; e++) {
+                    const C h = (toCompute(v[j].v[e]) - mu) * s;
+                    C a = toCompute(d[j].v[e]);
+                    if (gain != nullptr) a *= toCompute(g[j].v[e]);
+                    o.v[e] = fromCompute<T>(s * (a - meanA - h * meanAH));
+                }
+                storePackAnywhere(dxr + at[j], o);
+            }
+        if (rest < length) dxr[rest] = fromCompute<T>(s * (dRest * gRest - meanA - (vRest - mu) * s * meanAH));
+    }
+    if (partial == nullptr) return;
+#pragma unroll
+    for (int which = 0; which < 2; which++) {
+        // the upper half of the teams hands its sums to the lower half, until the first team has them all
+#pragma unroll
+        for (int half = TEAMS / 2; half >= 1; half /= 2) {
+            C *shared = columns + (size_t)(team % half) * length;
+            __syncthreads();
+            if (team >= half && team < 2 * half) {
+#pragma unroll
+                for (int j = 0; j < PACKS; j++)
+                    if (lane + j * TEAM < vectors) {
+#pragma unroll
+                        for (int e = 0; e < N; e++) shared[at[j] + e] = which == 0 ? gainSum[j][e] : biasSum[j][e];
+                    }
+                if (rest < length) shared[rest] = which == 0 ? gainRest : biasRest;
+            }
+            __syncthreads();
+            if (team < half) {
+#pragma unroll
+                for (int j = 0; j < PACKS; j++)
+                    if (lane + j * TEAM < vectors) {
+#pragma unroll
+                        for (int e = 0; e < N; e++) (which == 0 ? gainSum[j][e] : biasSum[j][e]) += shared[at[j] + e];
+                    }
+                if (rest < length) (which == 0 ? gainRest : biasRest) += shared[rest];
+            }
+        }
+        if (team > 0) continue;
+        C *out = partial + ((size_t)which * gridDim.x + blockIdx.x) * length;
+#pragma unroll
+        for (int j = 0; j < PACKS; j++)
+            if (lane + j * TEAM < vectors) {
+#pragma unroll
+                for (int e = 0; e < N; e++) out[at[j] + e] = which == 0 ? gainSum[j][e] : biasSum[j][e];
+            }
+        if (rest < length) out[rest] = which == 0 ? gainRest : biasRest;
     }
 }
 
@@ -109,28 +324,32 @@ __global__ void __launch_bounds__(kRowThreads) layerNormBpColumnsKernel(const T 
     }
 }
 
+// A block takes 32 columns: its 32 half waves share the splits, then add up in LDS in a fixed order.
+constexpr int kFinishThreads = 1024, kFinishColumns = 32, kFinishGroups = kFinishThreads / kFinishColumns;
 template <typename T>
-__global__ void __launch_bounds__(kRowThreads) layerNormBpFinishKernel(const typename Compute<T>::type *partial, int splits, Long length, T *dGain,
-                                                                       T *dBias) {
+__global__ void __launch_bounds__(kFinishThreads) layerNormBpFinishKernel(const typename Compute<T>::type *partial, int splits, Long length,
+                                                                          T *dGain, T *dBias) {
     typedef typename Compute<T>::type C;
-    constexpr int WAVES = kRowThreads / kWaveLanes;
-    __shared__ C smem[WAVES][kWaveLanes];
-    const int lane = threadIdx.x % kWaveLanes, wave = threadIdx.x / kWaveLanes;
+    __shared__ C smem[kFinishGroups][kFinishColumns + 1];
+    const int column = threadIdx.x % kFinishColumns, group = threadIdx.x / kFinishColumns;
     const int which = blockIdx.y;
     T *out = which == 0 ? dGain : dBias;
     if (out == nullptr) return;
-    const Long tiles = (length + kWaveLanes - 1) / kWaveLanes;
+    const Long tiles = (length + kFinishColumns - 1) / kFinishColumns;
     for (Long tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-        const Long c = tile * kWaveLanes + lane;
+        const Long c = tile * kFinishColumns + column;
         C sum = (C)0;
-        if (c < length)
-            for (int s = wave; s < splits; s += WAVES) sum += partial[((Long)which * splits + s) * length + c];
+        if (c < length) {
+            const C *from = partial + (size_t)which * splits * length + c;
+#pragma unroll 4
+            for (int s = group; s < splits; s += kFinishGroups) sum += from[(size_t)s * length];
+        }
         __syncthreads();
-        smem[wave][lane] = sum;
+        smem[group][column] = sum;
         __syncthreads();
-        if (wave == 0 && c < length) {
+        if (group == 0 && c < length) {
 #pragma unroll
-            for (int w = 1; w < WAVES; w++) sum += smem[w][lane];
+            for (int k = 1; k < kFinishGroups; k++) sum += smem[k][column];
             out[c] = fromCompute<T>(sum);
         }
     }
@@ -148,13 +367,57 @@ unsigned gridOf(Long blocks) { return (unsigned)(blocks < 1 ? 1 : (blocks > (1 <
 
 }  // namespace
 
-size_t layerNormBpScratch(Long rows, Long length) { return (size_t)2 * columnSplits(rows, length) * length * sizeof(double); }
+// The blocks of the register kernel: two a compute unit, which is what its registers and LDS leave room for
+constexpr int kBpBlocks = 512;
+
+size_t layerNormBpScratch(Long rows, Long length) {
+    const Long any = columnSplits(rows, length), held = rows < kBpBlocks ? (rows < 1 ? 1 : rows) : kBpBlocks;
+    return (size_t)2 * (any > held ? any : held) * length * sizeof(double);
+}
+
+template <typename T, int TEAM, int PACKS>
+void runRows(hipStream_t s, const T *x, const RowView &xv, const T *gain, const T *bias, T *z, const RowView &zv,
+             typename Compute<T>::type *mean, typename Compute<T>::type *invStd, double epsilon) {
+    typedef typename Compute<T>::type C;
+    constexpr int THREADS = TEAM > kRowThreads ? TEAM : kRowThreads, TEAMS = THREADS / TEAM;
+    const unsigned blocks = (unsigned)gridFor(xv.rows, TEAMS, kGridCap * kRowThreads / THREADS);
+    ND4J_LAUNCH((layerNormRowsKernel<T, TEAM, PACKS>), dim3(blocks), dim3(THREADS), 0, s, x, xv, gain, bias, z, zv, mean, invStd, (C)epsilon);
+}
 
 template <typename T>
 void launchLayerNorm(hipStream_t s, const T *x, const RowView &xv, const T *gain, const T *bias, T *z, const RowView &zv,
                      typename Compute<T>::type *mean, typename Compute<T>::type *invStd, double epsilon) {
     typedef typename Compute<T>::type C;
+    if (xv.el == 1 && zv.el == 1) {
+        const Long vectors = xv.length / Pack<T>::N;
+#define ROWS(TEAM, PACKS) return runRows<T, TEAM, PACKS>(s, x, xv, gain, bias, z, zv, mean, invStd, epsilon)
+        if (vectors <= 16) ROWS(16, 1);
+        if (vectors <= 32) ROWS(16, 2);
+        if (vectors <= 64) ROWS(64, 1);
+        if (vectors <= 128) ROWS(64, 2);
+        if (vectors <= 256) ROWS(64, 4);
+        if (vectors <= 512) ROWS(256, 2);
+        if (vectors <= 1024) ROWS(256, 4);
+        if (vectors <= 2048) ROWS(1024, 2);
+        if constexpr (sizeof(T) > 2)  // (32 halves a lane do not fit its 128 registers as floats)
+            if (vectors <= 4096) ROWS(1024, 4);
+#undef ROWS
+    }
     ND4J_LAUNCH((layerNormAnyKernel<T>), dim3(gridOf(xv.rows)), dim3(kRowThreads), 0, s, x, xv, gain, bias, z, zv, mean, invStd, (C)epsilon);
+}
+
+// runs the register kernel and returns the number of its blocks
+template <typename T, int TEAM, int PACKS>
+int runBpRows(hipStream_t s, const T *x, const RowView &xv, const T *gain, const typename Compute<T>::type *mean,
+              const typename Compute<T>::type *invStd, const T *dz, const RowView &dzv, T *dx, const RowView &dxv,
+              typename Compute<T>::type *partial) {
+    typedef typename Compute<T>::type C;
+    constexpr int THREADS = bpThreads<TEAM>(), TEAMS = THREADS / TEAM;
+    const int blocks = gridFor(xv.rows, TEAMS, kBpBlocks);
+    const size_t lds = TEAMS > 1 && partial != nullptr ? (size_t)(TEAMS / 2) * xv.length * sizeof(C) : 0;
+    ND4J_LAUNCH((layerNormBpRowsKernel<T, TEAM, PACKS>), dim3(blocks), dim3(THREADS), lds, s, x, xv, gain, mean, invStd, dz, dzv, dx, dxv,
+                partial);
+    return blocks;
 }
 
 template <typename T>
@@ -162,17 +425,33 @@ void launchLayerNormBp(hipStream_t s, const T *x, const RowView &xv, const T *ga
                        const typename Compute<T>::type *invStd, const T *dz, const RowView &dzv, T *dx, const RowView &dxv, T *dGain,
                        T *dBias, void *scratch) {
     typedef typename Compute<T>::type C;
-    if (dGain != nullptr || dBias != nullptr) {
-        // before dx is written, which may lie where dz or x does
-        const int splits = columnSplits(xv.rows, xv.length);
-        const Long tiles = (xv.length + kWaveLanes - 1) / kWaveLanes;
-        C *partial = reinterpret_cast<C *>(scratch);
-        ND4J_LAUNCH((layerNormBpColumnsKernel<T>), dim3(gridOf(tiles * splits)), dim3(kRowThreads), 0, s, x, xv, mean, invStd, dz, dzv, partial,
-                    splits);
-        ND4J_LAUNCH((layerNormBpFinishKernel<T>), dim3(gridOf(tiles), 2), dim3(kRowThreads), 0, s, partial, splits, xv.length, dGain, dBias);
+    const bool columns = dGain != nullptr || dBias != nullptr;
+    C *partial = columns ? reinterpret_cast<C *>(scratch) : nullptr;
+    int splits = 0;
+    if (xv.el == 1 && dzv.el == 1 && dxv.el == 1 && xv.rows > 0) {
+        const Long vectors = xv.length / Pack<T>::N;
+#define ROWS(TEAM, PACKS) splits = runBpRows<T, TEAM, PACKS>(s, x, xv, gain, mean, invStd, dz, dzv, dx, dxv, partial)
+        if (vectors <= 16) ROWS(16, 1);
+        else if (vectors <= 64) ROWS(64, 1);
+        else if (vectors <= 128) ROWS(64, 2);
+        else if (vectors <= 256) ROWS(64, 4);
+        else if (vectors <= 512) ROWS(256, 2);
+        else if (vectors <= 1024) ROWS(256, 4);
+        else if (vectors <= 2048) ROWS(1024, 2);
+#undef ROWS
     }
-    if (dx != nullptr && xv.rows > 0)
-        ND4J_LAUNCH((layerNormBpAnyKernel<T>), dim3(gridOf(xv.rows)), dim3(kRowThreads), 0, s, x, xv, gain, mean, invStd, dz, dzv, dx, dxv);
+    if (splits == 0) {  // any other view: the columns first, since dx may lie where dz or x does
+        splits = columnSplits(xv.rows, xv.length);
+        const Long tiles = (xv.length + kWaveLanes - 1) / kWaveLanes;
+        if (columns)
+            ND4J_LAUNCH((layerNormBpColumnsKernel<T>), dim3(gridOf(tiles * splits)), dim3(kRowThreads), 0, s, x, xv, mean, invStd, dz, dzv, partial,
+                        splits);
+        if (dx != nullptr && xv.rows > 0)
+            ND4J_LAUNCH((layerNormBpAnyKernel<T>), dim3(gridOf(xv.rows)), dim3(kRowThreads), 0, s, x, xv, gain, mean, invStd, dz, dzv, dx, dxv);
+    }
+    if (columns)
+        ND4J_LAUNCH((layerNormBpFinishKernel<T>), dim3(gridOf((xv.length + kFinishColumns - 1) / kFinishColumns), 2), dim3(kFinishThreads), 0, s,
+                    partial, splits, xv.length, dGain, dBias);
 }
 
 #define INST(T)                                                                                                                       \

@@ -11,24 +11,6 @@ namespace tr {
 
 static constexpr int kWaveLanes = 64;
 
-template <typename C> __device__ __forceinline__ C laneFrom(C v, int lane) {
-    static_assert(sizeof(C) % 4 == 0, "a multiple of 4 bytes");
-    constexpr int W = sizeof(C) / 4;
-    struct Words { int w[W]; };
-    Words in = __builtin_bit_cast(Words, v), out;
-#pragma unroll
-    for (int i = 0; i < W; i++) out.w[i] = __shfl(in.w[i], lane);
-    return __builtin_bit_cast(C, out);
-}
-template <typename C> __device__ __forceinline__ C laneXorOf(C v, int mask) {
-    static_assert(sizeof(C) % 4 == 0, "a multiple of 4 bytes");
-    constexpr int W = sizeof(C) / 4;
-    struct Words { int w[W]; };
-    Words in = __builtin_bit_cast(Words, v), out;
-#pragma unroll
-    for (int i = 0; i < W; i++) out.w[i] = __shfl_xor(in.w[i], mask);
-    return __builtin_bit_cast(C, out);
-}
 struct Add {
     template <typename C> __device__ __forceinline__ C operator()(C a, C b) const { return a + b; }
 };
@@ -36,24 +18,68 @@ struct Largest {  // a NaN loses against anything
     __device__ __forceinline__ float operator()(float a, float b) const { return ::fmaxf(a, b); }
     __device__ __forceinline__ double operator()(double a, double b) const { return ::fmax(a, b); }
 };
-// every lane of a group of LANES neighbouring lanes gets the group's value
-template <int LANES, class Op, typename C> __device__ __forceinline__ C waveAll(C v, Op op) {
+// The value of another lane of the same 16, by the data path of the vector unit itself (a shuffle goes through LDS).
+// CTRL: 0xb1 and 0x4e swap neighbours and pairs, 0x141 and 0x140 mirror 8 and 16 lanes.
+template <int CTRL, typename C> __device__ __forceinline__ C laneDpp(C v) {
+    constexpr int W = sizeof(C) / 4;
+    struct Words { int w[W]; };
+    Words in = __builtin_bit_cast(Words, v), out;
 #pragma unroll
-    for (int d = LANES / 2; d >= 1; d >>= 1) v = op(v, laneXorOf(v, d));
+    for (int i = 0; i < W; i++) out.w[i] = __builtin_amdgcn_update_dpp(in.w[i], in.w[i], CTRL, 0xf, 0xf, false);
+    return __builtin_bit_cast(C, out);
+}
+// Lane i's value beside that of the lane 16 (32) away: every lane gets both values of its pair, in the same order.
+template <int APART, typename C> __device__ __forceinline__ void lanePair(C v, C &a, C &b) {
+    static_assert(APART == 16 || APART == 32, "rows or halves of a wave");
+    constexpr int W = sizeof(C) / 4;
+    struct Words { unsigned w[W]; };
+    Words in = __builtin_bit_cast(Words, v), x, y;
+#pragma unroll
+    for (int i = 0; i < W; i++) {
+        auto both = APART == 16 ? __builtin_amdgcn_permlane16_swap(in.w[i], in.w[i], false, false)
+                                : __builtin_amdgcn_permlane32_swap(in.w[i], in.w[i], false, false);
+        x.w[i] = both[0];
+        y.w[i] = both[1];
+    }
+    a = __builtin_bit_cast(C, x);
+    b = __builtin_bit_cast(C, y);
+}
+// every lane of a group of LANES neighbouring lanes gets the group's value; op commutes
+template <int LANES, class Op, typename C> __device__ __forceinline__ C waveAll(C v, Op op) {
+    static_assert(LANES == 16 || LANES == 32 || LANES == 64, "whole rows of a wave");
+    v = op(v, laneDpp<0xb1>(v));
+    v = op(v, laneDpp<0x4e>(v));
+    v = op(v, laneDpp<0x141>(v));
+    v = op(v, laneDpp<0x140>(v));
+    C a, b;
+    if (LANES >= 32) {
+        lanePair<16>(v, a, b);
+        v = op(a, b);
+    }
+    if (LANES == 64) {
+        lanePair<32>(v, a, b);
+        v = op(a, b);
+    }
     return v;
 }
-// every thread of a block of THREADS threads gets the block's value; smem: one C per wave, free for reuse behind the
-// next barrier the caller passes
+// every thread of a team of THREADS neighbouring threads gets the team's value (all teams of the block call it together);
+// smem: one C per wave of the team, free for reuse behind the next barrier the caller passes
 template <int THREADS, class Op, typename C> __device__ __forceinline__ C blockAll(C v, Op op, C *smem) {
     v = waveAll<kWaveLanes>(v, op);
     if (THREADS == kWaveLanes) return v;
     __syncthreads();  // smem may still be read from the round before
-    if (threadIdx.x % kWaveLanes == 0) smem[threadIdx.x / kWaveLanes] = v;
+    if (threadIdx.x % kWaveLanes == 0) smem[threadIdx.x % THREADS / kWaveLanes] = v;
     __syncthreads();
     v = smem[0];
 #pragma unroll
     for (int w = 1; w < THREADS / kWaveLanes; w++) v = op(v, smem[w]);
     return v;
+}
+
+// the same for teams of 16, 32 or 64 lanes or whole blocks
+template <int TEAM, class Op, typename C> __device__ __forceinline__ C teamAll(C v, Op op, C *smem) {
+    if constexpr (TEAM <= kWaveLanes) return waveAll<TEAM>(v, op);
+    else return blockAll<TEAM>(v, op, smem);
 }
 
 __device__ __forceinline__ float sqrtOf(float v) { return ::sqrtf(v); }
