@@ -2,8 +2,15 @@
 //
 //   norm = sqrt(sum of g^2),  f = maxNorm / norm where maxNorm < norm < infinity, else 1,  out = f g
 //
-// The tensors' elements count as one range of `total` elements; a block takes the same part of it in both launches.  Squares
-// are summed in double: the square of any float is finite there, and the order of the sum does not show in the result's type.
+// The tensors' elements count as one range, cut into tiles that the blocks take in turn, from the range's start for the norm
+// and from its end for the result, so that what the first launch read last - the most that the last-level cache holds of
+// it - is read first by the second.  A tile inside one tensor is walked in vectors (unaligned ones: tensors may begin
+// anywhere), a tile that holds ends of tensors vector by vector too, every thread looking the tensor up for its own
+// (a vector across tensors goes element by element): a thousand tensors of ten elements cost no more launches than one of
+// ten thousand.
+//
+// Squares are summed in double: the square of any float is finite there, and the order of the sum does not show in the
+// result's type.  (Squares of halves are exact in float; eight of them are added there first.)
 #include "launch.h"
 #include "training.cuh"
 
@@ -12,57 +19,161 @@ namespace {
 
 using namespace tr;
 
-constexpr int kNormThreads = 256;
-constexpr int kNormBlocks = 1024;
+constexpr int kNormThreads = 512;
+constexpr int kNormBlocks = 1024;  // four a compute unit: all waves that it holds
 
 // The elements of the range: what the offsets say, and no more than the host was told.
 __device__ __forceinline__ Long wholeLength(const Long *offsets, int n, Long total) {
     if (n == 0) return 0;
     return offsets[n] < total ? offsets[n] : total;
 }
-// The tensor i with offsets[i] <= at < offsets[i + 1] (at < offsets[n]); 0 where at lies before the first.
-__device__ __forceinline__ int tensorAt(const Long *offsets, int n, Long at) {
-    int low = 0, high = n;
-    while (high - low > 1) {
-        const int mid = (low + high) >> 1;
+// The tensor i with offsets[i] <= at < offsets[i + 1], known to lie in low .. high (low where at lies before the first).
+__device__ __forceinline__ int tensorAt(const Long *offsets, int low, int high, Long at) {
+    while (high > low) {
+        const int mid = (low + high + 1) >> 1;
         if (offsets[mid] <= at) low = mid;
-        else high = mid;
+        else high = mid - 1;
     }
     return low;
 }
 
+// Searches wait for one offset after the other, and for the tensor's address then, a trip to the cache each: of up to
+// kStaged - 1 tensors a block copies both tables into LDS first.
+constexpr int kStaged = 1024;
+template <typename T> struct Tables {
+    const Long *offsets;
+    const T *const *in;
+};
 template <typename T>
-__global__ void __launch_bounds__(kNormThreads) squaresKernel(const T *const *in, const Long *offsets, int n, Long total, double *partial) {
+__device__ __forceinline__ Tables<T> stagedTables(const T *const *in, const Long *offsets, int n, Long *stagedOffsets, const T **stagedIn) {
+    Tables<T> t;
+    t.offsets = offsets;
+    t.in = in;
+    if (n >= kStaged || n == 0) return t;
+    for (int i = threadIdx.x; i <= n; i += kNormThreads) {
+        stagedOffsets[i] = offsets[i];
+        if (i < n) stagedIn[i] = in[i];
+    }
+    __syncthreads();
+    t.offsets = stagedOffsets;
+    t.in = stagedIn;
+    return t;
+}
+
+template <typename T> __device__ __forceinline__ double squaresOf(const Pack<T> &v) {
+    constexpr int N = Pack<T>::N;
+    if constexpr (sizeof(T) == 2) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int e = 0; e < N; e++) sum += toCompute(v.v[e]) * toCompute(v.v[e]);
+        return (double)sum;
+    } else {
+        double sum = 0.0;
+#pragma unroll
+        for (int e = 0; e < N; e++) sum = __builtin_fma((double)toCompute(v.v[e]), (double)toCompute(v.v[e]), sum);
+        return sum;
+    }
+}
+
+template <typename T, int VECTORS>
+__global__ void __launch_bounds__(kNormThreads) squaresKernel(const T *const *givenIn, const Long *givenOffsets, int n, Long total, double *partial) {
+    constexpr int N = Pack<T>::N;
+    constexpr Long tile = (Long)kNormThreads * VECTORS * N;
     __shared__ double smem[kNormThreads / kWaveLanes];
+    __shared__ Long stagedOffsets[kStaged];
+    __shared__ const T *stagedIn[kStaged];
+    const Tables<T> tables = stagedTables<T>(givenIn, givenOffsets, n, stagedOffsets, stagedIn);
+    const Long *offsets = tables.offsets;
+    const T *const *in = tables.in;
+    const Long whole = wholeLength(offsets, n, total);
     double sum = 0.0;
-    const Long end = wholeLength(offsets, n, total);
-    for (Long i = (Long)blockIdx.x * kNormThreads + threadIdx.x; i < end; i += (Long)gridDim.x * kNormThreads) {
-        const int k = tensorAt(offsets, n, i);
-        if (i < offsets[k]) continue;
-        const double v = (double)toCompute(in[k][i - offsets[k]]);
-        sum += v * v;
+    int low = 0;  // (the tiles of a block ascend)
+    for (Long t = (Long)blockIdx.x * tile; t < whole; t += (Long)gridDim.x * tile) {
+        const Long end = t + tile < whole ? t + tile : whole;
+        low = tensorAt(offsets, low, n - 1, t);
+        const int high = end <= offsets[low + 1] ? low : tensorAt(offsets, low, n - 1, end - 1);
+        if (low == high && end - t == tile && t >= offsets[low]) {
+            const T *from = in[low] + (t - offsets[low]) + threadIdx.x * N;
+            Pack<T> v[VECTORS];
+#pragma unroll
+            for (int j = 0; j < VECTORS; j++) v[j] = loadPackAnywhere(from + j * (kNormThreads * N));
+#pragma unroll
+            for (int j = 0; j < VECTORS; j++) sum += squaresOf<T>(v[j]);
+        } else {
+            for (Long i = t + threadIdx.x * N; i < end; i += kNormThreads * N) {
+                int k = tensorAt(offsets, low, high, i);
+                if (i >= offsets[k] && i + N <= end && i + N <= offsets[k + 1]) {
+                    sum += squaresOf<T>(loadPackAnywhere(in[k] + (i - offsets[k])));
+                    continue;
+                }
+                for (Long j = i; j < i + N && j < end; j++) {
+                    while (k < high && j >= offsets[k + 1]) k++;
+                    if (j < offsets[k]) continue;
+                    const double v = (double)toCompute(in[k][j - offsets[k]]);
+                    sum += v * v;
+                }
+            }
+        }
     }
     sum = blockAll<kNormThreads>(sum, Add(), smem);
     if (threadIdx.x == 0) partial[blockIdx.x] = sum;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kNormThreads) clipKernel(const T *const *in, T *const *out, const Long *offsets, int n, Long total,
+template <typename T, int VECTORS>
+__global__ void __launch_bounds__(kNormThreads) clipKernel(const T *const *givenIn, T *const *out, const Long *givenOffsets, int n, Long total,
                                                            double maxNorm, typename Compute<T>::type *norm, const double *partial, int parts) {
     typedef typename Compute<T>::type C;
+    constexpr int N = Pack<T>::N;
+    constexpr Long tile = (Long)kNormThreads * VECTORS * N;
     __shared__ double smem[kNormThreads / kWaveLanes];
+    __shared__ Long stagedOffsets[kStaged];
+    __shared__ const T *stagedIn[kStaged];
+    const Tables<T> tables = stagedTables<T>(givenIn, givenOffsets, n, stagedOffsets, stagedIn);
+    const Long *offsets = tables.offsets;
+    const T *const *in = tables.in;
     double sum = 0.0;
     for (int i = threadIdx.x; i < parts; i += kNormThreads) sum += partial[i];
-    const double whole = ::sqrt(blockAll<kNormThreads>(sum, Add(), smem));
-    if (norm != nullptr && blockIdx.x == 0 && threadIdx.x == 0) norm[0] = (C)whole;
+    const double value = ::sqrt(blockAll<kNormThreads>(sum, Add(), smem));
+    if (norm != nullptr && blockIdx.x == 0 && threadIdx.x == 0) norm[0] = (C)value;
     if (out == nullptr) return;
     // (a NaN norm compares false, so it leaves the factor at 1 like one that is infinite)
-    const C factor = whole > maxNorm && whole < infinite<double>() ? (C)(maxNorm / whole) : (C)1;
-    const Long end = wholeLength(offsets, n, total);
-    for (Long i = (Long)blockIdx.x * kNormThreads + threadIdx.x; i < end; i += (Long)gridDim.x * kNormThreads) {
-        const int k = tensorAt(offsets, n, i);
-        if (i < offsets[k]) continue;
-        out[k][i - offsets[k]] = fromCompute<T>(toCompute(in[k][i - offsets[k]]) * factor);
+    const C factor = value > maxNorm && value < infinite<double>() ? (C)(maxNorm / value) : (C)1;
+    const Long whole = wholeLength(offsets, n, total);
+    int last = n - 1;  // (the tiles of a block descend)
+    for (Long left = (whole + tile - 1) / tile - blockIdx.x; left > 0; left -= gridDim.x) {
+        const Long t = (left - 1) * tile, end = t + tile < whole ? t + tile : whole;
+        const int low = tensorAt(offsets, 0, last, t), high = end <= offsets[low + 1] ? low : tensorAt(offsets, low, last, end - 1);
+        last = low;
+        if (low == high && end - t == tile && t >= offsets[low]) {
+            const Long at = (t - offsets[low]) + threadIdx.x * N;
+            const T *from = in[low] + at;
+            T *to = out[low] + at;
+            Pack<T> v[VECTORS];
+#pragma unroll
+            for (int j = 0; j < VECTORS; j++) v[j] = streamPackAnywhere(from + j * (kNormThreads * N));
+#pragma unroll
+            for (int j = 0; j < VECTORS; j++) {
+#pragma unroll
+                for (int e = 0; e < N; e++) v[j].v[e] = fromCompute<T>(toCompute(v[j].v[e]) * factor);
+                streamPackAnywhere(to + j * (kNormThreads * N), v[j]);
+            }
+        } else {
+            for (Long i = t + threadIdx.x * N; i < end; i += kNormThreads * N) {
+                int k = tensorAt(offsets, low, high, i);
+                if (i >= offsets[k] && i + N <= end && i + N <= offsets[k + 1]) {
+                    Pack<T> v = loadPackAnywhere(in[k] + (i - offsets[k]));
+#pragma unroll
+                    for (int e = 0; e < N; e++) v.v[e] = fromCompute<T>(toCompute(v.v[e]) * factor);
+                    storePackAnywhere(out[k] + (i - offsets[k]), v);
+                    continue;
+                }
+                for (Long j = i; j < i + N && j < end; j++) {
+                    while (k < high && j >= offsets[k + 1]) k++;
+                    if (j < offsets[k]) continue;
+                    out[k][j - offsets[k]] = fromCompute<T>(toCompute(in[k][j - offsets[k]]) * factor);
+                }
+            }
+        }
     }
 }
 
@@ -74,10 +185,18 @@ template <typename T>
 void launchClipByGlobalNorm(hipStream_t s, const T *const *in, T *const *out, const Long *offsets, int n, Long total, double maxNorm,
                             typename Compute<T>::type *norm, void *scratch) {
     double *partial = reinterpret_cast<double *>(scratch);
-    const int blocks = gridFor(total, kNormThreads, kNormBlocks);
-    ND4J_LAUNCH((squaresKernel<T>), dim3(blocks), dim3(kNormThreads), 0, s, in, offsets, n, total, partial);
-    ND4J_LAUNCH((clipKernel<T>), dim3(out != nullptr ? blocks : 1), dim3(kNormThreads), 0, s, in, out, offsets, n, total, maxNorm, norm, partial,
-                blocks);
+    // Four vectors a thread where that leaves every block a tile; one where the tensors are small, for more blocks
+    const Long wide = (Long)kNormThreads * 4 * Pack<T>::N, narrow = (Long)kNormThreads * Pack<T>::N;
+    const bool isWide = total >= wide * kNormBlocks;
+    const int blocks = gridFor(total, isWide ? wide : narrow, kNormBlocks);
+    const dim3 grid(blocks), resultGrid(out != nullptr ? blocks : 1), block(kNormThreads);
+    if (isWide) {
+        ND4J_LAUNCH((squaresKernel<T, 4>), grid, block, 0, s, in, offsets, n, total, partial);
+        ND4J_LAUNCH((clipKernel<T, 4>), resultGrid, block, 0, s, in, out, offsets, n, total, maxNorm, norm, partial, blocks);
+    } else {
+        ND4J_LAUNCH((squaresKernel<T, 1>), grid, block, 0, s, in, offsets, n, total, partial);
+        ND4J_LAUNCH((clipKernel<T, 1>), resultGrid, block, 0, s, in, out, offsets, n, total, maxNorm, norm, partial, blocks);
+    }
 }
 
 #define INST(T)                                                                                                                    \
