@@ -17,7 +17,7 @@ namespace {
 [[noreturn]] void refuse(const char *op, const std::string &why) { throw std::invalid_argument(std::string(op) + ": " + why); }
 
 const Long kMostRows = (Long)1 << 40;
-const Long kMostLength = ((Long)1 << 31) - 65;  // columns and row numbers fit an int with a wave's width to spare
+const Long kMostLength = ((Long)1 << 31) - ((Long)1 << 20);  // columns fit an int with any block's round to spare
 
 // The rows of a view: its last dimension, at every position of the others, which have to lie a common distance apart.
 RowView rowsOf(const char *op, const char *name, Nd4jPointer *extra, int slot, const Long *arg, std::vector<Long> &storage, hipStream_t s) {
@@ -46,7 +46,7 @@ RowView rowsOf(const char *op, const char *name, Nd4jPointer *extra, int slot, c
         v.rows *= shape[d];
     }
     if (v.length < 1) refuse(op, std::string(name) + " has rows without elements");
-    if (v.length > kMostLength) refuse(op, std::string(name) + " has rows of 2^31 elements or more");
+    if (v.length > kMostLength) refuse(op, std::string(name) + " has rows of more than 2^31 - 2^20 elements");
     return v;
 }
 
@@ -165,7 +165,7 @@ void embeddingBp(Nd4jPointer *extra, T *dz, Long *dzInfo, Long *tokens, Long n, 
     if (dzv.rows != n || dzv.length != tv.length) refuse(op, "dz is not a row of the table's length for every token");
     if (tv.rows == 0 || (n == 0 && accumulate != 0)) return;
     // (tokens are sorted as 32-bit keys with 32-bit positions)
-    if (n > kMostLength || tv.rows > kMostLength) refuse(op, "2^31 tokens or rows of the table and more are not supported");
+    if (n > kMostLength || tv.rows > kMostLength) refuse(op, "more than 2^31 - 2^20 tokens or rows of the table are not supported");
     if (!embeddingBpFits(n, tv.length)) refuse(op, "too many elements");
     must(op, "dTable", dTable);
     if (n > 0) {

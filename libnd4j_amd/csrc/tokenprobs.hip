@@ -94,6 +94,263 @@ __global__ void __launch_bounds__(kRowThreads) tokenProbsAnyKernel(const T *x, R
     }
 }
 
+// ---- rows of contiguous elements, forward ------------------------------------------------------------------------------
+// One sweep: every lane keeps the maximum of its elements, the sum of exp(x - maximum) and of (maximum - x) exp(x - maximum),
+// rescaled where a tile raises the maximum, and its wave keeps the k best elements sorted over its lanes.  A tile takes part
+// in the search for alternatives only if one of its lanes' maxima (which the sums need anyway) beats the wave's k-th best so
+// far, which is rare after the first tiles.  The waves of a block, and the slices of a row where rows are few, are
+// joined in a fixed order.
+
+// exp for the sums: the relative error grows with |d| (a rounding of d log2 e), on terms whose share is exp(d)
+__device__ __forceinline__ float expOf(float d) { return __builtin_amdgcn_exp2f(d * 1.44269502162933349609375f); }
+__device__ __forceinline__ double expOf(double d) { return ::exp(d); }
+__device__ __forceinline__ float fma_(float a, float b, float c) { return __builtin_fmaf(a, b, c); }
+__device__ __forceinline__ double fma_(double a, double b, double c) { return __builtin_fma(a, b, c); }
+
+// A value of one lane, for all of them (in scalar registers)
+template <typename C> __device__ __forceinline__ C laneValue(C v, int lane) {
+    constexpr int W = sizeof(C) / 4;
+    struct Words { int w[W]; };
+    Words in = __builtin_bit_cast(Words, v), out;
+#pragma unroll
+    for (int i = 0; i < W; i++) out.w[i] = __builtin_amdgcn_readlane(in.w[i], lane);
+    return __builtin_bit_cast(C, out);
+}
+template <typename C> __device__ __forceinline__ C laneBelow(C v) {  // lane l gets lane l - 1's (lane 0 its own)
+    constexpr int W = sizeof(C) / 4;
+    struct Words { int w[W]; };
+    Words in = __builtin_bit_cast(Words, v), out;
+#pragma unroll
+    for (int i = 0; i < W; i++) out.w[i] = __shfl_up(in.w[i], 1);
+    return __builtin_bit_cast(C, out);
+}
+
+constexpr int kNoIndex = 0x7fffffff;
+// The k best elements a wave has seen, the j-th in lane j: larger values first, lower indexes first among equals.  Places
+// not taken yet hold -infinity under kNoIndex, which every element beats, one of -infinity too.
+template <typename C> struct BestList {
+    C value;
+    int index;
+    C worstValue;  // of place k - 1, in all lanes
+    int worstIndex;
+    int k;
+    __device__ __forceinline__ void clear(int places) {
+        k = places;
+        value = worstValue = -infinite<C>();
+        index = worstIndex = kNoIndex;
+    }
+    __device__ __forceinline__ bool beats(C v, int i) const { return v > worstValue || (v == worstValue && i < worstIndex); }
+    // v and i are the same in all lanes, and beat the worst entry
+    __device__ __forceinline__ void insert(C v, int i) {
+        const int lane = threadIdx.x % kWaveLanes;
+        const int place = __popcll(__ballot(value > v || (value == v && index < i)));
+        const C above = laneBelow(value);
+        const int aboveIndex = laneBelow(index);
+        value = lane == place ? v : (lane > place ? above : value);
+        index = lane == place ? i : (lane > place ? aboveIndex : index);
+        worstValue = laneValue(value, k - 1);
+        worstIndex = laneValue(index, k - 1);
+    }
+    // every lane offers an element
+    __device__ __forceinline__ void offer(C v, int i, bool live) {
+        unsigned long long mask = __ballot(live && beats(v, i));
+        while (mask != 0ull) {
+            const int from = __ffsll((unsigned long long)mask) - 1;
+            insert(laneValue(v, from), laneValue(i, from));
+            mask &= mask - 1;
+            mask &= __ballot(live && beats(v, i));
+        }
+    }
+};
+
+// maximum, sum of exp(x - maximum), sum of (maximum - x) exp(x - maximum)
+template <typename C> struct Sums {
+    C largest, sum, weighted;
+    __device__ __forceinline__ void clear() {
+        largest = -infinite<C>();
+        sum = weighted = (C)0;
+    }
+    __device__ __forceinline__ void raiseTo(C to) {  // to >= largest
+        if (!(to > largest)) return;
+        if (largest > -infinite<C>()) {
+            const C d = largest - to, f = expOf(d);
+            // (from the type's lowest value d sum may overflow, and nothing of it is left)
+            weighted = f > (C)0 ? (weighted - d * sum) * f : (C)0;
+            sum *= f;
+        }
+        largest = to;
+    }
+    __device__ __forceinline__ void add(Sums o) {
+        const C to = Largest()(largest, o.largest);
+        raiseTo(to);
+        o.raiseTo(to);
+        sum += o.sum;
+        weighted += o.weighted;
+    }
+};
+
+template <typename T>
+__device__ __forceinline__ void writeRow(const T *xr, Long length, Long r, const Long *tokens, const TokenProbsOut<T> &out,
+                                         const Sums<typename Compute<T>::type> &s) {
+    typedef typename Compute<T>::type C;
+    const bool none = s.sum == (C)0;
+    const C from = s.largest > -infinite<C>() ? s.largest : (C)0, logSum = m::logSoft_(s.sum);
+    if (threadIdx.x % kWaveLanes == 0) {
+        if (out.logSum != nullptr) out.logSum[r] = from + logSum;
+        if (out.entropy != nullptr) out.entropy[r] = none ? (C)0 : logSum + s.weighted / s.sum;
+        if (out.logProbs != nullptr) {
+            const Long t = tokens[r];
+            C lp = (C)0;
+            if (t >= length) lp = notANumber<C>();
+            else if (t >= 0) lp = none ? -infinite<C>() : (toCompute(xr[t]) - from) - logSum;
+            out.logProbs[r] = lp;
+        }
+    }
+}
+template <typename T>
+__device__ __forceinline__ void writeBest(Long r, const TokenProbsOut<T> &out, const Sums<typename Compute<T>::type> &s,
+                                          const BestList<typename Compute<T>::type> &best) {
+    typedef typename Compute<T>::type C;
+    const int lane = threadIdx.x % kWaveLanes;
+    if (lane >= out.k) return;
+    const bool none = s.sum == (C)0, entry = best.index != kNoIndex;
+    const C from = s.largest > -infinite<C>() ? s.largest : (C)0, logSum = m::logSoft_(s.sum);
+    out.top[r * out.k + lane] = entry ? best.index : -1;
+    if (out.topLogProbs != nullptr)
+        out.topLogProbs[r * out.k + lane] = !entry ? notANumber<C>() : (none ? -infinite<C>() : (best.value - from) - logSum);
+}
+
+// A slice of a row leaves 3 + 2 k values for the join: its sums, and its list's values and indexes.
+template <typename T, int VECTORS, bool ENTROPY, bool TOP>
+__global__ void __launch_bounds__(kRowThreads) tokenProbsRowsKernel(const T *x, RowView xv, const Long *tokens, TokenProbsOut<T> out,
+                                                                    typename Compute<T>::type *scratch, int slices, int sliceLength) {
+    typedef typename Compute<T>::type C;
+    constexpr int N = Pack<T>::N, WAVES = kRowThreads / kWaveLanes, TILE = kWaveLanes * N * VECTORS;
+    __shared__ Sums<C> waveSums[WAVES];
+    __shared__ C values[WAVES][kWaveLanes];
+    __shared__ int indexes[WAVES][kWaveLanes];
+    const int lane = threadIdx.x % kWaveLanes, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWaveLanes);
+    for (Long work = blockIdx.x; work < xv.rows * slices; work += gridDim.x) {
+        const Long r = work / slices;
+        const int slice = (int)(work - r * slices);
+        const int begin = slice * sliceLength, end = (int)(begin + (Long)sliceLength < xv.length ? begin + sliceLength : xv.length);
+        const T *xr = x + r * xv.row;
+        Sums<C> s;
+        s.clear();
+        BestList<C> best;
+        best.clear(TOP ? out.k : 1);
+        for (int t = begin + wave * TILE; t < end; t += WAVES * TILE) {
+            Pack<T> v[VECTORS];
+            const bool whole = t + TILE <= end;
+            if (whole) {
+#pragma unroll
+                for (int j = 0; j < VECTORS; j++) v[j] = streamPackAnywhere(xr + t + (j * kWaveLanes + lane) * N);
+            } else {
+#pragma unroll
+                for (int j = 0; j < VECTORS; j++)
+#pragma unroll
+                    for (int e = 0; e < N; e++) {
+                        const int c = t + (j * kWaveLanes + lane) * N + e;
+                        v[j].v[e] = c < end ? xr[c] : fromCompute<T>(-infinite<C>());  // adds nothing to the sums
+                    }
+            }
+            C tileLargest = -infinite<C>();
+#pragma unroll
+            for (int j = 0; j < VECTORS; j++)
+#pragma unroll
+                for (int e = 0; e < N; e++) tileLargest = Largest()(tileLargest, toCompute(v[j].v[e]));
+            // (equal values further on in the row never beat what the list holds)
+            if (TOP && __ballot(tileLargest > best.worstValue || best.worstIndex == kNoIndex) != 0ull) {
+#pragma unroll
+                for (int j = 0; j < VECTORS; j++)
+#pragma unroll
+                    for (int e = 0; e < N; e++) {
+                        const int c = t + (j * kWaveLanes + lane) * N + e;
+                        best.offer(toCompute(v[j].v[e]), c, c < end);
+                    }
+            }
+            s.raiseTo(tileLargest);
+            const C from = s.largest > -infinite<C>() ? s.largest : (C)0;
+#pragma unroll
+            for (int j = 0; j < VECTORS; j++)
+#pragma unroll
+                for (int e = 0; e < N; e++) {
+                    const C d = toCompute(v[j].v[e]) - from, p = expOf(d);
+                    s.sum += p;
+                    // (0 for an element of -infinity, where d p is not a number)
+                    if (ENTROPY) s.weighted = fma_(Largest()(d, (C)-1e30f), -p, s.weighted);
+                }
+        }
+        // the wave's sums: everything relative to the largest maximum first
+        s.raiseTo(waveAll<kWaveLanes>(s.largest, Largest()));
+        s.sum = waveAll<kWaveLanes>(s.sum, Add());
+        if (ENTROPY) s.weighted = waveAll<kWaveLanes>(s.weighted, Add());
+        __syncthreads();  // the arrays may still be read from the round before
+        if (lane == 0) waveSums[wave] = s;
+        if (TOP) {
+            values[wave][lane] = best.value;
+            indexes[wave][lane] = best.index;
+        }
+        __syncthreads();
+        if (wave != 0) continue;
+#pragma unroll
+        for (int w = 1; w < WAVES; w++) {
+            s.add(waveSums[w]);
+            if (TOP) best.offer(values[w][lane], indexes[w][lane], lane < out.k);
+        }
+        if (slices == 1) {
+            writeRow<T>(xr, xv.length, r, tokens, out, s);
+            if (TOP) writeBest<T>(r, out, s, best);
+        } else {
+            C *to = scratch + (size_t)work * (3 + 2 * out.k);
+            if (lane < 3) to[lane] = lane == 0 ? s.largest : (lane == 1 ? s.sum : s.weighted);
+            if (TOP && lane < out.k) {
+                to[3 + lane] = best.value;
+                reinterpret_cast<int *>(to + 3 + out.k)[lane] = best.index;
+            }
+        }
+    }
+}
+
+// A wave takes a row and joins its slices.
+template <typename T, bool TOP>
+__global__ void __launch_bounds__(kWaveLanes) tokenProbsJoinKernel(const T *x, RowView xv, const Long *tokens, TokenProbsOut<T> out,
+                                                                   const typename Compute<T>::type *scratch, int slices) {
+    typedef typename Compute<T>::type C;
+    const int lane = threadIdx.x;
+    const size_t each = 3 + 2 * (size_t)out.k;
+    for (Long r = blockIdx.x; r < xv.rows; r += gridDim.x) {
+        const C *from = scratch + (size_t)r * slices * each;
+        Sums<C> s;
+        s.clear();
+        for (int i = lane; i < slices; i += kWaveLanes) {
+            Sums<C> o;
+            o.largest = from[i * each];
+            o.sum = from[i * each + 1];
+            o.weighted = from[i * each + 2];
+            s.add(o);
+        }
+        s.raiseTo(waveAll<kWaveLanes>(s.largest, Largest()));
+        s.sum = waveAll<kWaveLanes>(s.sum, Add());
+        s.weighted = waveAll<kWaveLanes>(s.weighted, Add());
+        writeRow<T>(x + r * xv.row, xv.length, r, tokens, out, s);
+        if (TOP) {
+            BestList<C> best;
+            best.clear(out.k);
+            // 64 entries at a time, over the lists as they lie behind each other
+            const int entries = slices * out.k;
+            for (int i = 0; i < entries; i += kWaveLanes) {
+                const int mine = i + lane < entries ? i + lane : entries - 1, slice = mine / out.k, place = mine - slice * out.k;
+                const C value = from[slice * each + 3 + place];
+                const int index = reinterpret_cast<const int *>(from + slice * each + 3 + out.k)[place];
+                best.offer(value, index, i + lane < entries);
+            }
+            writeBest<T>(r, out, s, best);
+        }
+    }
+}
+
+// ---- backward ----------------------------------------------------------------------------------------------------------
 template <typename T>
 __global__ void __launch_bounds__(kRowThreads) tokenProbsBpAnyKernel(const T *x, RowView xv, const Long *tokens,
                                                                      const typename Compute<T>::type *logSum,
@@ -118,14 +375,138 @@ __global__ void __launch_bounds__(kRowThreads) tokenProbsBpAnyKernel(const T *x,
     }
 }
 
+// Rows of contiguous elements: a team of a wave or a block takes a stretch of a row, four vectors a lane and round.
+template <typename T, int TEAM, bool ENTROPY>
+__global__ void __launch_bounds__(kRowThreads) tokenProbsBpRowsKernel(const T *x, RowView xv, const Long *tokens,
+                                                                      const typename Compute<T>::type *logSum,
+                                                                      const typename Compute<T>::type *entropy,
+                                                                      const typename Compute<T>::type *dLogProbs,
+                                                                      const typename Compute<T>::type *dEntropy, T *dx, RowView dxv,
+                                                                      int stretches, int stretch) {
+    typedef typename Compute<T>::type C;
+    constexpr int N = Pack<T>::N, VECTORS = 4, TEAMS = kRowThreads / TEAM, ROUND = TEAM * N * VECTORS;
+    const int lane = threadIdx.x % TEAM, team = TEAM == kRowThreads ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / TEAM);
+    for (Long work = (Long)blockIdx.x * TEAMS + team; work < xv.rows * stretches; work += (Long)gridDim.x * TEAMS) {
+        const Long r = work / stretches;
+        const int begin = (int)(work - r * stretches) * stretch, end = (int)(begin + (Long)stretch < xv.length ? begin + stretch : xv.length);
+        const T *xr = x + r * xv.row;
+        T *dxr = dx + r * dxv.row;
+        const C ls = logSum[r];
+        const Long t = dLogProbs != nullptr ? tokens[r] : -1;
+        C a = t < 0 ? (C)0 : dLogProbs[r];
+        if (t >= xv.length) a = notANumber<C>();
+        const C b = ENTROPY ? dEntropy[r] : (C)0, h = ENTROPY ? entropy[r] : (C)0;
+        const bool none = ls == -infinite<C>();
+        auto gradient = [&](C v) {
+            const C lp = v - ls, p = expOf(lp);
+            C d = -a * p;
+            if (ENTROPY) d -= p != (C)0 ? b * p * (lp + h) : (C)0;
+            return none ? (C)0 : d;
+        };
+        for (int c0 = begin; c0 < end; c0 += ROUND) {
+            const bool hasToken = t >= c0 && t < (Long)c0 + ROUND && !none;
+            if (c0 + (Long)ROUND <= end) {
+                Pack<T> v[VECTORS];
+#pragma unroll
+                for (int j = 0; j < VECTORS; j++) v[j] = streamPackAnywhere(xr + c0 + (j * TEAM + lane) * N);
+#pragma unroll
+                for (int j = 0; j < VECTORS; j++) {
+                    const int c = c0 + (j * TEAM + lane) * N;
+                    C d[N];
+#pragma unroll
+                    for (int e = 0; e < N; e++) d[e] = gradient(toCompute(v[j].v[e]));
+                    if (hasToken) {
+#pragma unroll
+                        for (int e = 0; e < N; e++) d[e] += c + e == t ? a : (C)0;
+                    }
+#pragma unroll
+                    for (int e = 0; e < N; e++) v[j].v[e] = fromCompute<T>(d[e]);
+                    streamPackAnywhere(dxr + c, v[j]);
+                }
+            } else {
+                for (int c = c0 + lane * N; c < end; c += TEAM * N) {
+                    if (c + N <= end) {
+                        Pack<T> v = streamPackAnywhere(xr + c);
+#pragma unroll
+                        for (int e = 0; e < N; e++) v.v[e] = fromCompute<T>(gradient(toCompute(v.v[e])) + (hasToken && c + e == t ? a : (C)0));
+                        streamPackAnywhere(dxr + c, v);
+                    } else {
+                        for (int i = c; i < end; i++)
+                            dxr[i] = fromCompute<T>(gradient(toCompute(xr[i])) + (hasToken && i == t ? a : (C)0));
+                    }
+                }
+            }
+        }
+    }
+}
+
 unsigned gridOf(Long blocks) { return (unsigned)(blocks < 1 ? 1 : (blocks > (1 << 20) ? (1 << 20) : blocks)); }
 
 }  // namespace
 
-size_t tokenLogProbsScratch(Long, Long, int) { return 0; }
+namespace {
+
+// The slices of a row: rows alone fill the chip from kEnoughBlocks on; fewer are cut into equal slices of whole rounds of a
+// block's waves.  `vectors`: 16-byte vectors a lane and round, four for the most in flight, one where that leaves too few blocks.
+constexpr Long kEnoughBlocks = 1024;
+struct Cut {
+    int vectors, slices, sliceLength;
+};
+Cut cutOf(Long rows, Long length, int perVector) {
+    Cut c;
+    const Long wide = (Long)kRowThreads * perVector * 4;
+    c.vectors = rows * ((length + wide - 1) / wide) >= kEnoughBlocks ? 4 : 1;
+    const Long round = (Long)kRowThreads * perVector * c.vectors, most = (length + round - 1) / round;
+    Long slices = (kEnoughBlocks + rows - 1) / rows;
+    if (slices > most) slices = most;
+    const Long rounds = (most + slices - 1) / slices;
+    c.slices = (int)((most + rounds - 1) / rounds);
+    c.sliceLength = c.slices == 1 ? (int)length : (int)(rounds * round);
+    return c;
+}
+
+template <typename T, int VECTORS>
+void runTokenProbs(hipStream_t s, const T *x, const RowView &xv, const Long *tokens, const TokenProbsOut<T> &out,
+                   typename Compute<T>::type *scratch, const Cut &cut) {
+    const dim3 grid(gridOf(xv.rows * cut.slices)), block(kRowThreads);
+#define RUN(ENTROPY, TOP)                                                                                                             \
+    ND4J_LAUNCH((tokenProbsRowsKernel<T, VECTORS, ENTROPY, TOP>), grid, block, 0, s, x, xv, tokens, out, scratch, cut.slices, cut.sliceLength)
+    if (out.entropy != nullptr) {
+        if (out.k > 0) RUN(true, true);
+        else RUN(true, false);
+    } else {
+        if (out.k > 0) RUN(false, true);
+        else RUN(false, false);
+    }
+#undef RUN
+}
+
+}  // namespace
+
+// (Bounded over the types: a double's rounds are the shortest, so its rows are cut into the most slices.)
+size_t tokenLogProbsScratch(Long rows, Long length, int k) {
+    if (rows <= 0 || rows >= kEnoughBlocks) return 0;
+    const Long round = (Long)kRowThreads * 2, most = (length + round - 1) / round;
+    Long slices = (kEnoughBlocks + rows - 1) / rows;
+    if (slices > most) slices = most;
+    return slices <= 1 ? 0 : (size_t)rows * slices * (3 + 2 * k) * sizeof(double);
+}
 
 template <typename T>
-void launchTokenLogProbs(hipStream_t s, const T *x, const RowView &xv, const Long *tokens, const TokenProbsOut<T> &out, void *) {
+void launchTokenLogProbs(hipStream_t s, const T *x, const RowView &xv, const Long *tokens, const TokenProbsOut<T> &out, void *scratch) {
+    typedef typename Compute<T>::type C;
+    if (xv.el == 1) {
+        const Cut cut = cutOf(xv.rows, xv.length, Pack<T>::N);
+        C *work = reinterpret_cast<C *>(scratch);
+        if (cut.vectors == 4) runTokenProbs<T, 4>(s, x, xv, tokens, out, work, cut);
+        else runTokenProbs<T, 1>(s, x, xv, tokens, out, work, cut);
+        if (cut.slices > 1) {
+            const dim3 grid(gridOf(xv.rows)), block(kWaveLanes);
+            if (out.k > 0) ND4J_LAUNCH((tokenProbsJoinKernel<T, true>), grid, block, 0, s, x, xv, tokens, out, work, cut.slices);
+            else ND4J_LAUNCH((tokenProbsJoinKernel<T, false>), grid, block, 0, s, x, xv, tokens, out, work, cut.slices);
+        }
+        return;
+    }
     ND4J_LAUNCH((tokenProbsAnyKernel<T>), dim3(gridOf(xv.rows)), dim3(kRowThreads), 0, s, x, xv, tokens, out);
 }
 
@@ -133,6 +514,25 @@ template <typename T>
 void launchTokenLogProbsBp(hipStream_t s, const T *x, const RowView &xv, const Long *tokens, const typename Compute<T>::type *logSum,
                            const typename Compute<T>::type *entropy, const typename Compute<T>::type *dLogProbs,
                            const typename Compute<T>::type *dEntropy, T *dx, const RowView &dxv) {
+    if (xv.el == 1 && dxv.el == 1) {
+        // a wave for rows of up to one round of a wave, else a block for every round of a block
+        const bool waves = xv.length <= (Long)kWaveLanes * Pack<T>::N * 4;
+        const int stretch = waves ? (int)xv.length : kRowThreads * Pack<T>::N * 4, stretches = (int)((xv.length + stretch - 1) / stretch);
+        const Long teams = xv.rows * stretches;
+        const dim3 grid(gridOf(waves ? (teams + 3) / 4 : teams)), block(kRowThreads);
+#define RUN(TEAM, ENTROPY)                                                                                                                 \
+    ND4J_LAUNCH((tokenProbsBpRowsKernel<T, TEAM, ENTROPY>), grid, block, 0, s, x, xv, tokens, logSum, entropy, dLogProbs, dEntropy, dx, dxv, \
+                stretches, stretch)
+        if (waves) {
+            if (dEntropy != nullptr) RUN(kWaveLanes, true);
+            else RUN(kWaveLanes, false);
+        } else {
+            if (dEntropy != nullptr) RUN(kRowThreads, true);
+            else RUN(kRowThreads, false);
+        }
+#undef RUN
+        return;
+    }
     ND4J_LAUNCH((tokenProbsBpAnyKernel<T>), dim3(gridOf(xv.rows)), dim3(kRowThreads), 0, s, x, xv, tokens, logSum, entropy, dLogProbs, dEntropy,
                 dx, dxv);
 }

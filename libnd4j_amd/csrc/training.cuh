@@ -85,7 +85,15 @@ template <int TEAM, class Op, typename C> __device__ __forceinline__ C teamAll(C
 __device__ __forceinline__ float sqrtOf(float v) { return ::sqrtf(v); }
 __device__ __forceinline__ double sqrtOf(double v) { return ::sqrt(v); }
 template <typename C> __device__ __forceinline__ C notANumber() { return (C)__builtin_nanf(""); }
-template <typename C> __device__ __forceinline__ C infinite() { return (C)__builtin_inff(); }
+template <typename C> __device__ __forceinline__ C infinite();
+template <> __device__ __forceinline__ float infinite<float>() { return __builtin_inff(); }
+// (From a register that the compiler does not see into: it moves a 64-bit constant into a pair of scalar registers in one
+// instruction here, of which the hardware takes 32 bits, and a list that begins with minus infinity began with 0.)
+template <> __device__ __forceinline__ double infinite<double>() {
+    unsigned high = 0x7ff00000u;
+    asm("" : "+v"(high));
+    return __builtin_bit_cast(double, (unsigned long long)high << 32);
+}
 
 }  // namespace tr
 }  // namespace nd4j_amd

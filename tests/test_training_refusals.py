@@ -70,8 +70,8 @@ def test_embedding(ops, S, why, args):
 @pytest.mark.parametrize("S", SUFFIXES)
 @pytest.mark.parametrize("why,args", [
     ("negative number", {"n": -1}), ("not a row of the table's length", {"n": 5}), ("not a row of the table's length", {"dzi": B}),
-    ("dTable is null", {"t": None}), ("tokens is null", {"k": None}), ("dz is null", {"dz": None}), ("2\\^31 tokens", {"n": 1 << 31, "dzi": info(1 << 31, 8)}),
-    ("2\\^31 tokens", {"ti": info(1 << 31, 8)}), ("too many elements", {"n": 1 << 30, "dzi": info(1 << 30, 1 << 20), "ti": info(50, 1 << 20)}),
+    ("dTable is null", {"t": None}), ("tokens is null", {"k": None}), ("dz is null", {"dz": None}), ("2\\^31 - 2\\^20 tokens", {"n": 1 << 31, "dzi": info(1 << 31, 8)}),
+    ("2\\^31 - 2\\^20 tokens", {"ti": info(1 << 31, 8)}), ("too many elements", {"n": 1 << 30, "dzi": info(1 << 30, 1 << 20), "ti": info(50, 1 << 20)}),
     ("scratch holds", {"w": P, "wb": 8}), ("not aligned to 16", {"w": P + 8, "wb": 1 << 40})])
 def test_embedding_bp(ops, S, why, args):
     g = lambda key, other=P: args.get(key, other)  # noqa: E731
