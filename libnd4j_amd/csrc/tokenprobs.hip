@@ -95,11 +95,15 @@ __global__ void __launch_bounds__(kRowThreads) tokenProbsAnyKernel(const T *x, R
 }
 
 // ---- rows of contiguous elements, forward ------------------------------------------------------------------------------
-// One sweep: every lane keeps the maximum of its elements, the sum of exp(x - maximum) and of (maximum - x) exp(x - maximum),
-// rescaled where a tile raises the maximum, and its wave keeps the k best elements sorted over its lanes.  A tile takes part
-// in the search for alternatives only if one of its lanes' maxima (which the sums need anyway) beats the wave's k-th best so
-// far, which is rare after the first tiles.  The waves of a block, and the slices of a row where rows are few, are
-// joined in a fixed order.
+// One sweep of a row by a block: every thread keeps the maximum of its elements, the sum of exp(x - maximum) and of
+// (maximum - x) exp(x - maximum), rescaled where its next elements raise the maximum.  The alternatives cost that sweep
+// nothing: the k-th largest of the 64 thread maxima of any one wave is a lower bound of the row's k-th largest element, so
+// only threads whose maximum reaches the largest of these bounds hold alternatives - k of them and a few more, where
+// values differ - and only their elements are read again, by all threads together.  Where rows are few they are cut
+// into slices, whose sums and lists a second launch joins.
+//
+// (Keeping the best elements during the sweep, as the first form did, took 118 us over [4096, 32000] floats at k = 5, where
+// the sweep alone takes 81.)
 
 // exp for the sums: the relative error grows with |d| (a rounding of d log2 e), on terms whose share is exp(d)
 __device__ __forceinline__ float expOf(float d) { return __builtin_amdgcn_exp2f(d * 1.44269502162933349609375f); }
@@ -117,14 +121,8 @@ template <typename C> __device__ __forceinline__ C laneValue(C v, int lane) {
     return __builtin_bit_cast(C, out);
 }
 template <typename C> __device__ __forceinline__ C laneBelow(C v) {  // lane l gets lane l - 1's (lane 0 its own)
-    constexpr int W = sizeof(C) / 4;
-    struct Words { int w[W]; };
-    Words in = __builtin_bit_cast(Words, v), out;
-#pragma unroll
-    for (int i = 0; i < W; i++) out.w[i] = __shfl_up(in.w[i], 1);
-    return __builtin_bit_cast(C, out);
+    return laneDpp<0x138>(v);
 }
-
 constexpr int kNoIndex = 0x7fffffff;
 // The k best elements a wave has seen, the j-th in lane j: larger values first, lower indexes first among equals.  Places
 // not taken yet hold -infinity under kNoIndex, which every element beats, one of -infinity too.
@@ -163,6 +161,69 @@ template <typename C> struct BestList {
     }
 };
 
+struct Lowest {
+    __device__ __forceinline__ int operator()(int a, int b) const { return a < b ? a : b; }
+};
+
+// The k best of several sorted lists, one a lane (list l: `count` places at values + l * count, indexes + l * count): the
+// best of the lists' heads k times over.
+template <typename C>
+__device__ __forceinline__ void mergeLists(BestList<C> &best, int lists, int count, const C *values, const int *indexes) {
+    const int lane = threadIdx.x % kWaveLanes;
+    best.clear(count);
+    int at = 0;
+    C head = lane < lists ? values[lane * count] : -infinite<C>();
+    int headIndex = lane < lists ? indexes[lane * count] : kNoIndex;
+    for (int j = 0; j < count; j++) {
+        const C top = waveAll<kWaveLanes>(head, Largest());
+        bool first = headIndex != kNoIndex && head == top;
+        unsigned long long mask = __ballot(first);
+        if (mask == 0ull) return;  // (no list holds more: the places left are not taken)
+        if ((mask & (mask - 1)) != 0ull) {
+            const int lowest = waveAll<kWaveLanes>(first ? headIndex : kNoIndex, Lowest());
+            first = first && headIndex == lowest;
+            mask = __ballot(first);
+        }
+        const int index = laneValue(headIndex, __ffsll(mask) - 1);
+        if (lane == j) {
+            best.value = top;
+            best.index = index;
+        }
+        if (first) {
+            at++;
+            head = at < count ? values[lane * count + at] : -infinite<C>();
+            headIndex = at < count ? indexes[lane * count + at] : kNoIndex;
+        }
+    }
+}
+
+// whole numbers in the order of the values (none of them NaN)
+__device__ __forceinline__ unsigned orderOf(float v) {
+    const unsigned b = __builtin_bit_cast(unsigned, v);
+    return (b >> 31) != 0u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ unsigned long long orderOf(double v) {
+    const unsigned long long b = __builtin_bit_cast(unsigned long long, v);
+    return (b >> 63) != 0ull ? ~b : b | 0x8000000000000000ull;
+}
+__device__ __forceinline__ float valueOf(unsigned o) { return __builtin_bit_cast(float, (o >> 31) != 0u ? o & 0x7fffffffu : ~o); }
+__device__ __forceinline__ double valueOf(unsigned long long o) {
+    return __builtin_bit_cast(double, (o >> 63) != 0ull ? o & 0x7fffffffffffffffull : ~o);
+}
+// the k-th largest of a wave's 64 values, by its bits from the highest on
+template <typename C> __device__ __forceinline__ C kthLargest(C v, int k) {
+    const auto mine = orderOf(v);
+    auto found = mine;
+    found = 0;
+#pragma unroll 4
+    for (int bit = (int)sizeof(C) * 8 - 1; bit >= 0; bit--) {
+        auto with = found;
+        with |= (decltype(found))1 << bit;
+        if (__popcll(__ballot(mine >= with)) >= k) found = with;
+    }
+    return valueOf(found);
+}
+
 // maximum, sum of exp(x - maximum), sum of (maximum - x) exp(x - maximum)
 template <typename C> struct Sums {
     C largest, sum, weighted;
@@ -190,7 +251,7 @@ template <typename C> struct Sums {
 };
 
 template <typename T>
-__device__ __forceinline__ void writeRow(const T *xr, Long length, Long r, const Long *tokens, const TokenProbsOut<T> &out,
+__device__ __forceinline__ void writeRow(Long length, Long r, Long token, typename Compute<T>::type tokenValue, const TokenProbsOut<T> &out,
                                          const Sums<typename Compute<T>::type> &s) {
     typedef typename Compute<T>::type C;
     const bool none = s.sum == (C)0;
@@ -199,10 +260,9 @@ __device__ __forceinline__ void writeRow(const T *xr, Long length, Long r, const
         if (out.logSum != nullptr) out.logSum[r] = from + logSum;
         if (out.entropy != nullptr) out.entropy[r] = none ? (C)0 : logSum + s.weighted / s.sum;
         if (out.logProbs != nullptr) {
-            const Long t = tokens[r];
             C lp = (C)0;
-            if (t >= length) lp = notANumber<C>();
-            else if (t >= 0) lp = none ? -infinite<C>() : (toCompute(xr[t]) - from) - logSum;
+            if (token >= length) lp = notANumber<C>();
+            else if (token >= 0) lp = none ? -infinite<C>() : (tokenValue - from) - logSum;
             out.logProbs[r] = lp;
         }
     }
@@ -221,54 +281,51 @@ __device__ __forceinline__ void writeBest(Long r, const TokenProbsOut<T> &out, c
 }
 
 // A slice of a row leaves 3 + 2 k values for the join: its sums, and its list's values and indexes.
-template <typename T, int VECTORS, bool ENTROPY, bool TOP>
-__global__ void __launch_bounds__(kRowThreads) tokenProbsRowsKernel(const T *x, RowView xv, const Long *tokens, TokenProbsOut<T> out,
-                                                                    typename Compute<T>::type *scratch, int slices, int sliceLength) {
+
+template <typename T, int THREADS, int VECTORS, bool ENTROPY, bool TOP>
+__global__ void __launch_bounds__(THREADS) tokenProbsRowsKernel(const T *x, RowView xv, const Long *tokens, TokenProbsOut<T> out,
+                                                                typename Compute<T>::type *scratch, int slices, int sliceLength) {
     typedef typename Compute<T>::type C;
-    constexpr int N = Pack<T>::N, WAVES = kRowThreads / kWaveLanes, TILE = kWaveLanes * N * VECTORS;
+    constexpr int N = Pack<T>::N, WAVES = THREADS / kWaveLanes, ROUND = THREADS * N;
     __shared__ Sums<C> waveSums[WAVES];
-    __shared__ C values[WAVES][kWaveLanes];
-    __shared__ int indexes[WAVES][kWaveLanes];
+    __shared__ C bounds[WAVES];
+    __shared__ int hotCounts[WAVES];
+    __shared__ short hot[THREADS];
+    extern __shared__ __align__(16) char dynamicLds[];
+    C *values = reinterpret_cast<C *>(dynamicLds);  // [WAVES][k], and as many indexes behind them
+    int *indexes = reinterpret_cast<int *>(values + WAVES * out.k);
     const int lane = threadIdx.x % kWaveLanes, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWaveLanes);
     for (Long work = blockIdx.x; work < xv.rows * slices; work += gridDim.x) {
         const Long r = work / slices;
         const int slice = (int)(work - r * slices);
         const int begin = slice * sliceLength, end = (int)(begin + (Long)sliceLength < xv.length ? begin + sliceLength : xv.length);
         const T *xr = x + r * xv.row;
+        const Long token = slices == 1 && wave == 0 && out.logProbs != nullptr ? tokens[r] : -1;
+        const C tokenValue = token >= 0 && token < xv.length ? toCompute(xr[token]) : (C)0;
         Sums<C> s;
         s.clear();
-        BestList<C> best;
-        best.clear(TOP ? out.k : 1);
-        for (int t = begin + wave * TILE; t < end; t += WAVES * TILE) {
+        for (int t = begin; t < end; t += ROUND * VECTORS) {
             Pack<T> v[VECTORS];
-            const bool whole = t + TILE <= end;
-            if (whole) {
+            if (t + ROUND * VECTORS <= end) {
 #pragma unroll
-                for (int j = 0; j < VECTORS; j++) v[j] = streamPackAnywhere(xr + t + (j * kWaveLanes + lane) * N);
+                for (int j = 0; j < VECTORS; j++) v[j] = loadPackAnywhere(xr + t + (j * THREADS + (int)threadIdx.x) * N);
             } else {
 #pragma unroll
-                for (int j = 0; j < VECTORS; j++)
+                for (int j = 0; j < VECTORS; j++) {
+                    const int c = t + (j * THREADS + (int)threadIdx.x) * N;
+                    if (c + N <= end) {
+                        v[j] = loadPackAnywhere(xr + c);
+                    } else {
 #pragma unroll
-                    for (int e = 0; e < N; e++) {
-                        const int c = t + (j * kWaveLanes + lane) * N + e;
-                        v[j].v[e] = c < end ? xr[c] : fromCompute<T>(-infinite<C>());  // adds nothing to the sums
+                        for (int e = 0; e < N; e++) v[j].v[e] = c + e < end ? xr[c + e] : fromCompute<T>(-infinite<C>());  // adds nothing
                     }
+                }
             }
             C tileLargest = -infinite<C>();
 #pragma unroll
             for (int j = 0; j < VECTORS; j++)
 #pragma unroll
                 for (int e = 0; e < N; e++) tileLargest = Largest()(tileLargest, toCompute(v[j].v[e]));
-            // (equal values further on in the row never beat what the list holds)
-            if (TOP && __ballot(tileLargest > best.worstValue || best.worstIndex == kNoIndex) != 0ull) {
-#pragma unroll
-                for (int j = 0; j < VECTORS; j++)
-#pragma unroll
-                    for (int e = 0; e < N; e++) {
-                        const int c = t + (j * kWaveLanes + lane) * N + e;
-                        best.offer(toCompute(v[j].v[e]), c, c < end);
-                    }
-            }
             s.raiseTo(tileLargest);
             const C from = s.largest > -infinite<C>() ? s.largest : (C)0;
 #pragma unroll
@@ -281,25 +338,81 @@ __global__ void __launch_bounds__(kRowThreads) tokenProbsRowsKernel(const T *x, 
                     if (ENTROPY) s.weighted = fma_(Largest()(d, (C)-1e30f), -p, s.weighted);
                 }
         }
+        const C own = s.largest;
         // the wave's sums: everything relative to the largest maximum first
         s.raiseTo(waveAll<kWaveLanes>(s.largest, Largest()));
         s.sum = waveAll<kWaveLanes>(s.sum, Add());
         if (ENTROPY) s.weighted = waveAll<kWaveLanes>(s.weighted, Add());
         __syncthreads();  // the arrays may still be read from the round before
         if (lane == 0) waveSums[wave] = s;
+        BestList<C> best;
         if (TOP) {
-            values[wave][lane] = best.value;
-            indexes[wave][lane] = best.index;
+            const C waveBound = kthLargest(own, out.k);
+            if (lane == 0) bounds[wave] = waveBound;
+            __syncthreads();
+            C bound = bounds[0];
+#pragma unroll
+            for (int w = 1; w < WAVES; w++) bound = Largest()(bound, bounds[w]);
+            const bool isHot = own >= bound;
+            const unsigned long long mask = __ballot(isHot);
+            if (lane == 0) hotCounts[wave] = __popcll(mask);
+            __syncthreads();
+            int before = 0, hots = 0;
+#pragma unroll
+            for (int w = 0; w < WAVES; w++) {
+                if (w == wave) before = hots;
+                hots += hotCounts[w];
+            }
+            if (isHot) hot[before + __popcll(mask & ((1ull << lane) - 1))] = (short)threadIdx.x;
+            __syncthreads();
+            // vector q of hot thread h, 64 of them to a wave at a time; positions ascend over h and then q, so every list
+            // entry's index is compared in full
+            best.clear(out.k);
+            const int rounds = (end - begin + ROUND - 1) / ROUND;
+            const Long items = (Long)hots * rounds;
+            for (Long i = wave * kWaveLanes; i < items; i += THREADS) {
+                const Long item = i + lane;
+                const int h = (int)(item / rounds), q = (int)(item - (Long)h * rounds);
+                const int c = item < items ? begin + (q * THREADS + hot[h]) * N : end;
+                Pack<T> v;
+                if (c + N <= end) {
+                    v = loadPackAnywhere(xr + c);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < N; e++) v.v[e] = c + e < end ? xr[c + e] : fromCompute<T>((C)0);
+                }
+                unsigned offers = 0;  // a bit per element
+#pragma unroll
+                for (int e = 0; e < N; e++) {
+                    const C value = toCompute(v.v[e]);
+                    if (c + e < end && value >= bound && best.beats(value, c + e)) offers |= 1u << e;
+                }
+                while (__ballot(offers != 0u) != 0ull) {
+                    const int which = __ffs((int)offers) - 1;
+                    C value = -infinite<C>();
+#pragma unroll
+                    for (int e = 0; e < N; e++)
+                        if (e == which) value = toCompute(v.v[e]);
+                    best.offer(value, c + which, offers != 0u);
+                    offers &= offers - 1;
+                }
+            }
+            if (WAVES > 1) {
+                if (lane < out.k) {
+                    values[wave * out.k + lane] = best.value;
+                    indexes[wave * out.k + lane] = best.index;
+                }
+                __syncthreads();
+            }
+        } else if (WAVES > 1) {
+            __syncthreads();
         }
-        __syncthreads();
         if (wave != 0) continue;
 #pragma unroll
-        for (int w = 1; w < WAVES; w++) {
-            s.add(waveSums[w]);
-            if (TOP) best.offer(values[w][lane], indexes[w][lane], lane < out.k);
-        }
+        for (int w = 1; w < WAVES; w++) s.add(waveSums[w]);
+        if (TOP && WAVES > 1) mergeLists<C>(best, WAVES, out.k, values, indexes);
         if (slices == 1) {
-            writeRow<T>(xr, xv.length, r, tokens, out, s);
+            writeRow<T>(xv.length, r, token, tokenValue, out, s);
             if (TOP) writeBest<T>(r, out, s, best);
         } else {
             C *to = scratch + (size_t)work * (3 + 2 * out.k);
@@ -312,39 +425,45 @@ __global__ void __launch_bounds__(kRowThreads) tokenProbsRowsKernel(const T *x, 
     }
 }
 
-// A wave takes a row and joins its slices.
+// A wave takes a row and joins its slices, of which there are at most kMostSlices: one a lane.
+constexpr int kMostSlices = kWaveLanes;
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(kWaveLanes) tokenProbsJoinKernel(const T *x, RowView xv, const Long *tokens, TokenProbsOut<T> out,
                                                                    const typename Compute<T>::type *scratch, int slices) {
     typedef typename Compute<T>::type C;
-    const int lane = threadIdx.x;
-    const size_t each = 3 + 2 * (size_t)out.k;
+    extern __shared__ __align__(16) char dynamicLds[];
+    const int lane = threadIdx.x, entries = slices * out.k, each = 3 + 2 * out.k;
+    C *values = reinterpret_cast<C *>(dynamicLds);  // [slices][k], and as many indexes behind them
+    int *indexes = reinterpret_cast<int *>(values + entries);
     for (Long r = blockIdx.x; r < xv.rows; r += gridDim.x) {
         const C *from = scratch + (size_t)r * slices * each;
+        // (everything that has to come from memory is asked for before anything waits)
+        const Long token = out.logProbs != nullptr ? tokens[r] : -1;
+        const C tokenValue = token >= 0 && token < xv.length ? toCompute(x[r * xv.row + token]) : (C)0;
         Sums<C> s;
         s.clear();
-        for (int i = lane; i < slices; i += kWaveLanes) {
-            Sums<C> o;
-            o.largest = from[i * each];
-            o.sum = from[i * each + 1];
-            o.weighted = from[i * each + 2];
-            s.add(o);
+        if (lane < slices) {
+            s.largest = from[lane * each];
+            s.sum = from[lane * each + 1];
+            s.weighted = from[lane * each + 2];
+        }
+        if (TOP) {
+            __syncthreads();
+#pragma unroll 4
+            for (int i = lane; i < entries; i += kWaveLanes) {
+                const int slice = i / out.k, place = i - slice * out.k;
+                values[i] = from[slice * each + 3 + place];
+                indexes[i] = reinterpret_cast<const int *>(from + slice * each + 3 + out.k)[place];
+            }
+            __syncthreads();
         }
         s.raiseTo(waveAll<kWaveLanes>(s.largest, Largest()));
         s.sum = waveAll<kWaveLanes>(s.sum, Add());
         s.weighted = waveAll<kWaveLanes>(s.weighted, Add());
-        writeRow<T>(x + r * xv.row, xv.length, r, tokens, out, s);
+        writeRow<T>(xv.length, r, token, tokenValue, out, s);
         if (TOP) {
             BestList<C> best;
-            best.clear(out.k);
-            // 64 entries at a time, over the lists as they lie behind each other
-            const int entries = slices * out.k;
-            for (int i = 0; i < entries; i += kWaveLanes) {
-                const int mine = i + lane < entries ? i + lane : entries - 1, slice = mine / out.k, place = mine - slice * out.k;
-                const C value = from[slice * each + 3 + place];
-                const int index = reinterpret_cast<const int *>(from + slice * each + 3 + out.k)[place];
-                best.offer(value, index, i + lane < entries);
-            }
+            mergeLists<C>(best, slices, out.k, values, indexes);
             writeBest<T>(r, out, s, best);
         }
     }
@@ -447,17 +566,20 @@ unsigned gridOf(Long blocks) { return (unsigned)(blocks < 1 ? 1 : (blocks > (1 <
 namespace {
 
 // The slices of a row: rows alone fill the chip from kEnoughBlocks on; fewer are cut into equal slices of whole rounds of a
-// block's waves.  `vectors`: 16-byte vectors a lane and round, four for the most in flight, one where that leaves too few blocks.
+// block.  `vectors`: 16-byte vectors a thread and round, four for the most in flight, one where that leaves too few blocks.
+// Rows of up to eight vectors a lane of one wave are a wave's, when there are enough of them.
 constexpr Long kEnoughBlocks = 1024;
 struct Cut {
-    int vectors, slices, sliceLength;
+    int threads, vectors, slices, sliceLength;
 };
 Cut cutOf(Long rows, Long length, int perVector) {
     Cut c;
-    const Long wide = (Long)kRowThreads * perVector * 4;
+    c.threads = rows >= kEnoughBlocks && length <= (Long)kWaveLanes * perVector * 8 ? kWaveLanes : kRowThreads;
+    const Long wide = (Long)c.threads * perVector * 4;
     c.vectors = rows * ((length + wide - 1) / wide) >= kEnoughBlocks ? 4 : 1;
-    const Long round = (Long)kRowThreads * perVector * c.vectors, most = (length + round - 1) / round;
+    const Long round = (Long)c.threads * perVector * c.vectors, most = (length + round - 1) / round;
     Long slices = (kEnoughBlocks + rows - 1) / rows;
+    if (slices > kMostSlices) slices = kMostSlices;
     if (slices > most) slices = most;
     const Long rounds = (most + slices - 1) / slices;
     c.slices = (int)((most + rounds - 1) / rounds);
@@ -465,12 +587,15 @@ Cut cutOf(Long rows, Long length, int perVector) {
     return c;
 }
 
-template <typename T, int VECTORS>
+template <typename T, int THREADS, int VECTORS>
 void runTokenProbs(hipStream_t s, const T *x, const RowView &xv, const Long *tokens, const TokenProbsOut<T> &out,
                    typename Compute<T>::type *scratch, const Cut &cut) {
-    const dim3 grid(gridOf(xv.rows * cut.slices)), block(kRowThreads);
-#define RUN(ENTROPY, TOP)                                                                                                             \
-    ND4J_LAUNCH((tokenProbsRowsKernel<T, VECTORS, ENTROPY, TOP>), grid, block, 0, s, x, xv, tokens, out, scratch, cut.slices, cut.sliceLength)
+    typedef typename Compute<T>::type C;
+    const dim3 grid(gridOf(xv.rows * cut.slices)), block(THREADS);
+    const size_t lds = (size_t)(THREADS / kWaveLanes) * out.k * (sizeof(C) + sizeof(int));
+#define RUN(ENTROPY, TOP)                                                                                                              \
+    ND4J_LAUNCH((tokenProbsRowsKernel<T, THREADS, VECTORS, ENTROPY, TOP>), grid, block, lds, s, x, xv, tokens, out, scratch, cut.slices, \
+                cut.sliceLength)
     if (out.entropy != nullptr) {
         if (out.k > 0) RUN(true, true);
         else RUN(true, false);
@@ -488,6 +613,7 @@ size_t tokenLogProbsScratch(Long rows, Long length, int k) {
     if (rows <= 0 || rows >= kEnoughBlocks) return 0;
     const Long round = (Long)kRowThreads * 2, most = (length + round - 1) / round;
     Long slices = (kEnoughBlocks + rows - 1) / rows;
+    if (slices > kMostSlices) slices = kMostSlices;
     if (slices > most) slices = most;
     return slices <= 1 ? 0 : (size_t)rows * slices * (3 + 2 * k) * sizeof(double);
 }
@@ -498,11 +624,13 @@ void launchTokenLogProbs(hipStream_t s, const T *x, const RowView &xv, const Lon
     if (xv.el == 1) {
         const Cut cut = cutOf(xv.rows, xv.length, Pack<T>::N);
         C *work = reinterpret_cast<C *>(scratch);
-        if (cut.vectors == 4) runTokenProbs<T, 4>(s, x, xv, tokens, out, work, cut);
-        else runTokenProbs<T, 1>(s, x, xv, tokens, out, work, cut);
+        if (cut.threads == kWaveLanes) runTokenProbs<T, kWaveLanes, 4>(s, x, xv, tokens, out, work, cut);
+        else if (cut.vectors == 4) runTokenProbs<T, kRowThreads, 4>(s, x, xv, tokens, out, work, cut);
+        else runTokenProbs<T, kRowThreads, 1>(s, x, xv, tokens, out, work, cut);
         if (cut.slices > 1) {
             const dim3 grid(gridOf(xv.rows)), block(kWaveLanes);
-            if (out.k > 0) ND4J_LAUNCH((tokenProbsJoinKernel<T, true>), grid, block, 0, s, x, xv, tokens, out, work, cut.slices);
+            const size_t lds = (size_t)cut.slices * out.k * (sizeof(C) + sizeof(int));
+            if (out.k > 0) ND4J_LAUNCH((tokenProbsJoinKernel<T, true>), grid, block, lds, s, x, xv, tokens, out, work, cut.slices);
             else ND4J_LAUNCH((tokenProbsJoinKernel<T, false>), grid, block, 0, s, x, xv, tokens, out, work, cut.slices);
         }
         return;
