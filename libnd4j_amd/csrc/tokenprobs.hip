@@ -97,10 +97,10 @@ __global__ void __launch_bounds__(kRowThreads) tokenProbsAnyKernel(const T *x, R
 // ---- rows of contiguous elements, forward ------------------------------------------------------------------------------
 // One sweep of a row by a block: every thread keeps the maximum of its elements, the sum of exp(x - maximum) and of
 // (maximum - x) exp(x - maximum), rescaled where its next elements raise the maximum.  The alternatives cost that sweep
-// nothing: the k-th largest of the 64 thread maxima of any one wave is a lower bound of the row's k-th largest element, so
-// only threads whose maximum reaches the largest of these bounds hold alternatives - k of them and a few more, where
-// values differ - and only their elements are read again, by all threads together.  Where rows are few they are cut
-// into slices, whose sums and lists a second launch joins.
+// nothing: if k / 4 threads of each of the block's four waves have a maximum of at least b, the row's k-th largest element
+// is no less than b, and only threads whose maximum reaches b hold alternatives - k of them and a few more, where values
+// differ.  Only their elements are read again, by all threads together, and those that reach b (a few more than k) find
+// their places by counting.  Where rows are few they are cut into slices, whose sums and lists a second launch joins.
 //
 // (Keeping the best elements during the sweep, as the first form did, took 118 us over [4096, 32000] floats at k = 5, where
 // the sweep alone takes 81.)
@@ -211,17 +211,19 @@ __device__ __forceinline__ double valueOf(unsigned long long o) {
     return __builtin_bit_cast(double, (o >> 63) != 0ull ? o & 0x7fffffffffffffffull : ~o);
 }
 // the k-th largest of a wave's 64 values, by its bits from the highest on
-template <typename C> __device__ __forceinline__ C kthLargest(C v, int k) {
+// (down to bit `last`: a bound below it by what the lower bits may hold)
+template <typename C> __device__ __forceinline__ C kthLargest(C v, int k, int last) {
     const auto mine = orderOf(v);
     auto found = mine;
     found = 0;
 #pragma unroll 4
-    for (int bit = (int)sizeof(C) * 8 - 1; bit >= 0; bit--) {
+    for (int bit = (int)sizeof(C) * 8 - 1; bit >= last; bit--) {
         auto with = found;
         with |= (decltype(found))1 << bit;
         if (__popcll(__ballot(mine >= with)) >= k) found = with;
     }
-    return valueOf(found);
+    const C bound = valueOf(found);
+    return bound == bound ? bound : -infinite<C>();  // (what lies below minus infinity is written like a NaN)
 }
 
 // maximum, sum of exp(x - maximum), sum of (maximum - x) exp(x - maximum)
@@ -291,6 +293,8 @@ __global__ void __launch_bounds__(THREADS) tokenProbsRowsKernel(const T *x, RowV
     __shared__ C bounds[WAVES];
     __shared__ int hotCounts[WAVES];
     __shared__ short hot[THREADS];
+    __shared__ int found, candidateIndexes[TOP ? THREADS : 1];
+    __shared__ C candidates[TOP ? THREADS : 1];
     extern __shared__ __align__(16) char dynamicLds[];
     C *values = reinterpret_cast<C *>(dynamicLds);  // [WAVES][k], and as many indexes behind them
     int *indexes = reinterpret_cast<int *>(values + WAVES * out.k);
@@ -308,7 +312,7 @@ __global__ void __launch_bounds__(THREADS) tokenProbsRowsKernel(const T *x, RowV
             Pack<T> v[VECTORS];
             if (t + ROUND * VECTORS <= end) {
 #pragma unroll
-                for (int j = 0; j < VECTORS; j++) v[j] = loadPackAnywhere(xr + t + (j * THREADS + (int)threadIdx.x) * N);
+                for (int j = 0; j < VECTORS; j++) v[j] = streamPackAnywhere(xr + t + (j * THREADS + (int)threadIdx.x) * N);
             } else {
 #pragma unroll
                 for (int j = 0; j < VECTORS; j++) {
@@ -347,12 +351,22 @@ __global__ void __launch_bounds__(THREADS) tokenProbsRowsKernel(const T *x, RowV
         if (lane == 0) waveSums[wave] = s;
         BestList<C> best;
         if (TOP) {
-            const C waveBound = kthLargest(own, out.k);
+            constexpr int LAST = sizeof(T) == 2 ? 13 : 0;  // (a half's bits end there)
+            const C waveBound = kthLargest(own, (out.k + WAVES - 1) / WAVES, LAST);
             if (lane == 0) bounds[wave] = waveBound;
+            if (threadIdx.x == 0) found = 0;
             __syncthreads();
             C bound = bounds[0];
 #pragma unroll
-            for (int w = 1; w < WAVES; w++) bound = Largest()(bound, bounds[w]);
+            for (int w = 1; w < WAVES; w++) bound = bounds[w] < bound ? bounds[w] : bound;
+            if (WAVES > 1 && bound == -infinite<C>()) {  // a wave without as many elements: the k-th largest of any other will do
+                const C other = kthLargest(own, out.k, LAST);
+                __syncthreads();
+                if (lane == 0) bounds[wave] = other;
+                __syncthreads();
+#pragma unroll
+                for (int w = 0; w < WAVES; w++) bound = Largest()(bound, bounds[w]);
+            }
             const bool isHot = own >= bound;
             const unsigned long long mask = __ballot(isHot);
             if (lane == 0) hotCounts[wave] = __popcll(mask);
@@ -365,44 +379,95 @@ __global__ void __launch_bounds__(THREADS) tokenProbsRowsKernel(const T *x, RowV
             }
             if (isHot) hot[before + __popcll(mask & ((1ull << lane) - 1))] = (short)threadIdx.x;
             __syncthreads();
-            // vector q of hot thread h, 64 of them to a wave at a time; positions ascend over h and then q, so every list
-            // entry's index is compared in full
-            best.clear(out.k);
+            // Vector q of hot thread h is an item.  The elements that reach the bound are gathered, and each counts those
+            // that come before it, which is its place.
             const int rounds = (end - begin + ROUND - 1) / ROUND;
             const Long items = (Long)hots * rounds;
-            for (Long i = wave * kWaveLanes; i < items; i += THREADS) {
-                const Long item = i + lane;
+            auto itemAt = [&](Long item, int &c, Pack<T> &v) {
                 const int h = (int)(item / rounds), q = (int)(item - (Long)h * rounds);
-                const int c = item < items ? begin + (q * THREADS + hot[h]) * N : end;
-                Pack<T> v;
+                c = item < items ? begin + (q * THREADS + hot[h]) * N : end;
                 if (c + N <= end) {
                     v = loadPackAnywhere(xr + c);
                 } else {
 #pragma unroll
                     for (int e = 0; e < N; e++) v.v[e] = c + e < end ? xr[c + e] : fromCompute<T>((C)0);
                 }
-                unsigned offers = 0;  // a bit per element
+            };
+            for (Long i = wave * kWaveLanes; i < items; i += THREADS) {
+                int c;
+                Pack<T> v;
+                itemAt(i + lane, c, v);
 #pragma unroll
                 for (int e = 0; e < N; e++) {
                     const C value = toCompute(v.v[e]);
-                    if (c + e < end && value >= bound && best.beats(value, c + e)) offers |= 1u << e;
+                    const bool is = c + e < end && value >= bound;
+                    const unsigned long long which = __ballot(is);
+                    if (which == 0ull) continue;
+                    int place = 0;
+                    if (lane == 0) place = atomicAdd(&found, __popcll(which));
+                    place = __builtin_amdgcn_readfirstlane(place) + __popcll(which & ((1ull << lane) - 1));
+                    if (is && place < THREADS) {
+                        candidates[place] = value;
+                        candidateIndexes[place] = c + e;
+                    }
                 }
-                while (__ballot(offers != 0u) != 0ull) {
-                    const int which = __ffs((int)offers) - 1;
-                    C value = -infinite<C>();
-#pragma unroll
-                    for (int e = 0; e < N; e++)
-                        if (e == which) value = toCompute(v.v[e]);
-                    best.offer(value, c + which, offers != 0u);
-                    offers &= offers - 1;
-                }
+                if (*(volatile int *)&found > THREADS) break;
             }
-            if (WAVES > 1) {
-                if (lane < out.k) {
-                    values[wave * out.k + lane] = best.value;
-                    indexes[wave * out.k + lane] = best.index;
+            __syncthreads();
+            const int count = found;
+            if (count <= THREADS) {
+                C value = -infinite<C>();
+                int index = kNoIndex, place = threadIdx.x;
+                if ((int)threadIdx.x < count) {
+                    value = candidates[threadIdx.x];
+                    index = candidateIndexes[threadIdx.x];
+                    place = 0;
+#pragma unroll 4
+                    for (int j = 0; j < count; j++) {
+                        const C other = candidates[j];
+                        const int otherIndex = candidateIndexes[j];
+                        place += other > value || (other == value && otherIndex < index);
+                    }
+                }
+                if (place < out.k) {
+                    values[place] = value;
+                    indexes[place] = index;
                 }
                 __syncthreads();
+                best.value = lane < out.k ? values[lane] : -infinite<C>();
+                best.index = lane < out.k ? indexes[lane] : kNoIndex;
+            } else {
+                // More than that are as large as the bound - rows of few different values: every wave keeps a list of its items,
+                // and the lists are merged.
+                best.clear(out.k);
+                for (Long i = wave * kWaveLanes; i < items; i += THREADS) {
+                    int c;
+                    Pack<T> v;
+                    itemAt(i + lane, c, v);
+                    unsigned offers = 0;  // a bit per element
+#pragma unroll
+                    for (int e = 0; e < N; e++) {
+                        const C value = toCompute(v.v[e]);
+                        if (c + e < end && value >= bound && best.beats(value, c + e)) offers |= 1u << e;
+                    }
+                    while (__ballot(offers != 0u) != 0ull) {
+                        const int which = __ffs((int)offers) - 1;
+                        C value = -infinite<C>();
+#pragma unroll
+                        for (int e = 0; e < N; e++)
+                            if (e == which) value = toCompute(v.v[e]);
+                        best.offer(value, c + which, offers != 0u);
+                        offers &= offers - 1;
+                    }
+                }
+                if (WAVES > 1) {
+                    if (lane < out.k) {
+                        values[wave * out.k + lane] = best.value;
+                        indexes[wave * out.k + lane] = best.index;
+                    }
+                    __syncthreads();
+                    if (wave == 0) mergeLists<C>(best, WAVES, out.k, values, indexes);
+                }
             }
         } else if (WAVES > 1) {
             __syncthreads();
@@ -410,7 +475,6 @@ __global__ void __launch_bounds__(THREADS) tokenProbsRowsKernel(const T *x, RowV
         if (wave != 0) continue;
 #pragma unroll
         for (int w = 1; w < WAVES; w++) s.add(waveSums[w]);
-        if (TOP && WAVES > 1) mergeLists<C>(best, WAVES, out.k, values, indexes);
         if (slices == 1) {
             writeRow<T>(xv.length, r, token, tokenValue, out, s);
             if (TOP) writeBest<T>(r, out, s, best);
