@@ -282,17 +282,20 @@ __device__ __forceinline__ void writeBest(Long r, const TokenProbsOut<T> &out, c
         out.topLogProbs[r * out.k + lane] = !entry ? notANumber<C>() : (none ? -infinite<C>() : (best.value - from) - logSum);
 }
 
+// A slice's tiles fall into at most this many spans of equal length, of which every thread keeps its maxima
+constexpr int kSpans = 16;
+
 // A slice of a row leaves 3 + 2 k values for the join: its sums, and its list's values and indexes.
 
 template <typename T, int THREADS, int VECTORS, bool ENTROPY, bool TOP>
 __global__ void __launch_bounds__(THREADS) tokenProbsRowsKernel(const T *x, RowView xv, const Long *tokens, TokenProbsOut<T> out,
                                                                 typename Compute<T>::type *scratch, int slices, int sliceLength) {
     typedef typename Compute<T>::type C;
-    constexpr int N = Pack<T>::N, WAVES = THREADS / kWaveLanes, ROUND = THREADS * N;
+    constexpr int N = Pack<T>::N, WAVES = THREADS / kWaveLanes, ROUND = THREADS * N, TILE = ROUND * VECTORS;
     __shared__ Sums<C> waveSums[WAVES];
     __shared__ C bounds[WAVES];
-    __shared__ int hotCounts[WAVES];
-    __shared__ short hot[THREADS];
+    __shared__ C maxima[TOP ? kSpans : 1][THREADS];  // of a thread's elements in each span of tiles
+    __shared__ int hotCount, hot[TOP ? THREADS : 1];  // (span, thread) pairs that reach the bound
     __shared__ int found, candidateIndexes[TOP ? THREADS : 1];
     __shared__ C candidates[TOP ? THREADS : 1];
     extern __shared__ __align__(16) char dynamicLds[];
@@ -308,9 +311,12 @@ __global__ void __launch_bounds__(THREADS) tokenProbsRowsKernel(const T *x, RowV
         const C tokenValue = token >= 0 && token < xv.length ? toCompute(xr[token]) : (C)0;
         Sums<C> s;
         s.clear();
-        for (int t = begin; t < end; t += ROUND * VECTORS) {
+        const int tiles = (end - begin + TILE - 1) / TILE, spanTiles = (tiles + kSpans - 1) / kSpans;
+        int span = 0, spanLeft = spanTiles;
+        C spanLargest = -infinite<C>();
+        for (int t = begin; t < end; t += TILE) {
             Pack<T> v[VECTORS];
-            if (t + ROUND * VECTORS <= end) {
+            if (t + TILE <= end) {
 #pragma unroll
                 for (int j = 0; j < VECTORS; j++) v[j] = streamPackAnywhere(xr + t + (j * THREADS + (int)threadIdx.x) * N);
             } else {
@@ -330,6 +336,15 @@ __global__ void __launch_bounds__(THREADS) tokenProbsRowsKernel(const T *x, RowV
             for (int j = 0; j < VECTORS; j++)
 #pragma unroll
                 for (int e = 0; e < N; e++) tileLargest = Largest()(tileLargest, toCompute(v[j].v[e]));
+            if (TOP) {
+                spanLargest = Largest()(spanLargest, tileLargest);
+                maxima[span][threadIdx.x] = spanLargest;
+                if (--spanLeft == 0) {
+                    span++;
+                    spanLeft = spanTiles;
+                    spanLargest = -infinite<C>();
+                }
+            }
             s.raiseTo(tileLargest);
             const C from = s.largest > -infinite<C>() ? s.largest : (C)0;
 #pragma unroll
@@ -354,7 +369,7 @@ __global__ void __launch_bounds__(THREADS) tokenProbsRowsKernel(const T *x, RowV
             constexpr int LAST = sizeof(T) == 2 ? 13 : 0;  // (a half's bits end there)
             const C waveBound = kthLargest(own, (out.k + WAVES - 1) / WAVES, LAST);
             if (lane == 0) bounds[wave] = waveBound;
-            if (threadIdx.x == 0) found = 0;
+            if (threadIdx.x == 0) found = hotCount = 0;
             __syncthreads();
             C bound = bounds[0];
 #pragma unroll
@@ -367,25 +382,29 @@ __global__ void __launch_bounds__(THREADS) tokenProbsRowsKernel(const T *x, RowV
 #pragma unroll
                 for (int w = 0; w < WAVES; w++) bound = Largest()(bound, bounds[w]);
             }
-            const bool isHot = own >= bound;
-            const unsigned long long mask = __ballot(isHot);
-            if (lane == 0) hotCounts[wave] = __popcll(mask);
-            __syncthreads();
-            int before = 0, hots = 0;
-#pragma unroll
-            for (int w = 0; w < WAVES; w++) {
-                if (w == wave) before = hots;
-                hots += hotCounts[w];
+            if (own >= bound) {
+                for (int k = 0; k * spanTiles < tiles; k++)
+                    if (maxima[k][threadIdx.x] >= bound) {
+                        const int place = atomicAdd(&hotCount, 1);
+                        if (place < THREADS) hot[place] = k * THREADS + (int)threadIdx.x;
+                    }
             }
-            if (isHot) hot[before + __popcll(mask & ((1ull << lane) - 1))] = (short)threadIdx.x;
             __syncthreads();
-            // Vector q of hot thread h is an item.  The elements that reach the bound are gathered, and each counts those
-            // that come before it, which is its place.
-            const int rounds = (end - begin + ROUND - 1) / ROUND;
-            const Long items = (Long)hots * rounds;
+            // The vectors of the hot pairs - where there are too many of them, all vectors - are the items.  The elements that
+            // reach the bound are gathered, and each counts those that come before it, which is its place.
+            const int hots = hotCount, perPair = spanTiles * VECTORS;
+            const bool few = hots <= THREADS;
+            const Long items = few ? (Long)hots * perPair : ((Long)end - begin + N - 1) / N;
             auto itemAt = [&](Long item, int &c, Pack<T> &v) {
-                const int h = (int)(item / rounds), q = (int)(item - (Long)h * rounds);
-                c = item < items ? begin + (q * THREADS + hot[h]) * N : end;
+                c = end;
+                if (item < items) {
+                    Long at = item;
+                    if (few) {
+                        const int h = (int)item / perPair, q = (int)item - h * perPair, pair = hot[h], k = pair / THREADS;
+                        at = (Long)(k * perPair + q) * THREADS + pair % THREADS;
+                    }
+                    if (at * N < end - begin) c = begin + (int)at * N;
+                }
                 if (c + N <= end) {
                     v = loadPackAnywhere(xr + c);
                 } else {
