@@ -30,6 +30,58 @@ __global__ void __launch_bounds__(kThreads) embeddingAnyKernel(const T *table, R
     }
 }
 
+// Rows of contiguous elements: a thread takes vectors of 16 bytes of the rows as they lie behind each other, kInFlight of
+// them at a time, since each waits for its token first and for the table then.
+constexpr int kInFlight = 4;
+template <typename T>
+__global__ void __launch_bounds__(kThreads) embeddingRowsKernel(const T *table, RowView tv, const Long *tokens, T *z, RowView zv,
+                                                                typename Compute<T>::type scale, FastDiv perRow, unsigned units) {
+    typedef typename Compute<T>::type C;
+    constexpr int N = Pack<T>::N;
+    const int length = (int)zv.length;
+    const unsigned step = gridDim.x * kThreads;
+    for (unsigned long long first = (unsigned long long)blockIdx.x * kThreads + threadIdx.x; first < units; first += (unsigned long long)step * kInFlight) {
+        unsigned row[kInFlight];
+        int c[kInFlight];
+        Long t[kInFlight];
+        Pack<T> v[kInFlight];
+#pragma unroll
+        for (int k = 0; k < kInFlight; k++) {
+            const unsigned long long u = first + (unsigned long long)k * step;
+            unsigned vec;
+            row[k] = perRow.divmod(u < units ? (unsigned)u : (unsigned)first, vec);  // (behind the end: the first one again)
+            c[k] = (int)vec * N;
+            t[k] = tokens[row[k]];
+        }
+#pragma unroll
+        for (int k = 0; k < kInFlight; k++) {
+            const T *from = table + (t[k] >= 0 && t[k] < tv.rows ? t[k] : 0) * tv.row + c[k];
+            if (c[k] + N <= length) {
+                v[k] = loadPackAnywhere(from);
+            } else {
+#pragma unroll
+                for (int e = 0; e < N; e++) v[k].v[e] = c[k] + e < length ? from[e] : fromCompute<T>((C)0);
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < kInFlight; k++) {
+            if (first + (unsigned long long)k * step >= units) break;
+            const C other = t[k] < 0 ? (C)0 : notANumber<C>();
+            const bool has = t[k] >= 0 && t[k] < tv.rows;
+#pragma unroll
+            for (int e = 0; e < N; e++) v[k].v[e] = fromCompute<T>(has ? toCompute(v[k].v[e]) * scale : other);
+            T *to = z + (Long)row[k] * zv.row + c[k];
+            if (c[k] + N <= length) {
+                streamPackAnywhere(to, v[k]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < N; e++)
+                    if (c[k] + e < length) to[e] = v[k].v[e];
+            }
+        }
+    }
+}
+
 // ---- sorting the tokens ----------------------------------------------------------------------------------------------
 // Least significant digit first, 8 bits a pass.  A block counts the digits of its tile (a multiple of kSubTile tokens), a
 // second launch places the tile's tokens behind those of lower digits and of the blocks before it.  At most kSortBlocks
@@ -352,6 +404,17 @@ size_t embeddingBpScratch(Long n, Long vocabulary, Long length) { return layoutO
 template <typename T>
 void launchEmbedding(hipStream_t s, const T *table, const RowView &tv, const Long *tokens, T *z, const RowView &zv, double scale) {
     typedef typename Compute<T>::type C;
+    if (tv.el == 1 && zv.el == 1 && tv.rows > 0) {
+        // (FastDiv takes units below 2^31: more are several launches of whole rows)
+        const Long perRow = (zv.length + Pack<T>::N - 1) / Pack<T>::N, most = (((Long)1 << 31) - 1) / perRow;
+        for (Long r = 0; r < zv.rows; r += most) {
+            const Long rows = zv.rows - r < most ? zv.rows - r : most;
+            const unsigned units = (unsigned)(rows * perRow);
+            ND4J_LAUNCH((embeddingRowsKernel<T>), dim3(gridFor(units, (Long)kThreads * kInFlight, kGridCap)), dim3(kThreads), 0, s, table, tv,
+                        tokens + r, z + r * zv.row, zv, (C)scale, FastDiv((unsigned)perRow), units);
+        }
+        return;
+    }
     ND4J_LAUNCH((embeddingAnyKernel<T>), dim3(gridFor(zv.rows * zv.length, kThreads, kGridCap)), dim3(kThreads), 0, s, table, tv, tokens, z, zv,
                 (C)scale);
 }
