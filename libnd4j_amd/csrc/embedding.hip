@@ -6,6 +6,10 @@
 // into chunks of equal length, sums every run of equal tokens inside a chunk in a wave's registers, and joins the runs that
 // cross chunks in the chunks' order: no atomics on values, the same bits from every run, and a token that comes a hundred
 // thousand times is shared by many waves.  Sums are held in the compute type and rounded to the storage type once.
+//
+// The sort's launches are a few small blocks that wait for memory; unless the gradient is added onto what the table holds,
+// the rest of the chip clears the table meanwhile, the rows that get sums later among them (they are few where clearing
+// takes long: clearing only the others, behind the sort, made [16384 of 32000, 768] floats 65 us).
 #include "launch.h"
 #include "training.cuh"
 
@@ -93,14 +97,43 @@ constexpr int kSortBlocks = 256;
 // the sort key of token t: tokens outside the table come last, under the key `vocabulary`
 __device__ __forceinline__ unsigned keyOf(Long t, unsigned vocabulary) { return t >= 0 && t < (Long)vocabulary ? (unsigned)t : vocabulary; }
 
+// A share of a table to be cleared, by the blocks of a launch from `firstBlock` on: `rows` rows of `bytes` bytes a `pitch` apart,
+// or, where elements are `apart` bytes from each other, of bytes / size elements
+struct Clearing {
+    char *base = nullptr;
+    Long rows = 0, bytes = 0, pitch = 0, apart = 0;
+    int size = 0;
+    unsigned firstBlock = 0;
+};
+typedef U32x4 U32x4Any __attribute__((aligned(2)));  // (the least that an element is aligned to)
+__device__ __forceinline__ void clearShare(const Clearing &c) {
+    constexpr int WAVES = kThreads / kWaveLanes;
+    const int lane = threadIdx.x % kWaveLanes;
+    const Long each = (Long)(gridDim.x - c.firstBlock) * WAVES;
+    for (Long r = (Long)(blockIdx.x - c.firstBlock) * WAVES + threadIdx.x / kWaveLanes; r < c.rows; r += each) {
+        char *row = c.base + r * c.pitch;
+        if (c.apart == c.size) {
+            const U32x4 zero = {0u, 0u, 0u, 0u};
+            for (Long at = (Long)lane * 16; at < c.bytes; at += kWaveLanes * 16) {
+                if (at + 16 <= c.bytes) {
+                    __builtin_nontemporal_store(zero, reinterpret_cast<U32x4Any *>(row + at));
+                } else {
+                    for (Long b = at; b < c.bytes; b += 2) *reinterpret_cast<unsigned short *>(row + b) = 0;
+                }
+            }
+        } else {
+            for (Long e = lane; e < c.bytes / c.size; e += kWaveLanes)
+                for (int b = 0; b < c.size; b += 2) *reinterpret_cast<unsigned short *>(row + e * c.apart + b) = 0;
+        }
+    }
+}
+__global__ void __launch_bounds__(kThreads) clearKernel(Clearing clearing) { clearShare(clearing); }
+
 __global__ void __launch_bounds__(kThreads) sortCountKernel(const Long *tokens, const unsigned *keys, unsigned n, unsigned vocabulary,
-                                                            unsigned tile, int shift, unsigned *counts, unsigned char *present) {
+                                                            unsigned tile, int shift, unsigned *counts, Clearing clearing) {
     __shared__ unsigned local[kDigits];
+    if (blockIdx.x >= clearing.firstBlock) return clearShare(clearing);
     local[threadIdx.x] = 0;
-    // the first pass clears the table of the tokens that occur (a whole number of words, see sortScratch)
-    if (present != nullptr)
-        for (size_t i = (size_t)blockIdx.x * kThreads + threadIdx.x; i < ((size_t)vocabulary + 4) / 4; i += (size_t)gridDim.x * kThreads)
-            reinterpret_cast<unsigned *>(present)[i] = 0u;
     __syncthreads();
     const unsigned long long first = (unsigned long long)blockIdx.x * tile;
     const unsigned end = (unsigned)(first + tile < n ? first + tile : n);
@@ -114,15 +147,17 @@ __global__ void __launch_bounds__(kThreads) sortCountKernel(const Long *tokens, 
 
 __global__ void __launch_bounds__(kThreads) sortPlaceKernel(const Long *tokens, const unsigned *keys, const unsigned *positions, unsigned n,
                                                             unsigned vocabulary, unsigned tile, int shift, const unsigned *counts,
-                                                            unsigned *keysOut, unsigned *positionsOut, unsigned char *present) {
+                                                            unsigned *keysOut, unsigned *positionsOut, Clearing clearing) {
     constexpr int WAVES = kThreads / kWaveLanes;
     __shared__ unsigned starts[kDigits];
     __shared__ unsigned waveCounts[WAVES][kDigits];
     const int d = threadIdx.x, lane = threadIdx.x % kWaveLanes, wave = threadIdx.x / kWaveLanes;
+    const unsigned blocks = clearing.firstBlock;
+    if (blockIdx.x >= blocks) return clearShare(clearing);
     // where this block's tokens of digit d begin: all tokens of lower digits, then those of digit d in the blocks before
     unsigned before = 0, whole = 0;
 #pragma unroll 8
-    for (unsigned b = 0; b < gridDim.x; b++) {
+    for (unsigned b = 0; b < blocks; b++) {
         const unsigned c = counts[(size_t)b * kDigits + d];
         whole += c;
         if (b < blockIdx.x) before += c;
@@ -190,7 +225,6 @@ __global__ void __launch_bounds__(kThreads) sortPlaceKernel(const Long *tokens, 
                 const unsigned to = waveCounts[wave][(key[k] >> shift) & (kDigits - 1)] + rank[k];
                 keysOut[to] = key[k];
                 positionsOut[to] = position[k];
-                if (present != nullptr) present[key[k]] = 1;  // (the table has a place for the key `vocabulary` too)
             }
         }
         __syncthreads();
@@ -250,26 +284,14 @@ template <typename C> __device__ __forceinline__ C *partialRow(C *partial, unsig
     return partial + ((size_t)chunk * 2 + which) * length;
 }
 
-// A wave takes one chunk and one tile of columns.  The blocks behind those clear the rows of tokens that do not occur.
+// A wave takes one chunk and one tile of columns.
 template <typename T, bool UNIT>
 __global__ void __launch_bounds__(kThreads) embeddingBpSumKernel(const T *dz, RowView dzv, const unsigned *keys, const unsigned *positions,
                                                                  SumPlan plan, T *dTable, RowView tv, typename Compute<T>::type scale,
-                                                                 int accumulate, typename Compute<T>::type *partial,
-                                                                 const unsigned char *present, unsigned sumBlocks) {
+                                                                 int accumulate, typename Compute<T>::type *partial) {
     typedef typename Compute<T>::type C;
     constexpr int N = Pack<T>::N, WAVES = kThreads / kWaveLanes;
     const int lane = threadIdx.x % kWaveLanes, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWaveLanes);
-    if (blockIdx.x >= sumBlocks) {
-        C zero[N];
-#pragma unroll
-        for (int e = 0; e < N; e++) zero[e] = (C)0;
-        for (Long v = (Long)(blockIdx.x - sumBlocks) * WAVES + wave; v < (Long)plan.vocabulary; v += (Long)(gridDim.x - sumBlocks) * WAVES) {
-            if (present[v]) continue;
-            for (Long c = (Long)lane * N; c < plan.length; c += kWaveLanes * N)
-                storeSum<T, UNIT>(dTable + v * tv.row, tv.el, c, plan.length, zero, (C)0, false);
-        }
-        return;
-    }
     const unsigned long long work = (unsigned long long)blockIdx.x * WAVES + wave;
     if (work >= (unsigned long long)plan.chunks * plan.tiles) return;
     const unsigned chunk = (unsigned)(work / plan.tiles), tile = (unsigned)(work % plan.tiles);
@@ -340,13 +362,17 @@ __global__ void __launch_bounds__(kThreads) embeddingBpJoinKernel(const unsigned
     const unsigned key = keys[behind - 1];
     if (key >= plan.vocabulary || keys[behind] != key) return;
     if (first > 0 && keys[first] == key && keys[first - 1] == key) return;  // began earlier
-    unsigned long long low = behind + 1, high = plan.n;                     // the run ends in [low, high]
-    while (low < high) {
-        const unsigned long long mid = (low + high) >> 1;
-        if (keys[mid] == key) low = mid + 1;
-        else high = mid;
+    // the run reaches into every chunk that begins with its key, as far as these follow each other: 64 looked at a time
+    unsigned lastChunk = chunk + 1;
+    for (;;) {
+        const unsigned long long next = (unsigned long long)lastChunk + 1 + lane, at = next * plan.chunk;
+        const unsigned long long other = __ballot(!(at < plan.n && keys[at < plan.n ? at : 0] == key));
+        if (other != 0ull) {
+            lastChunk += (unsigned)__ffsll(other) - 1;
+            break;
+        }
+        lastChunk += kWaveLanes;
     }
-    const unsigned lastChunk = (unsigned)((low - 1) / plan.chunk);
     const Long c0 = ((Long)tile * kWaveLanes + lane) * N;
     C acc[N];
 #pragma unroll
@@ -368,6 +394,8 @@ __global__ void __launch_bounds__(kThreads) embeddingBpJoinKernel(const unsigned
     storeSum<T, UNIT>(dTable + (Long)key * tv.row, tv.el, c0, plan.length, acc, scale, accumulate != 0);
 }
 
+constexpr Long kClearPiece = 16384;
+
 // the chunk's length: long enough that few runs cross chunks, short enough that a few thousand waves share a small batch
 int chunkOf(Long n) { return n >= (1 << 18) ? kMostChunk : (n >= (1 << 14) ? 32 : 16); }
 
@@ -375,9 +403,9 @@ size_t aligned(size_t bytes) { return (bytes + 255) & ~(size_t)255; }
 
 // the scratch's parts, in bytes from its start
 struct Layout {
-    size_t keys[2], positions[2], counts, present, partial, bytes;
+    size_t keys[2], positions[2], counts, partial, bytes;
 };
-Layout layoutOf(Long n, Long vocabulary, Long length) {
+Layout layoutOf(Long n, Long length) {
     Layout l;
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t here = at; at += aligned(bytes); return here; };
@@ -386,7 +414,6 @@ Layout layoutOf(Long n, Long vocabulary, Long length) {
         l.positions[i] = take((size_t)n * 4);
     }
     l.counts = take((size_t)kSortBlocks * kDigits * 4);
-    l.present = take((size_t)vocabulary + 8);
     const Long chunk = chunkOf(n), chunks = (n + chunk - 1) / chunk;
     l.partial = take((size_t)chunks * 2 * length * sizeof(double));
     l.bytes = at;
@@ -399,7 +426,7 @@ bool embeddingBpFits(Long n, Long length) {
     const Long chunk = chunkOf(n), tiles = length / (kWaveLanes * Pack<double>::N) + 1;
     return n / chunk + 1 < ((Long)1 << 30) / tiles;
 }
-size_t embeddingBpScratch(Long n, Long vocabulary, Long length) { return layoutOf(n, vocabulary, length).bytes; }
+size_t embeddingBpScratch(Long n, Long length) { return layoutOf(n, length).bytes; }
 
 template <typename T>
 void launchEmbedding(hipStream_t s, const T *table, const RowView &tv, const Long *tokens, T *z, const RowView &zv, double scale) {
@@ -424,7 +451,55 @@ void launchEmbeddingBp(hipStream_t s, const T *dz, const RowView &dzv, const Lon
                        bool accumulate, void *scratch) {
     typedef typename Compute<T>::type C;
     const unsigned n = (unsigned)dzv.rows, vocabulary = (unsigned)tv.rows;
-    const Layout l = layoutOf(n, vocabulary, tv.length);
+    int bits = 1;
+    while (bits < 32 && ((unsigned long long)1 << bits) <= vocabulary) bits++;  // the key `vocabulary` occurs too
+    const int passes = (bits + kSortBits - 1) / kSortBits;
+
+    // The table to be cleared, in equal shares for the sort's launches.  Rows that follow each other without gaps are one
+    // stretch, cut into pieces of kClearPiece bytes, of which a last, shorter one goes with the last share.
+    Clearing all;
+    Long lastPiece = 0;
+    if (!accumulate) {
+        all.base = reinterpret_cast<char *>(dTable);
+        all.size = (int)sizeof(T);
+        all.rows = tv.rows;
+        all.bytes = tv.length * sizeof(T);
+        all.pitch = tv.row * sizeof(T);
+        all.apart = tv.el * sizeof(T);
+        if (tv.el == 1 && (tv.row == tv.length || tv.rows == 1)) {
+            const Long bytes = tv.rows * all.bytes;
+            all.rows = bytes / kClearPiece;
+            lastPiece = bytes % kClearPiece;
+            all.bytes = all.pitch = kClearPiece;
+        }
+    }
+    int sharesLeft = n == 0 ? 1 : 2 * passes;
+    auto nextShare = [&](unsigned blocks) {
+        Clearing share = all;
+        share.firstBlock = blocks;
+        share.rows = all.rows / sharesLeft;
+        all.base += share.rows * all.pitch;
+        all.rows -= share.rows;
+        sharesLeft--;
+        return share;
+    };
+    auto gridWith = [&](const Clearing &share) {
+        return dim3(share.firstBlock + (share.rows > 0 ? (unsigned)gridFor(share.rows, kThreads / kWaveLanes, 4096) : 0u));
+    };
+    if (lastPiece > 0) {
+        Clearing piece = all;
+        piece.base += all.rows * all.pitch;
+        piece.rows = 1;
+        piece.bytes = lastPiece;
+        ND4J_LAUNCH(clearKernel, dim3(1), dim3(kThreads), 0, s, piece);
+    }
+    if (n == 0) {
+        const Clearing share = nextShare(0);
+        if (share.rows > 0) ND4J_LAUNCH(clearKernel, gridWith(share), dim3(kThreads), 0, s, share);
+        return;
+    }
+
+    const Layout l = layoutOf(n, tv.length);
     char *base = reinterpret_cast<char *>(scratch);
     unsigned *keys[2], *positions[2];
     for (int i = 0; i < 2; i++) {
@@ -432,22 +507,19 @@ void launchEmbeddingBp(hipStream_t s, const T *dz, const RowView &dzv, const Lon
         positions[i] = reinterpret_cast<unsigned *>(base + l.positions[i]);
     }
     unsigned *counts = reinterpret_cast<unsigned *>(base + l.counts);
-    unsigned char *present = reinterpret_cast<unsigned char *>(base + l.present);
     C *partial = reinterpret_cast<C *>(base + l.partial);
-    int bits = 1;
-    while (bits < 32 && ((unsigned long long)1 << bits) <= vocabulary) bits++;  // the key `vocabulary` occurs too
-    // (a grid of no blocks is not a launch: without tokens one block clears the table of those that occur)
     const unsigned tile = (unsigned)(((n + (unsigned long long)kSortBlocks * kSubTile - 1) / ((unsigned long long)kSortBlocks * kSubTile)) *
                                      kSubTile);
-    const unsigned blocks = n == 0 ? 1 : (unsigned)(((unsigned long long)n + tile - 1) / tile);
+    const unsigned blocks = (unsigned)(((unsigned long long)n + tile - 1) / tile);
     const unsigned *from = nullptr, *fromPositions = nullptr;
     int to = 0;
-    for (int shift = 0; shift < bits; shift += kSortBits) {
-        ND4J_LAUNCH(sortCountKernel, dim3(blocks), dim3(kThreads), 0, s, tokens, from, n, vocabulary, tile, shift, counts,
-                    shift == 0 ? present : nullptr);
-        if (n == 0) break;
-        ND4J_LAUNCH(sortPlaceKernel, dim3(blocks), dim3(kThreads), 0, s, tokens, from, fromPositions, n, vocabulary, tile, shift, counts,
-                    keys[to], positions[to], shift == 0 ? present : nullptr);
+    for (int pass = 0; pass < passes; pass++) {
+        const int shift = pass * kSortBits;
+        Clearing share = nextShare(blocks);
+        ND4J_LAUNCH(sortCountKernel, gridWith(share), dim3(kThreads), 0, s, tokens, from, n, vocabulary, tile, shift, counts, share);
+        share = nextShare(blocks);
+        ND4J_LAUNCH(sortPlaceKernel, gridWith(share), dim3(kThreads), 0, s, tokens, from, fromPositions, n, vocabulary, tile, shift, counts,
+                    keys[to], positions[to], share);
         from = keys[to];
         fromPositions = positions[to];
         to ^= 1;
@@ -461,16 +533,13 @@ void launchEmbeddingBp(hipStream_t s, const T *dz, const RowView &dzv, const Lon
     plan.tiles = (unsigned)((tv.length + kWaveLanes * Pack<T>::N - 1) / (kWaveLanes * Pack<T>::N));
     constexpr int WAVES = kThreads / kWaveLanes;
     const unsigned sumBlocks = (unsigned)(((unsigned long long)plan.chunks * plan.tiles + WAVES - 1) / WAVES);
-    const unsigned clearBlocks = accumulate ? 0 : (unsigned)gridFor(vocabulary, WAVES, 1 << 16);
     const bool unit = dzv.el == 1 && tv.el == 1;
-    if (sumBlocks + clearBlocks > 0) {
-        if (unit)
-            ND4J_LAUNCH((embeddingBpSumKernel<T, true>), dim3(sumBlocks + clearBlocks), dim3(kThreads), 0, s, dz, dzv, from, fromPositions, plan,
-                        dTable, tv, (C)scale, accumulate ? 1 : 0, partial, present, sumBlocks);
-        else
-            ND4J_LAUNCH((embeddingBpSumKernel<T, false>), dim3(sumBlocks + clearBlocks), dim3(kThreads), 0, s, dz, dzv, from, fromPositions, plan,
-                        dTable, tv, (C)scale, accumulate ? 1 : 0, partial, present, sumBlocks);
-    }
+    if (unit)
+        ND4J_LAUNCH((embeddingBpSumKernel<T, true>), dim3(sumBlocks), dim3(kThreads), 0, s, dz, dzv, from, fromPositions, plan, dTable, tv,
+                    (C)scale, accumulate ? 1 : 0, partial);
+    else
+        ND4J_LAUNCH((embeddingBpSumKernel<T, false>), dim3(sumBlocks), dim3(kThreads), 0, s, dz, dzv, from, fromPositions, plan, dTable, tv,
+                    (C)scale, accumulate ? 1 : 0, partial);
     if (plan.chunks > 1) {
         const unsigned joinBlocks = (plan.chunks - 1) * plan.tiles;
         if (unit)

@@ -172,7 +172,7 @@ void embeddingBp(Nd4jPointer *extra, T *dz, Long *dzInfo, Long *tokens, Long n, 
         must(op, "dz", dz);
         must(op, "tokens", tokens);
     }
-    void *work = scratchFor(op, s, scratch, scratchBytes, embeddingBpScratch(n, tv.rows, tv.length));
+    void *work = scratchFor(op, s, scratch, scratchBytes, n > 0 ? embeddingBpScratch(n, tv.length) : 0);
     launchEmbeddingBp<T>(s, dz, dzv, tokens, dTable, tv, scale, accumulate != 0, work);
     checkLaunch(op, s);
 }
@@ -265,7 +265,7 @@ Long embeddingBpScratchBytes(Long n, Long vocabulary, Long length) {
     if (n < 0 || vocabulary < 0 || length < 1 || n > kMostLength || vocabulary > kMostLength || length > kMostLength)
         refuse(op, "the number of tokens, the vocabulary or the length is out of range");
     if (!embeddingBpFits(n, length)) refuse(op, "too many elements");
-    return (Long)embeddingBpScratch(n, vocabulary, length);
+    return (Long)embeddingBpScratch(n, length);
 }
 Long tokenLogProbsScratchBytes(Long rows, Long length, int k) {
     const char *op = "scratchTokenLogProbs";

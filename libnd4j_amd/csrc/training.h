@@ -37,7 +37,7 @@ void launchEmbedding(hipStream_t stream, const T *table, const RowView &tv, cons
 template <typename T>
 void launchEmbeddingBp(hipStream_t stream, const T *dz, const RowView &dzv, const Long *tokens, T *dTable, const RowView &tv, double scale,
                        bool accumulate, void *scratch);
-size_t embeddingBpScratch(Long n, Long vocabulary, Long length);
+size_t embeddingBpScratch(Long n, Long length);
 bool embeddingBpFits(Long n, Long length);  // whether its grids hold n tokens of rows of this length
 
 // ---- log probabilities of tokens (tokenprobs.hip) ------------------------------------------------------------------------
