@@ -102,23 +102,24 @@ __device__ __forceinline__ unsigned keyOf(Long t, unsigned vocabulary) { return 
 struct Clearing {
     char *base = nullptr;
     Long rows = 0, bytes = 0, pitch = 0, apart = 0;
+    Long lastBytes = 0;  // of the last row
     int size = 0;
     unsigned firstBlock = 0;
 };
 typedef U32x4 U32x4Any __attribute__((aligned(2)));  // (the least that an element is aligned to)
 __device__ __forceinline__ void clearShare(const Clearing &c) {
-    constexpr int WAVES = kThreads / kWaveLanes;
-    const int lane = threadIdx.x % kWaveLanes;
-    const Long each = (Long)(gridDim.x - c.firstBlock) * WAVES;
-    for (Long r = (Long)(blockIdx.x - c.firstBlock) * WAVES + threadIdx.x / kWaveLanes; r < c.rows; r += each) {
+    const int lane = threadIdx.x % kWaveLanes, waves = blockDim.x / kWaveLanes;
+    const Long each = (Long)(gridDim.x - c.firstBlock) * waves;
+    for (Long r = (Long)(blockIdx.x - c.firstBlock) * waves + threadIdx.x / kWaveLanes; r < c.rows; r += each) {
         char *row = c.base + r * c.pitch;
         if (c.apart == c.size) {
             const U32x4 zero = {0u, 0u, 0u, 0u};
-            for (Long at = (Long)lane * 16; at < c.bytes; at += kWaveLanes * 16) {
-                if (at + 16 <= c.bytes) {
+            const Long bytes = r + 1 < c.rows ? c.bytes : c.lastBytes;
+            for (Long at = (Long)lane * 16; at < bytes; at += kWaveLanes * 16) {
+                if (at + 16 <= bytes) {
                     __builtin_nontemporal_store(zero, reinterpret_cast<U32x4Any *>(row + at));
                 } else {
-                    for (Long b = at; b < c.bytes; b += 2) *reinterpret_cast<unsigned short *>(row + b) = 0;
+                    for (Long b = at; b < bytes; b += 2) *reinterpret_cast<unsigned short *>(row + b) = 0;
                 }
             }
         } else {
@@ -145,11 +146,39 @@ __global__ void __launch_bounds__(kThreads) sortCountKernel(const Long *tokens, 
     counts[(size_t)blockIdx.x * kDigits + threadIdx.x] = local[threadIdx.x];
 }
 
+// How many of the wave's live lanes below this one have the same digit; whole: how many lanes have it in all
+__device__ __forceinline__ unsigned equalBelow(unsigned digit, bool live, unsigned &whole) {
+    unsigned long long equal = __ballot(live);
+#pragma unroll
+    for (int bit = 0; bit < kSortBits; bit++) {
+        const unsigned long long set = __ballot((digit >> bit) & 1);
+        equal &= (digit >> bit) & 1 ? set : ~set;
+    }
+    whole = (unsigned)__popcll(equal);
+    return (unsigned)__popcll(equal & ((1ull << (threadIdx.x % kWaveLanes)) - 1));
+}
+// where a digit's tokens begin, for the thread of that digit: the sum over lower digits (threads 0 .. 255; all threads of the
+// block call it)
+__device__ __forceinline__ unsigned digitStart(unsigned mine, unsigned *waveTotals) {
+    const int lane = threadIdx.x % kWaveLanes, wave = threadIdx.x / kWaveLanes;
+    unsigned sum = mine;
+#pragma unroll
+    for (int step = 1; step < kWaveLanes; step <<= 1) {
+        const unsigned v = __shfl_up(sum, step);
+        if (lane >= step) sum += v;
+    }
+    if (lane == kWaveLanes - 1 && wave < kDigits / kWaveLanes) waveTotals[wave] = sum;
+    __syncthreads();
+    sum -= mine;
+    for (int w = 0; w < wave && w < kDigits / kWaveLanes; w++) sum += waveTotals[w];
+    return sum;
+}
+
 __global__ void __launch_bounds__(kThreads) sortPlaceKernel(const Long *tokens, const unsigned *keys, const unsigned *positions, unsigned n,
                                                             unsigned vocabulary, unsigned tile, int shift, const unsigned *counts,
                                                             unsigned *keysOut, unsigned *positionsOut, Clearing clearing) {
     constexpr int WAVES = kThreads / kWaveLanes;
-    __shared__ unsigned starts[kDigits];
+    __shared__ unsigned starts[kDigits], waveTotals[WAVES];
     __shared__ unsigned waveCounts[WAVES][kDigits];
     const int d = threadIdx.x, lane = threadIdx.x % kWaveLanes, wave = threadIdx.x / kWaveLanes;
     const unsigned blocks = clearing.firstBlock;
@@ -162,17 +191,7 @@ __global__ void __launch_bounds__(kThreads) sortPlaceKernel(const Long *tokens, 
         whole += c;
         if (b < blockIdx.x) before += c;
     }
-    starts[d] = whole;
-    __syncthreads();
-    for (int step = 1; step < kDigits; step <<= 1) {
-        const unsigned v = d >= step ? starts[d - step] : 0u;
-        __syncthreads();
-        starts[d] += v;
-        __syncthreads();
-    }
-    const unsigned mine = starts[d] - whole + before;
-    __syncthreads();
-    starts[d] = mine;
+    starts[d] = digitStart(whole, waveTotals) + before;
     const unsigned long long first = (unsigned long long)blockIdx.x * tile;
     const unsigned long long end = first + tile < n ? first + tile : n;
     for (unsigned long long at = first; at < end; at += kSubTile) {
@@ -193,18 +212,13 @@ __global__ void __launch_bounds__(kThreads) sortPlaceKernel(const Long *tokens, 
                 position[k] = positions != nullptr ? positions[i] : (unsigned)i;
             }
             const unsigned digit = (key[k] >> shift) & (kDigits - 1);
-            unsigned long long equal = __ballot(live);
-#pragma unroll
-            for (int bit = 0; bit < kSortBits; bit++) {
-                const unsigned long long set = __ballot((digit >> bit) & 1);
-                equal &= (digit >> bit) & 1 ? set : ~set;
-            }
-            const unsigned lower = __popcll(equal & ((1ull << lane) - 1));
+            unsigned whole;
+            const unsigned lower = equalBelow(digit, live, whole);
             rank[k] = 0;
             if (live) {
                 const unsigned seen = mineCounts[digit];
                 rank[k] = seen + lower;
-                if (lower == 0) mineCounts[digit] = seen + (unsigned)__popcll(equal);
+                if (lower == 0) mineCounts[digit] = seen + whole;
             }
             __builtin_amdgcn_wave_barrier();
         }
@@ -231,6 +245,88 @@ __global__ void __launch_bounds__(kThreads) sortPlaceKernel(const Long *tokens, 
     }
 }
 
+// Up to kSmallSort tokens: one block does all passes in LDS, in one launch instead of two a pass.
+constexpr int kSmallThreads = 1024, kSmallRounds = 4, kSmallSort = kSmallThreads * kSmallRounds;
+__global__ void __launch_bounds__(kSmallThreads) sortSmallKernel(const Long *tokens, unsigned n, unsigned vocabulary, int passes, unsigned *keysOut,
+                                                                 unsigned *positionsOut, Clearing clearing) {
+    constexpr int WAVES = kSmallThreads / kWaveLanes;
+    __shared__ unsigned sortedKeys[kSmallSort], sortedPositions[kSmallSort];
+    __shared__ unsigned short waveCounts[WAVES][kDigits];
+    __shared__ unsigned waveTotals[WAVES];
+    if (blockIdx.x >= clearing.firstBlock) return clearShare(clearing);
+    const int d = threadIdx.x, lane = threadIdx.x % kWaveLanes, wave = threadIdx.x / kWaveLanes;
+    const int rounds = (int)((n + kSmallThreads - 1) / kSmallThreads);  // a wave's tokens: rounds x 64 consecutive ones
+    unsigned key[kSmallRounds], position[kSmallRounds], rank[kSmallRounds];
+#pragma unroll
+    for (int k = 0; k < kSmallRounds; k++) {
+        const unsigned i = (unsigned)(wave * rounds + k) * kWaveLanes + lane;
+        key[k] = k < rounds && i < n ? keyOf(tokens[i], vocabulary) : 0u;
+        position[k] = i;
+    }
+    for (int pass = 0; pass < passes; pass++) {
+        const int shift = pass * kSortBits;
+        for (int i = threadIdx.x; i < WAVES * kDigits; i += kSmallThreads) (&waveCounts[0][0])[i] = 0;
+        __syncthreads();
+        volatile unsigned short *mineCounts = waveCounts[wave];
+#pragma unroll
+        for (int k = 0; k < kSmallRounds; k++) {
+            if (k >= rounds) break;
+            const bool live = (unsigned)(wave * rounds + k) * kWaveLanes + lane < n;
+            const unsigned digit = (key[k] >> shift) & (kDigits - 1);
+            unsigned whole;
+            const unsigned lower = equalBelow(digit, live, whole);
+            if (live) {
+                const unsigned seen = mineCounts[digit];
+                rank[k] = seen + lower;
+                if (lower == 0) mineCounts[digit] = (unsigned short)(seen + whole);
+            }
+            __builtin_amdgcn_wave_barrier();
+        }
+        __syncthreads();
+        unsigned whole = 0;
+        if (d < kDigits) {
+#pragma unroll
+            for (int w = 0; w < WAVES; w++) whole += waveCounts[w][d];
+        }
+        unsigned running = digitStart(whole, waveTotals);
+        if (d < kDigits) {
+#pragma unroll
+            for (int w = 0; w < WAVES; w++) {
+                const unsigned c = waveCounts[w][d];
+                waveCounts[w][d] = (unsigned short)running;
+                running += c;
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kSmallRounds; k++) {
+            const unsigned i = (unsigned)(wave * rounds + k) * kWaveLanes + lane;
+            if (k < rounds && i < n) {
+                const unsigned to = waveCounts[wave][(key[k] >> shift) & (kDigits - 1)] + rank[k];
+                sortedKeys[to] = key[k];
+                sortedPositions[to] = position[k];
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < kSmallRounds; k++) {
+            const unsigned i = (unsigned)(wave * rounds + k) * kWaveLanes + lane;
+            if (k < rounds && i < n) {
+                key[k] = sortedKeys[i];
+                position[k] = sortedPositions[i];
+            }
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < kSmallRounds; k++) {
+        const unsigned i = (unsigned)(wave * rounds + k) * kWaveLanes + lane;
+        if (k < rounds && i < n) {
+            keysOut[i] = key[k];
+            positionsOut[i] = position[k];
+        }
+    }
+}
+
 // ---- summing ---------------------------------------------------------------------------------------------------------
 constexpr int kMostChunk = 64;   // a wave holds its chunk's keys and positions one a lane
 constexpr int kRowsInFlight = 8;
@@ -241,48 +337,70 @@ struct SumPlan {
     int chunk;
     unsigned chunks;
     Long length;
-    unsigned tiles;  // tiles of 64 vectors of columns
+    Long vectors;    // of columns
+    unsigned tiles;  // tiles of 64 vectors
 };
 
-template <typename T, bool UNIT>
-__device__ __forceinline__ void loadColumns(const T *row, Long el, Long c0, Long length, Pack<T> &v) {
+// A lane's columns: N of them from c0 on.  With UNIT (elements next to each other, rows of N elements or more) a lane whose
+// vector would pass the row's end takes the row's last N columns instead, so that every load is one vector without a
+// branch, and stores those from `first` on, which are its own.  Otherwise element by element.
+template <typename T> struct Columns {
+    Long c0;
+    int first, count;  // own: [first, count) of the N from c0 on
+};
+template <typename T, bool UNIT> __device__ __forceinline__ Columns<T> columnsOf(Long vector, Long length) {
     constexpr int N = Pack<T>::N;
-    if (UNIT && c0 + N <= length) {
-        v = loadPackAnywhere(row + c0);
-        return;
+    Columns<T> c;
+    const Long c0 = vector * N;
+    if (UNIT) {
+        c.c0 = c0 + N <= length ? c0 : length - N;
+        c.first = (int)(c0 - c.c0 < N ? c0 - c.c0 : N);
+        c.count = N;
+    } else {
+        c.c0 = c0;
+        c.first = 0;
+        c.count = (int)(c0 >= length ? 0 : (length - c0 < N ? length - c0 : N));
     }
-#pragma unroll
-    for (int e = 0; e < N; e++) v.v[e] = fromCompute<T>((typename Compute<T>::type)0);
-#pragma unroll
-    for (int e = 0; e < N; e++)
-        if (c0 + e < length) v.v[e] = row[(c0 + e) * el];
+    return c;
 }
-
+template <typename T, bool UNIT> __device__ __forceinline__ void loadColumns(const T *row, Long el, const Columns<T> &c, Pack<T> &v) {
+    constexpr int N = Pack<T>::N;
+    if (UNIT) {
+        v = loadPackAnywhere(row + c.c0);
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; e++) v.v[e] = e < c.count ? row[(c.c0 + e) * el] : fromCompute<T>((typename Compute<T>::type)0);
+    }
+}
 template <typename T, bool UNIT>
-__device__ __forceinline__ void storeSum(T *row, Long el, Long c0, Long length, const typename Compute<T>::type *acc,
+__device__ __forceinline__ void storeSum(T *row, Long el, const Columns<T> &c, const typename Compute<T>::type *acc,
                                          typename Compute<T>::type scale, bool accumulate) {
     typedef typename Compute<T>::type C;
     constexpr int N = Pack<T>::N;
-    if (UNIT && c0 + N <= length) {
+    if (UNIT && c.first == 0) {
         Pack<T> o;
-        if (accumulate) o = loadPackAnywhere(row + c0);
+        if (accumulate) o = loadPackAnywhere(row + c.c0);
 #pragma unroll
         for (int e = 0; e < N; e++) o.v[e] = fromCompute<T>(acc[e] * scale + (accumulate ? toCompute(o.v[e]) : (C)0));
-        storePackAnywhere(row + c0, o);
+        storePackAnywhere(row + c.c0, o);
         return;
     }
 #pragma unroll
     for (int e = 0; e < N; e++)
-        if (c0 + e < length) {
-            T *p = row + (c0 + e) * el;
+        if (e >= c.first && e < c.count) {
+            T *p = row + (c.c0 + e) * el;
             *p = fromCompute<T>(acc[e] * scale + (accumulate ? toCompute(*p) : (C)0));
         }
 }
 
-// the row of partial sums of a chunk: which = 0 for a run that began in an earlier chunk, 1 for one that goes on behind it
-template <typename C> __device__ __forceinline__ C *partialRow(C *partial, unsigned chunk, int which, Long length) {
-    return partial + ((size_t)chunk * 2 + which) * length;
+// the partial sums of a chunk, a vector of columns next to the other: which = 0 for a run that began in an earlier chunk, 1
+// for one that goes on behind it
+template <typename C> __device__ __forceinline__ C *partialRow(C *partial, unsigned chunk, int which, Long vectors, int perVector) {
+    return partial + ((size_t)chunk * 2 + which) * vectors * perVector;
 }
+template <typename C, int N> struct alignas(16) Partial {
+    C v[N];
+};
 
 // A wave takes one chunk and one tile of columns.
 template <typename T, bool UNIT>
@@ -295,7 +413,8 @@ __global__ void __launch_bounds__(kThreads) embeddingBpSumKernel(const T *dz, Ro
     const unsigned long long work = (unsigned long long)blockIdx.x * WAVES + wave;
     if (work >= (unsigned long long)plan.chunks * plan.tiles) return;
     const unsigned chunk = (unsigned)(work / plan.tiles), tile = (unsigned)(work % plan.tiles);
-    const Long c0 = ((Long)tile * kWaveLanes + lane) * N;
+    const Long vector = (Long)tile * kWaveLanes + lane;
+    const Columns<T> columns = columnsOf<T, UNIT>(vector, plan.length);
     const unsigned long long first = (unsigned long long)chunk * plan.chunk;
     const int count = (int)(first + plan.chunk <= plan.n ? plan.chunk : plan.n - first);
     const int mineAt = lane < count ? lane : count - 1;
@@ -308,14 +427,14 @@ __global__ void __launch_bounds__(kThreads) embeddingBpSumKernel(const T *dz, Ro
     unsigned current = __builtin_amdgcn_readlane(myKey, 0);
     bool fromBefore = current == keyBefore;
     auto finish = [&](bool goesOn) {
-        if (current < plan.vocabulary && c0 < plan.length) {
+        if (current < plan.vocabulary && vector < plan.vectors) {
             if (fromBefore || goesOn) {
-                C *row = partialRow(partial, chunk, fromBefore ? 0 : 1, plan.length);
+                Partial<C, N> sums;
 #pragma unroll
-                for (int e = 0; e < N; e++)
-                    if (c0 + e < plan.length) row[c0 + e] = acc[e];
+                for (int e = 0; e < N; e++) sums.v[e] = acc[e];
+                reinterpret_cast<Partial<C, N> *>(partialRow(partial, chunk, fromBefore ? 0 : 1, plan.vectors, N))[vector] = sums;
             } else {
-                storeSum<T, UNIT>(dTable + (Long)current * tv.row, tv.el, c0, plan.length, acc, scale, accumulate != 0);
+                storeSum<T, UNIT>(dTable + (Long)current * tv.row, tv.el, columns, acc, scale, accumulate != 0);
             }
         }
 #pragma unroll
@@ -328,7 +447,7 @@ __global__ void __launch_bounds__(kThreads) embeddingBpSumKernel(const T *dz, Ro
         for (int u = 0; u < kRowsInFlight; u++) {
             const int at = i + u < count ? i + u : count - 1;
             const unsigned p = __builtin_amdgcn_readlane(myPosition, at);
-            loadColumns<T, UNIT>(dz + (Long)p * dzv.row, dzv.el, c0, plan.length, v[u]);
+            loadColumns<T, UNIT>(dz + (Long)p * dzv.row, dzv.el, columns, v[u]);
         }
 #pragma unroll
         for (int u = 0; u < kRowsInFlight; u++) {
@@ -354,7 +473,7 @@ __global__ void __launch_bounds__(kThreads) embeddingBpJoinKernel(const unsigned
                                                                   const typename Compute<T>::type *partial) {
     typedef typename Compute<T>::type C;
     constexpr int N = Pack<T>::N, WAVES = kThreads / kWaveLanes;
-    __shared__ C smem[WAVES][kWaveLanes][N];
+    __shared__ C smem[WAVES][N][kWaveLanes];
     const int lane = threadIdx.x % kWaveLanes, wave = threadIdx.x / kWaveLanes;
     const unsigned chunk = (unsigned)(blockIdx.x / plan.tiles), tile = (unsigned)(blockIdx.x % plan.tiles);
     const unsigned long long first = (unsigned long long)chunk * plan.chunk, behind = first + plan.chunk;
@@ -373,31 +492,34 @@ __global__ void __launch_bounds__(kThreads) embeddingBpJoinKernel(const unsigned
         }
         lastChunk += kWaveLanes;
     }
-    const Long c0 = ((Long)tile * kWaveLanes + lane) * N;
+    const Long vector = (Long)tile * kWaveLanes + lane;
     C acc[N];
 #pragma unroll
     for (int e = 0; e < N; e++) acc[e] = (C)0;
-    for (unsigned c = chunk + wave; c <= lastChunk; c += WAVES) {
-        const C *row = partialRow(partial, c, c == chunk ? 1 : 0, plan.length);
+    if (vector < plan.vectors) {
+#pragma unroll 4
+        for (unsigned c = chunk + wave; c <= lastChunk; c += WAVES) {
+            const Partial<C, N> sums =
+                reinterpret_cast<const Partial<C, N> *>(partialRow(const_cast<C *>(partial), c, c == chunk ? 1 : 0, plan.vectors, N))[vector];
 #pragma unroll
-        for (int e = 0; e < N; e++)
-            if (c0 + e < plan.length) acc[e] += row[c0 + e];
+            for (int e = 0; e < N; e++) acc[e] += sums.v[e];
+        }
     }
 #pragma unroll
-    for (int e = 0; e < N; e++) smem[wave][lane][e] = acc[e];
+    for (int e = 0; e < N; e++) smem[wave][e][lane] = acc[e];
     __syncthreads();
-    if (wave != 0 || c0 >= plan.length) return;
+    if (wave != 0 || vector >= plan.vectors) return;
 #pragma unroll
     for (int w = 1; w < WAVES; w++)
 #pragma unroll
-        for (int e = 0; e < N; e++) acc[e] += smem[w][lane][e];
-    storeSum<T, UNIT>(dTable + (Long)key * tv.row, tv.el, c0, plan.length, acc, scale, accumulate != 0);
+        for (int e = 0; e < N; e++) acc[e] += smem[w][e][lane];
+    storeSum<T, UNIT>(dTable + (Long)key * tv.row, tv.el, columnsOf<T, UNIT>(vector, plan.length), acc, scale, accumulate != 0);
 }
 
 constexpr Long kClearPiece = 16384;
 
 // the chunk's length: long enough that few runs cross chunks, short enough that a few thousand waves share a small batch
-int chunkOf(Long n) { return n >= (1 << 18) ? kMostChunk : (n >= (1 << 14) ? 32 : 16); }
+int chunkOf(Long n) { return n >= (1 << 18) ? kMostChunk : (n >= (1 << 15) ? 32 : 16); }
 
 size_t aligned(size_t bytes) { return (bytes + 255) & ~(size_t)255; }
 
@@ -415,7 +537,7 @@ Layout layoutOf(Long n, Long length) {
     }
     l.counts = take((size_t)kSortBlocks * kDigits * 4);
     const Long chunk = chunkOf(n), chunks = (n + chunk - 1) / chunk;
-    l.partial = take((size_t)chunks * 2 * length * sizeof(double));
+    l.partial = take((size_t)chunks * 2 * ((length + 7) / 8 * 8) * sizeof(double));  // (a half's vectors are 8 columns)
     l.bytes = at;
     return l;
 }
@@ -456,46 +578,39 @@ void launchEmbeddingBp(hipStream_t s, const T *dz, const RowView &dzv, const Lon
     const int passes = (bits + kSortBits - 1) / kSortBits;
 
     // The table to be cleared, in equal shares for the sort's launches.  Rows that follow each other without gaps are one
-    // stretch, cut into pieces of kClearPiece bytes, of which a last, shorter one goes with the last share.
+    // stretch, cut into pieces of kClearPiece bytes.
     Clearing all;
-    Long lastPiece = 0;
     if (!accumulate) {
         all.base = reinterpret_cast<char *>(dTable);
         all.size = (int)sizeof(T);
         all.rows = tv.rows;
-        all.bytes = tv.length * sizeof(T);
+        all.bytes = all.lastBytes = tv.length * sizeof(T);
         all.pitch = tv.row * sizeof(T);
         all.apart = tv.el * sizeof(T);
         if (tv.el == 1 && (tv.row == tv.length || tv.rows == 1)) {
             const Long bytes = tv.rows * all.bytes;
-            all.rows = bytes / kClearPiece;
-            lastPiece = bytes % kClearPiece;
+            all.rows = (bytes + kClearPiece - 1) / kClearPiece;
+            all.lastBytes = bytes - (all.rows - 1) * kClearPiece;
             all.bytes = all.pitch = kClearPiece;
         }
     }
-    int sharesLeft = n == 0 ? 1 : 2 * passes;
+    int sharesLeft = n <= kSmallSort ? 1 : 2 * passes;
     auto nextShare = [&](unsigned blocks) {
         Clearing share = all;
         share.firstBlock = blocks;
-        share.rows = all.rows / sharesLeft;
+        share.rows = (all.rows + sharesLeft - 1) / sharesLeft;
+        if (share.rows < all.rows) share.lastBytes = all.bytes;
         all.base += share.rows * all.pitch;
         all.rows -= share.rows;
         sharesLeft--;
         return share;
     };
-    auto gridWith = [&](const Clearing &share) {
-        return dim3(share.firstBlock + (share.rows > 0 ? (unsigned)gridFor(share.rows, kThreads / kWaveLanes, 4096) : 0u));
+    auto gridWith = [&](const Clearing &share, int threads) {
+        return dim3(share.firstBlock + (share.rows > 0 ? (unsigned)gridFor(share.rows, threads / kWaveLanes, 4096) : 0u));
     };
-    if (lastPiece > 0) {
-        Clearing piece = all;
-        piece.base += all.rows * all.pitch;
-        piece.rows = 1;
-        piece.bytes = lastPiece;
-        ND4J_LAUNCH(clearKernel, dim3(1), dim3(kThreads), 0, s, piece);
-    }
     if (n == 0) {
         const Clearing share = nextShare(0);
-        if (share.rows > 0) ND4J_LAUNCH(clearKernel, gridWith(share), dim3(kThreads), 0, s, share);
+        if (share.rows > 0) ND4J_LAUNCH(clearKernel, gridWith(share, kThreads), dim3(kThreads), 0, s, share);
         return;
     }
 
@@ -513,12 +628,19 @@ void launchEmbeddingBp(hipStream_t s, const T *dz, const RowView &dzv, const Lon
     const unsigned blocks = (unsigned)(((unsigned long long)n + tile - 1) / tile);
     const unsigned *from = nullptr, *fromPositions = nullptr;
     int to = 0;
-    for (int pass = 0; pass < passes; pass++) {
+    if (n <= kSmallSort) {
+        const Clearing share = nextShare(1);
+        ND4J_LAUNCH(sortSmallKernel, gridWith(share, kSmallThreads), dim3(kSmallThreads), 0, s, tokens, n, vocabulary, passes, keys[0], positions[0],
+                    share);
+        from = keys[0];
+        fromPositions = positions[0];
+    }
+    for (int pass = 0; pass < passes && n > kSmallSort; pass++) {
         const int shift = pass * kSortBits;
         Clearing share = nextShare(blocks);
-        ND4J_LAUNCH(sortCountKernel, gridWith(share), dim3(kThreads), 0, s, tokens, from, n, vocabulary, tile, shift, counts, share);
+        ND4J_LAUNCH(sortCountKernel, gridWith(share, kThreads), dim3(kThreads), 0, s, tokens, from, n, vocabulary, tile, shift, counts, share);
         share = nextShare(blocks);
-        ND4J_LAUNCH(sortPlaceKernel, gridWith(share), dim3(kThreads), 0, s, tokens, from, fromPositions, n, vocabulary, tile, shift, counts,
+        ND4J_LAUNCH(sortPlaceKernel, gridWith(share, kThreads), dim3(kThreads), 0, s, tokens, from, fromPositions, n, vocabulary, tile, shift, counts,
                     keys[to], positions[to], share);
         from = keys[to];
         fromPositions = positions[to];
@@ -530,10 +652,11 @@ void launchEmbeddingBp(hipStream_t s, const T *dz, const RowView &dzv, const Lon
     plan.chunk = chunkOf(n);
     plan.chunks = (unsigned)(((unsigned long long)n + plan.chunk - 1) / plan.chunk);
     plan.length = tv.length;
-    plan.tiles = (unsigned)((tv.length + kWaveLanes * Pack<T>::N - 1) / (kWaveLanes * Pack<T>::N));
+    plan.vectors = (tv.length + Pack<T>::N - 1) / Pack<T>::N;
+    plan.tiles = (unsigned)((plan.vectors + kWaveLanes - 1) / kWaveLanes);
     constexpr int WAVES = kThreads / kWaveLanes;
     const unsigned sumBlocks = (unsigned)(((unsigned long long)plan.chunks * plan.tiles + WAVES - 1) / WAVES);
-    const bool unit = dzv.el == 1 && tv.el == 1;
+    const bool unit = dzv.el == 1 && tv.el == 1 && tv.length >= Pack<T>::N;
     if (unit)
         ND4J_LAUNCH((embeddingBpSumKernel<T, true>), dim3(sumBlocks), dim3(kThreads), 0, s, dz, dzv, from, fromPositions, plan, dTable, tv,
                     (C)scale, accumulate ? 1 : 0, partial);
