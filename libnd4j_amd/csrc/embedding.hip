@@ -87,11 +87,13 @@ __global__ void __launch_bounds__(kThreads) embeddingRowsKernel(const T *table, 
 }
 
 // ---- sorting the tokens ----------------------------------------------------------------------------------------------
-// Least significant digit first, 8 bits a pass.  A block counts the digits of its tile (a multiple of kSubTile tokens), a
-// second launch places the tile's tokens behind those of lower digits and of the blocks before it.  At most kSortBlocks
-// tiles, so that the placing block can add up the counts of all blocks itself.
+// Least significant digit first, 8 bits a pass.  A block counts the digits of its tile (a multiple of kSortThreads tokens); a
+// second launch places the tile's tokens behind those of lower digits and of the blocks before it.  (Counting the next
+// pass's digits while placing, by atomics where the tokens come to lie, took longer than the launch that it saved: frequent
+// tokens meet in one counter.)  At most kSortBlocks tiles, so that the placing block can add up the counts of all blocks
+// itself.
 constexpr int kSortBits = 8, kDigits = 1 << kSortBits;
-constexpr int kSortRounds = 4, kSubTile = kThreads * kSortRounds;
+constexpr int kSortThreads = 1024;
 constexpr int kSortBlocks = 256;
 
 // the sort key of token t: tokens outside the table come last, under the key `vocabulary`
@@ -130,20 +132,20 @@ __device__ __forceinline__ void clearShare(const Clearing &c) {
 }
 __global__ void __launch_bounds__(kThreads) clearKernel(Clearing clearing) { clearShare(clearing); }
 
-__global__ void __launch_bounds__(kThreads) sortCountKernel(const Long *tokens, const unsigned *keys, unsigned n, unsigned vocabulary,
-                                                            unsigned tile, int shift, unsigned *counts, Clearing clearing) {
+__global__ void __launch_bounds__(kSortThreads) sortCountKernel(const Long *tokens, const unsigned *keys, unsigned n, unsigned vocabulary,
+                                                                unsigned tile, int shift, unsigned *counts, Clearing clearing) {
     __shared__ unsigned local[kDigits];
     if (blockIdx.x >= clearing.firstBlock) return clearShare(clearing);
-    local[threadIdx.x] = 0;
+    if (threadIdx.x < kDigits) local[threadIdx.x] = 0;
     __syncthreads();
     const unsigned long long first = (unsigned long long)blockIdx.x * tile;
     const unsigned end = (unsigned)(first + tile < n ? first + tile : n);
-    for (unsigned i = (unsigned)first + threadIdx.x; i < end; i += kThreads) {
+    for (unsigned i = (unsigned)first + threadIdx.x; i < end; i += kSortThreads) {
         const unsigned key = keys != nullptr ? keys[i] : keyOf(tokens[i], vocabulary);
         atomicAdd(&local[(key >> shift) & (kDigits - 1)], 1u);
     }
     __syncthreads();
-    counts[(size_t)blockIdx.x * kDigits + threadIdx.x] = local[threadIdx.x];
+    if (threadIdx.x < kDigits) counts[(size_t)blockIdx.x * kDigits + threadIdx.x] = local[threadIdx.x];
 }
 
 // How many of the wave's live lanes below this one have the same digit; whole: how many lanes have it in all
@@ -174,105 +176,98 @@ __device__ __forceinline__ unsigned digitStart(unsigned mine, unsigned *waveTota
     return sum;
 }
 
-__global__ void __launch_bounds__(kThreads) sortPlaceKernel(const Long *tokens, const unsigned *keys, const unsigned *positions, unsigned n,
-                                                            unsigned vocabulary, unsigned tile, int shift, const unsigned *counts,
-                                                            unsigned *keysOut, unsigned *positionsOut, Clearing clearing) {
-    constexpr int WAVES = kThreads / kWaveLanes;
+__global__ void __launch_bounds__(kSortThreads) sortPlaceKernel(const Long *tokens, const unsigned *keys, const unsigned *positions, unsigned n,
+                                                                unsigned vocabulary, unsigned tile, int shift, const unsigned *counts,
+                                                                unsigned *keysOut, unsigned *positionsOut, Clearing clearing) {
+    constexpr int WAVES = kSortThreads / kWaveLanes;
     __shared__ unsigned starts[kDigits], waveTotals[WAVES];
     __shared__ unsigned waveCounts[WAVES][kDigits];
-    const int d = threadIdx.x, lane = threadIdx.x % kWaveLanes, wave = threadIdx.x / kWaveLanes;
+    const int d = threadIdx.x, wave = threadIdx.x / kWaveLanes;
     const unsigned blocks = clearing.firstBlock;
     if (blockIdx.x >= blocks) return clearShare(clearing);
-    // where this block's tokens of digit d begin: all tokens of lower digits, then those of digit d in the blocks before
-    unsigned before = 0, whole = 0;
-#pragma unroll 8
-    for (unsigned b = 0; b < blocks; b++) {
-        const unsigned c = counts[(size_t)b * kDigits + d];
-        whole += c;
-        if (b < blockIdx.x) before += c;
-    }
-    starts[d] = digitStart(whole, waveTotals) + before;
     const unsigned long long first = (unsigned long long)blockIdx.x * tile;
     const unsigned long long end = first + tile < n ? first + tile : n;
-    for (unsigned long long at = first; at < end; at += kSubTile) {
-#pragma unroll
-        for (int w = 0; w < WAVES; w++) waveCounts[w][d] = 0;
+    unsigned key = 0, position = 0;
+    auto load = [&](unsigned long long i) {
+        if (i < end) {
+            key = keys != nullptr ? keys[i] : keyOf(tokens[i], vocabulary);
+            position = positions != nullptr ? positions[i] : (unsigned)i;
+        }
+    };
+    load(first + threadIdx.x);  // (on its way while the counts are added up)
+    // where this block's tokens of digit d begin: all tokens of lower digits, then those of digit d in the blocks before
+    unsigned before = 0, all = 0;
+    if (d < kDigits) {
+#pragma unroll 8
+        for (unsigned b = 0; b < blocks; b++) {
+            const unsigned c = counts[(size_t)b * kDigits + d];
+            all += c;
+            if (b < blockIdx.x) before += c;
+        }
+    }
+    const unsigned start = digitStart(all, waveTotals) + before;
+    if (d < kDigits) starts[d] = start;
+    for (unsigned long long at = first; at < end; at += kSortThreads) {
+        for (int i = threadIdx.x; i < WAVES * kDigits; i += kSortThreads) (&waveCounts[0][0])[i] = 0;
         __syncthreads();
-        // a wave ranks kSortRounds x 64 consecutive tokens: behind the equal digits of its earlier rounds and lower lanes
-        unsigned key[kSortRounds], position[kSortRounds], rank[kSortRounds];
-        volatile unsigned *mineCounts = waveCounts[wave];
+        const unsigned long long i = at + threadIdx.x;
+        const bool live = i < end;
+        const unsigned digit = (key >> shift) & (kDigits - 1);
+        unsigned whole;
+        const unsigned lower = equalBelow(digit, live, whole);
+        if (live && lower == 0) waveCounts[wave][digit] = whole;
+        __syncthreads();
+        if (d < kDigits) {
+            unsigned running = starts[d];
 #pragma unroll
-        for (int k = 0; k < kSortRounds; k++) {
-            const unsigned long long i = at + (unsigned)(wave * kSortRounds + k) * kWaveLanes + lane;
-            const bool live = i < end;
-            key[k] = 0;
-            position[k] = 0;
-            if (live) {
-                key[k] = keys != nullptr ? keys[i] : keyOf(tokens[i], vocabulary);
-                position[k] = positions != nullptr ? positions[i] : (unsigned)i;
+            for (int w = 0; w < WAVES; w++) {
+                const unsigned c = waveCounts[w][d];
+                waveCounts[w][d] = running;
+                running += c;
             }
-            const unsigned digit = (key[k] >> shift) & (kDigits - 1);
-            unsigned whole;
-            const unsigned lower = equalBelow(digit, live, whole);
-            rank[k] = 0;
-            if (live) {
-                const unsigned seen = mineCounts[digit];
-                rank[k] = seen + lower;
-                if (lower == 0) mineCounts[digit] = seen + whole;
-            }
-            __builtin_amdgcn_wave_barrier();
+            starts[d] = running;
         }
         __syncthreads();
-        unsigned running = starts[d];
-#pragma unroll
-        for (int w = 0; w < WAVES; w++) {
-            const unsigned c = waveCounts[w][d];
-            waveCounts[w][d] = running;
-            running += c;
+        if (live) {
+            const unsigned to = waveCounts[wave][digit] + lower;
+            keysOut[to] = key;
+            positionsOut[to] = position;
         }
-        starts[d] = running;
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < kSortRounds; k++) {
-            const unsigned long long i = at + (unsigned)(wave * kSortRounds + k) * kWaveLanes + lane;
-            if (i < end) {
-                const unsigned to = waveCounts[wave][(key[k] >> shift) & (kDigits - 1)] + rank[k];
-                keysOut[to] = key[k];
-                positionsOut[to] = position[k];
-            }
-        }
+        load(i + kSortThreads);
         __syncthreads();
     }
 }
 
-// Up to kSmallSort tokens: one block does all passes in LDS, in one launch instead of two a pass.
-constexpr int kSmallThreads = 1024, kSmallRounds = 4, kSmallSort = kSmallThreads * kSmallRounds;
+// Up to kSmallSort tokens of fewer than 2^18: one block does all passes in LDS, in one launch instead of two a pass, each
+// token as one word of its key and, below it, its position.  (A round of 1024 tokens takes about 1 us a pass: 16384 tokens took
+// 35 us this way.)
+constexpr int kSmallThreads = 1024, kSmallBits = 12, kSmallSort = 1 << kSmallBits, kSmallRounds = kSmallSort / kSmallThreads;
 __global__ void __launch_bounds__(kSmallThreads) sortSmallKernel(const Long *tokens, unsigned n, unsigned vocabulary, int passes, unsigned *keysOut,
                                                                  unsigned *positionsOut, Clearing clearing) {
     constexpr int WAVES = kSmallThreads / kWaveLanes;
-    __shared__ unsigned sortedKeys[kSmallSort], sortedPositions[kSmallSort];
+    __shared__ unsigned sorted[kSmallSort];
     __shared__ unsigned short waveCounts[WAVES][kDigits];
     __shared__ unsigned waveTotals[WAVES];
     if (blockIdx.x >= clearing.firstBlock) return clearShare(clearing);
     const int d = threadIdx.x, lane = threadIdx.x % kWaveLanes, wave = threadIdx.x / kWaveLanes;
     const int rounds = (int)((n + kSmallThreads - 1) / kSmallThreads);  // a wave's tokens: rounds x 64 consecutive ones
-    unsigned key[kSmallRounds], position[kSmallRounds], rank[kSmallRounds];
+    const unsigned mine = (unsigned)(wave * rounds) * kWaveLanes + lane;
+    unsigned word[kSmallRounds], rank[kSmallRounds];
 #pragma unroll
     for (int k = 0; k < kSmallRounds; k++) {
-        const unsigned i = (unsigned)(wave * rounds + k) * kWaveLanes + lane;
-        key[k] = k < rounds && i < n ? keyOf(tokens[i], vocabulary) : 0u;
-        position[k] = i;
+        const unsigned i = mine + k * kWaveLanes;
+        word[k] = k < rounds && i < n ? keyOf(tokens[i], vocabulary) << kSmallBits | i : 0u;
     }
     for (int pass = 0; pass < passes; pass++) {
-        const int shift = pass * kSortBits;
+        const int shift = kSmallBits + pass * kSortBits;
         for (int i = threadIdx.x; i < WAVES * kDigits; i += kSmallThreads) (&waveCounts[0][0])[i] = 0;
         __syncthreads();
         volatile unsigned short *mineCounts = waveCounts[wave];
 #pragma unroll
         for (int k = 0; k < kSmallRounds; k++) {
             if (k >= rounds) break;
-            const bool live = (unsigned)(wave * rounds + k) * kWaveLanes + lane < n;
-            const unsigned digit = (key[k] >> shift) & (kDigits - 1);
+            const bool live = mine + k * kWaveLanes < n;
+            const unsigned digit = (word[k] >> shift) & (kDigits - 1);
             unsigned whole;
             const unsigned lower = equalBelow(digit, live, whole);
             if (live) {
@@ -299,30 +294,19 @@ __global__ void __launch_bounds__(kSmallThreads) sortSmallKernel(const Long *tok
         }
         __syncthreads();
 #pragma unroll
-        for (int k = 0; k < kSmallRounds; k++) {
-            const unsigned i = (unsigned)(wave * rounds + k) * kWaveLanes + lane;
-            if (k < rounds && i < n) {
-                const unsigned to = waveCounts[wave][(key[k] >> shift) & (kDigits - 1)] + rank[k];
-                sortedKeys[to] = key[k];
-                sortedPositions[to] = position[k];
-            }
-        }
+        for (int k = 0; k < kSmallRounds; k++)
+            if (k < rounds && mine + k * kWaveLanes < n) sorted[waveCounts[wave][(word[k] >> shift) & (kDigits - 1)] + rank[k]] = word[k];
         __syncthreads();
 #pragma unroll
-        for (int k = 0; k < kSmallRounds; k++) {
-            const unsigned i = (unsigned)(wave * rounds + k) * kWaveLanes + lane;
-            if (k < rounds && i < n) {
-                key[k] = sortedKeys[i];
-                position[k] = sortedPositions[i];
-            }
-        }
+        for (int k = 0; k < kSmallRounds; k++)
+            if (k < rounds && mine + k * kWaveLanes < n) word[k] = sorted[mine + k * kWaveLanes];
     }
 #pragma unroll
     for (int k = 0; k < kSmallRounds; k++) {
-        const unsigned i = (unsigned)(wave * rounds + k) * kWaveLanes + lane;
+        const unsigned i = mine + k * kWaveLanes;
         if (k < rounds && i < n) {
-            keysOut[i] = key[k];
-            positionsOut[i] = position[k];
+            keysOut[i] = word[k] >> kSmallBits;
+            positionsOut[i] = word[k] & (kSmallSort - 1);
         }
     }
 }
@@ -466,38 +450,46 @@ __global__ void __launch_bounds__(kThreads) embeddingBpSumKernel(const T *dz, Ro
 }
 
 // A block takes one chunk and one tile: where a run begins in the chunk and goes on behind it, the run's partial sums are
-// added up in the order of the chunks (each wave every fourth of them, then the waves in order).
+// added up in the order of the chunks (each wave every eighth of them, then the waves in order).  With four waves of four
+// rows in flight the most frequent of 32000 tokens, 7 % of 16384, took 8 us, with eight of eight 6.6 us.
+constexpr int kJoinThreads = 512;
 template <typename T, bool UNIT>
-__global__ void __launch_bounds__(kThreads) embeddingBpJoinKernel(const unsigned *keys, SumPlan plan, T *dTable, RowView tv,
-                                                                  typename Compute<T>::type scale, int accumulate,
-                                                                  const typename Compute<T>::type *partial) {
+__global__ void __launch_bounds__(kJoinThreads) embeddingBpJoinKernel(const unsigned *keys, SumPlan plan, T *dTable, RowView tv,
+                                                                      typename Compute<T>::type scale, int accumulate,
+                                                                      const typename Compute<T>::type *partial) {
     typedef typename Compute<T>::type C;
-    constexpr int N = Pack<T>::N, WAVES = kThreads / kWaveLanes;
+    constexpr int N = Pack<T>::N, WAVES = kJoinThreads / kWaveLanes;
     __shared__ C smem[WAVES][N][kWaveLanes];
     const int lane = threadIdx.x % kWaveLanes, wave = threadIdx.x / kWaveLanes;
     const unsigned chunk = (unsigned)(blockIdx.x / plan.tiles), tile = (unsigned)(blockIdx.x % plan.tiles);
     const unsigned long long first = (unsigned long long)chunk * plan.chunk, behind = first + plan.chunk;
     if (behind >= plan.n) return;
-    const unsigned key = keys[behind - 1];
-    if (key >= plan.vocabulary || keys[behind] != key) return;
-    if (first > 0 && keys[first] == key && keys[first - 1] == key) return;  // began earlier
+    // (all of these are asked for before any is waited for)
+    const unsigned key = keys[behind - 1], keyBehind = keys[behind], keyFirst = keys[first], keyBefore = first > 0 ? keys[first - 1] : 0xffffffffu;
     // the run reaches into every chunk that begins with its key, as far as these follow each other: 64 looked at a time
     unsigned lastChunk = chunk + 1;
+    auto beginOf = [&](unsigned c) {
+        const unsigned long long at = ((unsigned long long)c + lane) * plan.chunk;
+        return at < plan.n ? keys[at] : 0xffffffffu;
+    };
+    unsigned begins = beginOf(lastChunk + 1);
+    if (key >= plan.vocabulary || keyBehind != key) return;
+    if (keyFirst == key && keyBefore == key) return;  // the run began in an earlier chunk, whose block joins it
     for (;;) {
-        const unsigned long long next = (unsigned long long)lastChunk + 1 + lane, at = next * plan.chunk;
-        const unsigned long long other = __ballot(!(at < plan.n && keys[at < plan.n ? at : 0] == key));
+        const unsigned long long other = __ballot(begins != key);
         if (other != 0ull) {
             lastChunk += (unsigned)__ffsll(other) - 1;
             break;
         }
         lastChunk += kWaveLanes;
+        begins = beginOf(lastChunk + 1);
     }
     const Long vector = (Long)tile * kWaveLanes + lane;
     C acc[N];
 #pragma unroll
     for (int e = 0; e < N; e++) acc[e] = (C)0;
     if (vector < plan.vectors) {
-#pragma unroll 4
+#pragma unroll 8
         for (unsigned c = chunk + wave; c <= lastChunk; c += WAVES) {
             const Partial<C, N> sums =
                 reinterpret_cast<const Partial<C, N> *>(partialRow(const_cast<C *>(partial), c, c == chunk ? 1 : 0, plan.vectors, N))[vector];
@@ -519,7 +511,7 @@ __global__ void __launch_bounds__(kThreads) embeddingBpJoinKernel(const unsigned
 constexpr Long kClearPiece = 16384;
 
 // the chunk's length: long enough that few runs cross chunks, short enough that a few thousand waves share a small batch
-int chunkOf(Long n) { return n >= (1 << 18) ? kMostChunk : (n >= (1 << 15) ? 32 : 16); }
+int chunkOf(Long n) { return n >= (1 << 18) ? kMostChunk : (n >= (1 << 15) ? 32 : (n >= (1 << 12) ? 16 : 8)); }
 
 size_t aligned(size_t bytes) { return (bytes + 255) & ~(size_t)255; }
 
@@ -594,7 +586,8 @@ void launchEmbeddingBp(hipStream_t s, const T *dz, const RowView &dzv, const Lon
             all.bytes = all.pitch = kClearPiece;
         }
     }
-    int sharesLeft = n <= kSmallSort ? 1 : 2 * passes;
+    const bool small = n <= (unsigned)kSmallSort && vocabulary < 1u << (32 - kSmallBits);
+    int sharesLeft = small ? 1 : 2 * passes;
     auto nextShare = [&](unsigned blocks) {
         Clearing share = all;
         share.firstBlock = blocks;
@@ -623,25 +616,26 @@ void launchEmbeddingBp(hipStream_t s, const T *dz, const RowView &dzv, const Lon
     }
     unsigned *counts = reinterpret_cast<unsigned *>(base + l.counts);
     C *partial = reinterpret_cast<C *>(base + l.partial);
-    const unsigned tile = (unsigned)(((n + (unsigned long long)kSortBlocks * kSubTile - 1) / ((unsigned long long)kSortBlocks * kSubTile)) *
-                                     kSubTile);
+    constexpr unsigned long long most = (unsigned long long)kSortBlocks * kSortThreads;
+    const unsigned tile = (unsigned)((n + most - 1) / most * kSortThreads);
     const unsigned blocks = (unsigned)(((unsigned long long)n + tile - 1) / tile);
     const unsigned *from = nullptr, *fromPositions = nullptr;
     int to = 0;
-    if (n <= kSmallSort) {
+    if (small) {
         const Clearing share = nextShare(1);
         ND4J_LAUNCH(sortSmallKernel, gridWith(share, kSmallThreads), dim3(kSmallThreads), 0, s, tokens, n, vocabulary, passes, keys[0], positions[0],
                     share);
         from = keys[0];
         fromPositions = positions[0];
     }
-    for (int pass = 0; pass < passes && n > kSmallSort; pass++) {
+    for (int pass = 0; pass < passes && !small; pass++) {
         const int shift = pass * kSortBits;
         Clearing share = nextShare(blocks);
-        ND4J_LAUNCH(sortCountKernel, gridWith(share, kThreads), dim3(kThreads), 0, s, tokens, from, n, vocabulary, tile, shift, counts, share);
+        ND4J_LAUNCH(sortCountKernel, gridWith(share, kSortThreads), dim3(kSortThreads), 0, s, tokens, from, n, vocabulary, tile, shift, counts,
+                    share);
         share = nextShare(blocks);
-        ND4J_LAUNCH(sortPlaceKernel, gridWith(share, kThreads), dim3(kThreads), 0, s, tokens, from, fromPositions, n, vocabulary, tile, shift, counts,
-                    keys[to], positions[to], share);
+        ND4J_LAUNCH(sortPlaceKernel, gridWith(share, kSortThreads), dim3(kSortThreads), 0, s, tokens, from, fromPositions, n, vocabulary, tile,
+                    shift, counts, keys[to], positions[to], share);
         from = keys[to];
         fromPositions = positions[to];
         to ^= 1;
@@ -666,10 +660,10 @@ void launchEmbeddingBp(hipStream_t s, const T *dz, const RowView &dzv, const Lon
     if (plan.chunks > 1) {
         const unsigned joinBlocks = (plan.chunks - 1) * plan.tiles;
         if (unit)
-            ND4J_LAUNCH((embeddingBpJoinKernel<T, true>), dim3(joinBlocks), dim3(kThreads), 0, s, from, plan, dTable, tv, (C)scale,
+            ND4J_LAUNCH((embeddingBpJoinKernel<T, true>), dim3(joinBlocks), dim3(kJoinThreads), 0, s, from, plan, dTable, tv, (C)scale,
                         accumulate ? 1 : 0, partial);
         else
-            ND4J_LAUNCH((embeddingBpJoinKernel<T, false>), dim3(joinBlocks), dim3(kThreads), 0, s, from, plan, dTable, tv, (C)scale,
+            ND4J_LAUNCH((embeddingBpJoinKernel<T, false>), dim3(joinBlocks), dim3(kJoinThreads), 0, s, from, plan, dTable, tv, (C)scale,
                         accumulate ? 1 : 0, partial);
     }
 }
