@@ -166,18 +166,22 @@ __global__ void __launch_bounds__(kRowThreads) layerNormBpAnyKernel(const T *x, 
 // The backward pass of rows that a team holds in its registers (as in layerNormRowsKernel): dx, and the row's share of the
 // gain's and bias's gradients added onto sums that a lane keeps for its own columns over all rows of its team.  At the end
 // the teams of a block add theirs up in LDS, and partial[0 / 1][block][column] receives the block's sums (null: not wanted).
-template <int TEAM> constexpr int bpThreads() { return TEAM > 512 ? TEAM : 512; }
+//
+// One block of 1024 threads a compute unit (two where a lane holds one vector): every block leaves two rows of partial sums,
+// which is why there are no more of them, and 16 waves hide the loads of each other.
+constexpr int kBpThreads = 1024;
 template <typename T, int TEAM, int PACKS>
-__global__ void __launch_bounds__(bpThreads<TEAM>())
+__global__ void __launch_bounds__(kBpThreads)
     layerNormBpRowsKernel(const T *x, RowView xv, const T *gain, const typename Compute<T>::type *mean, const typename Compute<T>::type *invStd,
                           const T *dz, RowView dzv, T *dx, RowView dxv, typename Compute<T>::type *partial) {
     typedef typename Compute<T>::type C;
-    constexpr int N = Pack<T>::N, THREADS = bpThreads<TEAM>(), TEAMS = THREADS / TEAM;
+    constexpr int N = Pack<T>::N, THREADS = kBpThreads, TEAMS = THREADS / TEAM;
     extern __shared__ __align__(16) char dynamicLds[];
     C *columns = reinterpret_cast<C *>(dynamicLds);  // [TEAMS / 2][columns of a row]
-    __shared__ C sums[2][THREADS / kWaveLanes];
+    __shared__ C sums[4 * (THREADS / kWaveLanes)];
     const int lane = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
-    C *smem = sums[0] + threadIdx.x / TEAM * (TEAM / kWaveLanes), *smem2 = smem + THREADS / kWaveLanes;
+    C *smem = sums + 4 * team * (TEAM / kWaveLanes);
+    int turn = 0;
     const int length = (int)xv.length, vectors = length / N, rest = vectors * N + lane;
     const C perLength = (C)1 / (C)length;
     int at[PACKS];
@@ -219,8 +223,8 @@ __global__ void __launch_bounds__(bpThreads<TEAM>())
                         const C dd = toCompute(d[j].v[e]), h = (toCompute(v[j].v[e]) - mu) * s;
                         const C a = gain != nullptr ? dd * toCompute(g[j].v[e]) : dd;
                         sumA += a;
-                        sumAH += a * h;
-                        gainSum[j][e] += dd * h;
+                        sumAH = fused(a, h, sumAH);
+                        gainSum[j][e] = fused(dd, h, gainSum[j][e]);
                         biasSum[j][e] += dd;
                     }
                 }
@@ -233,7 +237,8 @@ __global__ void __launch_bounds__(bpThreads<TEAM>())
             }
         }
         if (dx == nullptr) continue;
-        const C meanA = teamAll<TEAM>(sumA, Add(), smem) * perLength, meanAH = teamAll<TEAM>(sumAH, Add(), smem2) * perLength;
+        teamSums<TEAM>(sumA, sumAH, smem, turn);
+        const C meanA = sumA * perLength, meanAH = sumAH * perLength;
         if (!live) continue;
         T *dxr = dx + r * dxv.row;
 #pragma unroll
@@ -245,7 +250,7 @@ __global__ void __launch_bounds__(bpThreads<TEAM>())
                     const C h = (toCompute(v[j].v[e]) - mu) * s;
                     C a = toCompute(d[j].v[e]);
                     if (gain != nullptr) a *= toCompute(g[j].v[e]);
-                    o.v[e] = fromCompute<T>(s * (a - meanA - h * meanAH));
+                    o.v[e] = fromCompute<T>(s * fused(-h, meanAH, a - meanA));
                 }
                 storePackAnywhere(dxr + at[j], o);
             }
@@ -367,11 +372,10 @@ unsigned gridOf(Long blocks) { return (unsigned)(blocks < 1 ? 1 : (blocks > (1 <
 
 }  // namespace
 
-// The blocks of the register kernel: two a compute unit, which is what its registers and LDS leave room for
-constexpr int kBpBlocks = 512;
+constexpr int kBpBlocks = 256;  // of the register kernel; twice as many where a lane holds one vector
 
 size_t layerNormBpScratch(Long rows, Long length) {
-    const Long any = columnSplits(rows, length), held = rows < kBpBlocks ? (rows < 1 ? 1 : rows) : kBpBlocks;
+    const Long any = columnSplits(rows, length), held = rows < 2 * kBpBlocks ? (rows < 1 ? 1 : rows) : 2 * kBpBlocks;
     return (size_t)2 * (any > held ? any : held) * length * sizeof(double);
 }
 
@@ -412,8 +416,8 @@ int runBpRows(hipStream_t s, const T *x, const RowView &xv, const T *gain, const
               const typename Compute<T>::type *invStd, const T *dz, const RowView &dzv, T *dx, const RowView &dxv,
               typename Compute<T>::type *partial) {
     typedef typename Compute<T>::type C;
-    constexpr int THREADS = bpThreads<TEAM>(), TEAMS = THREADS / TEAM;
-    const int blocks = gridFor(xv.rows, TEAMS, kBpBlocks);
+    constexpr int THREADS = kBpThreads, TEAMS = THREADS / TEAM;
+    const int blocks = gridFor(xv.rows, TEAMS, PACKS == 1 ? 2 * kBpBlocks : kBpBlocks);
     const size_t lds = TEAMS > 1 && partial != nullptr ? (size_t)(TEAMS / 2) * xv.length * sizeof(C) : 0;
     ND4J_LAUNCH((layerNormBpRowsKernel<T, TEAM, PACKS>), dim3(blocks), dim3(THREADS), lds, s, x, xv, gain, mean, invStd, dz, dzv, dx, dxv,
                 partial);
@@ -434,9 +438,9 @@ void launchLayerNormBp(hipStream_t s, const T *x, const RowView &xv, const T *ga
         if (vectors <= 16) ROWS(16, 1);
         else if (vectors <= 64) ROWS(64, 1);
         else if (vectors <= 128) ROWS(64, 2);
-        else if (vectors <= 256) ROWS(64, 4);
+        else if (vectors <= 256) ROWS(128, 2);
         else if (vectors <= 512) ROWS(256, 2);
-        else if (vectors <= 1024) ROWS(256, 4);
+        else if (vectors <= 1024) ROWS(512, 2);
         else if (vectors <= 2048) ROWS(1024, 2);
 #undef ROWS
     }

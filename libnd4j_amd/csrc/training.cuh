@@ -82,6 +82,33 @@ template <int TEAM, class Op, typename C> __device__ __forceinline__ C teamAll(C
     else return blockAll<TEAM>(v, op, smem);
 }
 
+// Two sums at once, for teams that take turn after turn: smem holds two of C per wave of the team twice over, for even and
+// odd turns, so that one barrier a turn is enough.
+template <int TEAM, typename C> __device__ __forceinline__ void teamSums(C &a, C &b, C *smem, int &turn) {
+    constexpr int W = TEAM <= kWaveLanes ? TEAM : kWaveLanes;
+    a = waveAll<W>(a, Add());
+    b = waveAll<W>(b, Add());
+    if constexpr (TEAM > kWaveLanes) {
+        constexpr int WAVES = TEAM / kWaveLanes;
+        C *mine = smem + (turn & 1) * 2 * WAVES;
+        turn++;
+        if (threadIdx.x % kWaveLanes == 0) {
+            mine[threadIdx.x % TEAM / kWaveLanes] = a;
+            mine[WAVES + threadIdx.x % TEAM / kWaveLanes] = b;
+        }
+        __syncthreads();
+        a = mine[0];
+        b = mine[WAVES];
+#pragma unroll
+        for (int w = 1; w < WAVES; w++) {
+            a += mine[w];
+            b += mine[WAVES + w];
+        }
+    }
+}
+__device__ __forceinline__ float fused(float a, float b, float c) { return __builtin_fmaf(a, b, c); }
+__device__ __forceinline__ double fused(double a, double b, double c) { return __builtin_fma(a, b, c); }
+
 __device__ __forceinline__ float sqrtOf(float v) { return ::sqrtf(v); }
 __device__ __forceinline__ double sqrtOf(double v) { return ::sqrt(v); }
 template <typename C> __device__ __forceinline__ C notANumber() { return (C)__builtin_nanf(""); }
