@@ -195,24 +195,41 @@ __global__ void __launch_bounds__(kBpThreads)
         for (int e = 0; e < N; e++) gainSum[j][e] = biasSum[j][e] = (C)0;
     }
     if (rest < length && gain != nullptr) gRest = toCompute(gain[rest]);
-    for (Long r0 = (Long)blockIdx.x * TEAMS; r0 < xv.rows; r0 += (Long)gridDim.x * TEAMS) {
-        const bool live = r0 + team < xv.rows;
-        const Long r = live ? r0 + team : r0;
+    // the next row is on its way while this one is worked on
+    Pack<T> v[PACKS], d[PACKS], nextV[PACKS], nextD[PACKS];
+    C vRest = (C)0, dRest = (C)0, nextVRest = (C)0, nextDRest = (C)0, mu = (C)0, s = (C)0, nextMu = (C)0, nextS = (C)0;
+    const Long step = (Long)gridDim.x * TEAMS;
+    auto ask = [&](Long r0) {
+        const Long r = r0 + team < xv.rows ? r0 + team : (r0 < xv.rows ? r0 : 0);
         const T *xr = x + r * xv.row, *dzr = dz + r * dzv.row;
-        Pack<T> v[PACKS], d[PACKS];
-        C vRest = (C)0, dRest = (C)0;
         if (vectors > 0) {
 #pragma unroll
             for (int j = 0; j < PACKS; j++) {
-                v[j] = loadPackAnywhere(xr + at[j]);
-                d[j] = loadPackAnywhere(dzr + at[j]);
+                nextV[j] = loadPackAnywhere(xr + at[j]);
+                nextD[j] = loadPackAnywhere(dzr + at[j]);
             }
         }
-        const C mu = mean[r], s = invStd[r];
+        nextMu = mean[r];
+        nextS = invStd[r];
         if (rest < length) {
-            vRest = toCompute(xr[rest]);
-            dRest = toCompute(dzr[rest]);
+            nextVRest = toCompute(xr[rest]);
+            nextDRest = toCompute(dzr[rest]);
         }
+    };
+    ask((Long)blockIdx.x * TEAMS);
+    for (Long r0 = (Long)blockIdx.x * TEAMS; r0 < xv.rows; r0 += step) {
+        const bool live = r0 + team < xv.rows;
+        const Long r = live ? r0 + team : r0;
+#pragma unroll
+        for (int j = 0; j < PACKS; j++) {
+            v[j] = nextV[j];
+            d[j] = nextD[j];
+        }
+        vRest = nextVRest;
+        dRest = nextDRest;
+        mu = nextMu;
+        s = nextS;
+        if (r0 + step < xv.rows) ask(r0 + step);
         C sumA = (C)0, sumAH = (C)0;
         if (live) {
 #pragma unroll
