@@ -47,18 +47,22 @@ __global__ void __launch_bounds__(kRowThreads) layerNormAnyKernel(const T *x, Ro
     }
 }
 
-// Rows of contiguous elements that a team of TEAM lanes holds in its registers: PACKS vectors of 16 bytes a lane, and the
-// elements behind the last whole vector one a lane.  One read of x, one write of z; gain and bias stay in registers over
-// the team's rows (HELD).  Loads are unconditional (a vector that is not there re-reads the lane's first place, see `at`).
-template <typename T, int TEAM, int PACKS>
-__global__ void __launch_bounds__(TEAM > kRowThreads ? TEAM : kRowThreads)
+// Rows of contiguous elements that a team holds in its registers: a team is LANES lanes of a wave or as many whole waves as
+// the row needs with PACKS vectors of 16 bytes a lane, and the elements behind the last whole vector go one a lane.  One
+// read of x, one write of z, the next row on its way while one is worked on; gain and bias stay in registers over the
+// team's rows (HELD).  Loads are unconditional (a vector that is not there re-reads the row's first place, see `at`).
+template <typename T, int LANES, int PACKS, int THREADS>
+__global__ void __launch_bounds__(THREADS)
     layerNormRowsKernel(const T *x, RowView xv, const T *gain, const T *bias, T *z, RowView zv, typename Compute<T>::type *mean,
-                        typename Compute<T>::type *invStd, typename Compute<T>::type epsilon) {
+                        typename Compute<T>::type *invStd, typename Compute<T>::type epsilon, int teamWaves) {
     typedef typename Compute<T>::type C;
-    constexpr int N = Pack<T>::N, THREADS = TEAM > kRowThreads ? TEAM : kRowThreads, TEAMS = THREADS / TEAM;
-    constexpr bool HELD = TEAM < 1024;  // a lane of a block of 1024 has 128 registers, which the row itself needs
-    __shared__ C smem[THREADS / kWaveLanes];
-    const int lane = threadIdx.x % TEAM;
+    constexpr int N = Pack<T>::N;
+    constexpr bool HELD = PACKS <= 2;  // a lane of a block of 1024 has 128 registers, which more of the row needs
+    __shared__ C sums[2 * (THREADS / kWaveLanes)];
+    const int size = LANES < kWaveLanes ? LANES : teamWaves * kWaveLanes, teams = THREADS / size;
+    const int team = threadIdx.x / size, lane = threadIdx.x - team * size;
+    C *smem = sums + 2 * team * teamWaves;
+    int turn = 0;
     const int length = (int)xv.length, vectors = length / N, rest = vectors * N + lane;
     const C perLength = (C)1 / (C)length;
     int at[PACKS];
@@ -66,7 +70,7 @@ __global__ void __launch_bounds__(TEAM > kRowThreads ? TEAM : kRowThreads)
     C gRest = (C)1, bRest = (C)0;
 #pragma unroll
     for (int j = 0; j < PACKS; j++) {
-        at[j] = lane + j * TEAM < vectors ? (lane + j * TEAM) * N : 0;
+        at[j] = lane + j * size < vectors ? (lane + j * size) * N : 0;
         if (HELD && vectors > 0 && gain != nullptr) g[j] = loadPackAnywhere(gain + at[j]);
         if (HELD && vectors > 0 && bias != nullptr) b[j] = loadPackAnywhere(bias + at[j]);
     }
@@ -74,36 +78,46 @@ __global__ void __launch_bounds__(TEAM > kRowThreads ? TEAM : kRowThreads)
         if (gain != nullptr) gRest = toCompute(gain[rest]);
         if (bias != nullptr) bRest = toCompute(bias[rest]);
     }
-    for (Long r0 = (Long)blockIdx.x * TEAMS; r0 < xv.rows; r0 += (Long)gridDim.x * TEAMS) {
-        const Long r = r0 + threadIdx.x / TEAM;
-        const bool live = r < xv.rows;
-        const T *xr = x + (live ? r : r0) * xv.row;
-        Pack<T> v[PACKS];
-        C vRest = (C)0;
+    Pack<T> v[PACKS], next[PACKS];
+    C vRest = (C)0, nextRest = (C)0;
+    const Long step = (Long)gridDim.x * teams;
+    auto ask = [&](Long r0) {
+        const T *xr = x + (team < teams && r0 + team < xv.rows ? r0 + team : r0) * xv.row;
         if (vectors > 0) {
 #pragma unroll
-            for (int j = 0; j < PACKS; j++) v[j] = loadPackAnywhere(xr + at[j]);
+            for (int j = 0; j < PACKS; j++) next[j] = loadPackAnywhere(xr + at[j]);
         }
-        if (rest < length) vRest = toCompute(xr[rest]);
-        C sum = vRest;
+        if (rest < length) nextRest = toCompute(xr[rest]);
+    };
+    ask((Long)blockIdx.x * teams);
+    for (Long r0 = (Long)blockIdx.x * teams; r0 < xv.rows; r0 += step) {
+        const Long r = r0 + team;
+        const bool live = team < teams && r < xv.rows;
+#pragma unroll
+        for (int j = 0; j < PACKS; j++) v[j] = next[j];
+        vRest = nextRest;
+        if (r0 + step < xv.rows) ask(r0 + step);
+        C sum[1] = {vRest};
 #pragma unroll
         for (int j = 0; j < PACKS; j++)
-            if (lane + j * TEAM < vectors) {
+            if (lane + j * size < vectors) {
 #pragma unroll
-                for (int e = 0; e < N; e++) sum += toCompute(v[j].v[e]);
+                for (int e = 0; e < N; e++) sum[0] += toCompute(v[j].v[e]);
             }
-        const C mu = teamAll<TEAM>(sum, Add(), smem) * perLength;
-        C squares = rest < length ? (vRest - mu) * (vRest - mu) : (C)0;
+        teamSums<LANES>(sum, smem, teamWaves, turn);
+        const C mu = sum[0] * perLength;
+        C squares[1] = {rest < length ? (vRest - mu) * (vRest - mu) : (C)0};
 #pragma unroll
         for (int j = 0; j < PACKS; j++)
-            if (lane + j * TEAM < vectors) {
+            if (lane + j * size < vectors) {
 #pragma unroll
                 for (int e = 0; e < N; e++) {
                     const C d = toCompute(v[j].v[e]) - mu;
-                    squares += d * d;
+                    squares[0] = fused(d, d, squares[0]);
                 }
             }
-        const C s = (C)1 / sqrtOf(teamAll<TEAM>(squares, Add(), smem) * perLength + epsilon);
+        teamSums<LANES>(squares, smem, teamWaves, turn);
+        const C s = (C)1 / sqrtOf(squares[0] * perLength + epsilon);
         if (!live) continue;
         if (lane == 0) {
             if (mean != nullptr) mean[r] = mu;
@@ -112,7 +126,7 @@ __global__ void __launch_bounds__(TEAM > kRowThreads ? TEAM : kRowThreads)
         T *zr = z + r * zv.row;
 #pragma unroll
         for (int j = 0; j < PACKS; j++)
-            if (lane + j * TEAM < vectors) {
+            if (lane + j * size < vectors) {
                 Pack<T> o;
                 if (!HELD && gain != nullptr) g[j] = loadPackAnywhere(gain + at[j]);
                 if (!HELD && bias != nullptr) b[j] = loadPackAnywhere(bias + at[j]);
@@ -170,17 +184,18 @@ __global__ void __launch_bounds__(kRowThreads) layerNormBpAnyKernel(const T *x, 
 // One block of 1024 threads a compute unit (two where a lane holds one vector): every block leaves two rows of partial sums,
 // which is why there are no more of them, and 16 waves hide the loads of each other.
 constexpr int kBpThreads = 1024;
-template <typename T, int TEAM, int PACKS>
+template <typename T, int LANES, int PACKS>
 __global__ void __launch_bounds__(kBpThreads)
     layerNormBpRowsKernel(const T *x, RowView xv, const T *gain, const typename Compute<T>::type *mean, const typename Compute<T>::type *invStd,
-                          const T *dz, RowView dzv, T *dx, RowView dxv, typename Compute<T>::type *partial) {
+                          const T *dz, RowView dzv, T *dx, RowView dxv, typename Compute<T>::type *partial, int teamWaves) {
     typedef typename Compute<T>::type C;
-    constexpr int N = Pack<T>::N, THREADS = kBpThreads, TEAMS = THREADS / TEAM;
+    constexpr int N = Pack<T>::N;
     extern __shared__ __align__(16) char dynamicLds[];
-    C *columns = reinterpret_cast<C *>(dynamicLds);  // [TEAMS / 2][columns of a row]
-    __shared__ C sums[4 * (THREADS / kWaveLanes)];
-    const int lane = threadIdx.x % TEAM, team = threadIdx.x / TEAM;
-    C *smem = sums + 4 * team * (TEAM / kWaveLanes);
+    C *columns = reinterpret_cast<C *>(dynamicLds);  // [half of the teams][columns of a row]
+    __shared__ C sums[4 * (kBpThreads / kWaveLanes)];
+    const int size = LANES < kWaveLanes ? LANES : teamWaves * kWaveLanes, teams = kBpThreads / size;
+    const int team = threadIdx.x / size, lane = threadIdx.x - team * size;
+    C *smem = sums + 4 * team * teamWaves;
     int turn = 0;
     const int length = (int)xv.length, vectors = length / N, rest = vectors * N + lane;
     const C perLength = (C)1 / (C)length;
@@ -189,7 +204,7 @@ __global__ void __launch_bounds__(kBpThreads)
     C gainSum[PACKS][N], biasSum[PACKS][N], gainRest = (C)0, biasRest = (C)0, gRest = (C)1;
 #pragma unroll
     for (int j = 0; j < PACKS; j++) {
-        at[j] = lane + j * TEAM < vectors ? (lane + j * TEAM) * N : 0;
+        at[j] = lane + j * size < vectors ? (lane + j * size) * N : 0;
         if (vectors > 0 && gain != nullptr) g[j] = loadPackAnywhere(gain + at[j]);
 #pragma unroll
         for (int e = 0; e < N; e++) gainSum[j][e] = biasSum[j][e] = (C)0;
@@ -198,9 +213,9 @@ __global__ void __launch_bounds__(kBpThreads)
     // the next row is on its way while this one is worked on
     Pack<T> v[PACKS], d[PACKS], nextV[PACKS], nextD[PACKS];
     C vRest = (C)0, dRest = (C)0, nextVRest = (C)0, nextDRest = (C)0, mu = (C)0, s = (C)0, nextMu = (C)0, nextS = (C)0;
-    const Long step = (Long)gridDim.x * TEAMS;
+    const Long step = (Long)gridDim.x * teams;
     auto ask = [&](Long r0) {
-        const Long r = r0 + team < xv.rows ? r0 + team : (r0 < xv.rows ? r0 : 0);
+        const Long r = team < teams && r0 + team < xv.rows ? r0 + team : r0;
         const T *xr = x + r * xv.row, *dzr = dz + r * dzv.row;
         if (vectors > 0) {
 #pragma unroll
@@ -216,9 +231,9 @@ __global__ void __launch_bounds__(kBpThreads)
             nextDRest = toCompute(dzr[rest]);
         }
     };
-    ask((Long)blockIdx.x * TEAMS);
-    for (Long r0 = (Long)blockIdx.x * TEAMS; r0 < xv.rows; r0 += step) {
-        const bool live = r0 + team < xv.rows;
+    ask((Long)blockIdx.x * teams);
+    for (Long r0 = (Long)blockIdx.x * teams; r0 < xv.rows; r0 += step) {
+        const bool live = team < teams && r0 + team < xv.rows;
         const Long r = live ? r0 + team : r0;
 #pragma unroll
         for (int j = 0; j < PACKS; j++) {
@@ -230,37 +245,37 @@ __global__ void __launch_bounds__(kBpThreads)
         mu = nextMu;
         s = nextS;
         if (r0 + step < xv.rows) ask(r0 + step);
-        C sumA = (C)0, sumAH = (C)0;
+        C sum[2] = {(C)0, (C)0};  // of a and of a h
         if (live) {
 #pragma unroll
             for (int j = 0; j < PACKS; j++)
-                if (lane + j * TEAM < vectors) {
+                if (lane + j * size < vectors) {
 #pragma unroll
                     for (int e = 0; e < N; e++) {
                         const C dd = toCompute(d[j].v[e]), h = (toCompute(v[j].v[e]) - mu) * s;
                         const C a = gain != nullptr ? dd * toCompute(g[j].v[e]) : dd;
-                        sumA += a;
-                        sumAH = fused(a, h, sumAH);
+                        sum[0] += a;
+                        sum[1] = fused(a, h, sum[1]);
                         gainSum[j][e] = fused(dd, h, gainSum[j][e]);
                         biasSum[j][e] += dd;
                     }
                 }
             if (rest < length) {
                 const C h = (vRest - mu) * s, a = dRest * gRest;
-                sumA += a;
-                sumAH += a * h;
-                gainRest += dRest * h;
+                sum[0] += a;
+                sum[1] = fused(a, h, sum[1]);
+                gainRest = fused(dRest, h, gainRest);
                 biasRest += dRest;
             }
         }
         if (dx == nullptr) continue;
-        teamSums<TEAM>(sumA, sumAH, smem, turn);
-        const C meanA = sumA * perLength, meanAH = sumAH * perLength;
+        teamSums<LANES>(sum, smem, teamWaves, turn);
+        const C meanA = sum[0] * perLength, meanAH = sum[1] * perLength;
         if (!live) continue;
         T *dxr = dx + r * dxv.row;
 #pragma unroll
         for (int j = 0; j < PACKS; j++)
-            if (lane + j * TEAM < vectors) {
+            if (lane + j * size < vectors) {
                 Pack<T> o;
 #pragma unroll
                 for (int e = 0; e < N; e++) {
@@ -277,24 +292,24 @@ __global__ void __launch_bounds__(kBpThreads)
 #pragma unroll
     for (int which = 0; which < 2; which++) {
         // the upper half of the teams hands its sums to the lower half, until the first team has them all
-#pragma unroll
-        for (int half = TEAMS / 2; half >= 1; half /= 2) {
-            C *shared = columns + (size_t)(team % half) * length;
+        for (int have = teams; have > 1; have = (have + 1) / 2) {
+            const int half = (have + 1) / 2;
+            C *shared = columns + (size_t)(team < half ? team : team - half) * length;
             __syncthreads();
-            if (team >= half && team < 2 * half) {
+            if (team >= half && team < have) {
 #pragma unroll
                 for (int j = 0; j < PACKS; j++)
-                    if (lane + j * TEAM < vectors) {
+                    if (lane + j * size < vectors) {
 #pragma unroll
                         for (int e = 0; e < N; e++) shared[at[j] + e] = which == 0 ? gainSum[j][e] : biasSum[j][e];
                     }
                 if (rest < length) shared[rest] = which == 0 ? gainRest : biasRest;
             }
             __syncthreads();
-            if (team < half) {
+            if (team < have - half) {
 #pragma unroll
                 for (int j = 0; j < PACKS; j++)
-                    if (lane + j * TEAM < vectors) {
+                    if (lane + j * size < vectors) {
 #pragma unroll
                         for (int e = 0; e < N; e++) (which == 0 ? gainSum[j][e] : biasSum[j][e]) += shared[at[j] + e];
                     }
@@ -305,7 +320,7 @@ __global__ void __launch_bounds__(kBpThreads)
         C *out = partial + ((size_t)which * gridDim.x + blockIdx.x) * length;
 #pragma unroll
         for (int j = 0; j < PACKS; j++)
-            if (lane + j * TEAM < vectors) {
+            if (lane + j * size < vectors) {
 #pragma unroll
                 for (int e = 0; e < N; e++) out[at[j] + e] = which == 0 ? gainSum[j][e] : biasSum[j][e];
             }
@@ -385,6 +400,13 @@ int columnSplits(Long rows, Long length) {
     return (int)(splits < 1 ? 1 : splits);
 }
 
+// the waves of a team that holds a row in `packs` vectors a lane
+int teamWaves(Long vectors, int packs) {
+    const Long waves = (vectors + (Long)kWaveLanes * packs - 1) / ((Long)kWaveLanes * packs);
+    return (int)(waves < 1 ? 1 : waves);
+}
+constexpr int kFullBlocks = 512;  // blocks of 1024 threads that the chip holds at once
+
 unsigned gridOf(Long blocks) { return (unsigned)(blocks < 1 ? 1 : (blocks > (1 << 20) ? (1 << 20) : blocks)); }
 
 }  // namespace
@@ -396,13 +418,14 @@ size_t layerNormBpScratch(Long rows, Long length) {
     return (size_t)2 * (any > held ? any : held) * length * sizeof(double);
 }
 
-template <typename T, int TEAM, int PACKS>
+template <typename T, int LANES, int PACKS, int THREADS>
 void runRows(hipStream_t s, const T *x, const RowView &xv, const T *gain, const T *bias, T *z, const RowView &zv,
              typename Compute<T>::type *mean, typename Compute<T>::type *invStd, double epsilon) {
     typedef typename Compute<T>::type C;
-    constexpr int THREADS = TEAM > kRowThreads ? TEAM : kRowThreads, TEAMS = THREADS / TEAM;
-    const unsigned blocks = (unsigned)gridFor(xv.rows, TEAMS, kGridCap * kRowThreads / THREADS);
-    ND4J_LAUNCH((layerNormRowsKernel<T, TEAM, PACKS>), dim3(blocks), dim3(THREADS), 0, s, x, xv, gain, bias, z, zv, mean, invStd, (C)epsilon);
+    const int waves = teamWaves(xv.length / Pack<T>::N, PACKS), teams = LANES < kWaveLanes ? THREADS / LANES : THREADS / kWaveLanes / waves;
+    const unsigned blocks = (unsigned)gridFor(xv.rows, teams, kFullBlocks * 1024 / THREADS);
+    ND4J_LAUNCH((layerNormRowsKernel<T, LANES, PACKS, THREADS>), dim3(blocks), dim3(THREADS), 0, s, x, xv, gain, bias, z, zv, mean, invStd,
+                (C)epsilon, waves);
 }
 
 template <typename T>
@@ -411,33 +434,32 @@ void launchLayerNorm(hipStream_t s, const T *x, const RowView &xv, const T *gain
     typedef typename Compute<T>::type C;
     if (xv.el == 1 && zv.el == 1) {
         const Long vectors = xv.length / Pack<T>::N;
-#define ROWS(TEAM, PACKS) return runRows<T, TEAM, PACKS>(s, x, xv, gain, bias, z, zv, mean, invStd, epsilon)
-        if (vectors <= 16) ROWS(16, 1);
-        if (vectors <= 32) ROWS(16, 2);
-        if (vectors <= 64) ROWS(64, 1);
-        if (vectors <= 128) ROWS(64, 2);
-        if (vectors <= 256) ROWS(64, 4);
-        if (vectors <= 512) ROWS(256, 2);
-        if (vectors <= 1024) ROWS(256, 4);
-        if (vectors <= 2048) ROWS(1024, 2);
+#define ROWS(LANES, PACKS, THREADS) return runRows<T, LANES, PACKS, THREADS>(s, x, xv, gain, bias, z, zv, mean, invStd, epsilon)
+        if (vectors <= 16) ROWS(16, 1, 256);
+        if (vectors <= 32) ROWS(16, 2, 256);
+        if (vectors <= 64) ROWS(64, 1, 256);
+        if (vectors <= 256) ROWS(64, 2, 256);
+        if (vectors <= 1024) ROWS(64, 2, 512);
+        if (vectors <= 2048) ROWS(64, 2, 1024);
         if constexpr (sizeof(T) > 2)  // (32 halves a lane do not fit its 128 registers as floats)
-            if (vectors <= 4096) ROWS(1024, 4);
+            if (vectors <= 4096) ROWS(64, 4, 1024);
 #undef ROWS
     }
     ND4J_LAUNCH((layerNormAnyKernel<T>), dim3(gridOf(xv.rows)), dim3(kRowThreads), 0, s, x, xv, gain, bias, z, zv, mean, invStd, (C)epsilon);
 }
 
 // runs the register kernel and returns the number of its blocks
-template <typename T, int TEAM, int PACKS>
+template <typename T, int LANES, int PACKS>
 int runBpRows(hipStream_t s, const T *x, const RowView &xv, const T *gain, const typename Compute<T>::type *mean,
               const typename Compute<T>::type *invStd, const T *dz, const RowView &dzv, T *dx, const RowView &dxv,
               typename Compute<T>::type *partial) {
     typedef typename Compute<T>::type C;
-    constexpr int THREADS = kBpThreads, TEAMS = THREADS / TEAM;
-    const int blocks = gridFor(xv.rows, TEAMS, PACKS == 1 ? 2 * kBpBlocks : kBpBlocks);
-    const size_t lds = TEAMS > 1 && partial != nullptr ? (size_t)(TEAMS / 2) * xv.length * sizeof(C) : 0;
-    ND4J_LAUNCH((layerNormBpRowsKernel<T, TEAM, PACKS>), dim3(blocks), dim3(THREADS), lds, s, x, xv, gain, mean, invStd, dz, dzv, dx, dxv,
-                partial);
+    const int waves = teamWaves(xv.length / Pack<T>::N, PACKS);
+    const int teams = LANES < kWaveLanes ? kBpThreads / LANES : kBpThreads / kWaveLanes / waves;
+    const int blocks = gridFor(xv.rows, teams, PACKS == 1 ? 2 * kBpBlocks : kBpBlocks);
+    const size_t lds = partial != nullptr ? (size_t)(teams / 2) * xv.length * sizeof(C) : 0;
+    ND4J_LAUNCH((layerNormBpRowsKernel<T, LANES, PACKS>), dim3(blocks), dim3(kBpThreads), lds, s, x, xv, gain, mean, invStd, dz, dzv, dx, dxv,
+                partial, waves);
     return blocks;
 }
 
@@ -451,14 +473,10 @@ void launchLayerNormBp(hipStream_t s, const T *x, const RowView &xv, const T *ga
     int splits = 0;
     if (xv.el == 1 && dzv.el == 1 && dxv.el == 1 && xv.rows > 0) {
         const Long vectors = xv.length / Pack<T>::N;
-#define ROWS(TEAM, PACKS) splits = runBpRows<T, TEAM, PACKS>(s, x, xv, gain, mean, invStd, dz, dzv, dx, dxv, partial)
+#define ROWS(LANES, PACKS) splits = runBpRows<T, LANES, PACKS>(s, x, xv, gain, mean, invStd, dz, dzv, dx, dxv, partial)
         if (vectors <= 16) ROWS(16, 1);
         else if (vectors <= 64) ROWS(64, 1);
-        else if (vectors <= 128) ROWS(64, 2);
-        else if (vectors <= 256) ROWS(128, 2);
-        else if (vectors <= 512) ROWS(256, 2);
-        else if (vectors <= 1024) ROWS(512, 2);
-        else if (vectors <= 2048) ROWS(1024, 2);
+        else if (vectors <= 2048) ROWS(64, 2);
 #undef ROWS
     }
     if (splits == 0) {  // any other view: the columns first, since dx may lie where dz or x does

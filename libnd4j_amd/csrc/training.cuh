@@ -76,34 +76,27 @@ template <int THREADS, class Op, typename C> __device__ __forceinline__ C blockA
     return v;
 }
 
-// the same for teams of 16, 32 or 64 lanes or whole blocks
-template <int TEAM, class Op, typename C> __device__ __forceinline__ C teamAll(C v, Op op, C *smem) {
-    if constexpr (TEAM <= kWaveLanes) return waveAll<TEAM>(v, op);
-    else return blockAll<TEAM>(v, op, smem);
-}
-
-// Two sums at once, for teams that take turn after turn: smem holds two of C per wave of the team twice over, for even and
-// odd turns, so that one barrier a turn is enough.
-template <int TEAM, typename C> __device__ __forceinline__ void teamSums(C &a, C &b, C *smem, int &turn) {
-    constexpr int W = TEAM <= kWaveLanes ? TEAM : kWaveLanes;
-    a = waveAll<W>(a, Add());
-    b = waveAll<W>(b, Add());
-    if constexpr (TEAM > kWaveLanes) {
-        constexpr int WAVES = TEAM / kWaveLanes;
-        C *mine = smem + (turn & 1) * 2 * WAVES;
-        turn++;
-        if (threadIdx.x % kWaveLanes == 0) {
-            mine[threadIdx.x % TEAM / kWaveLanes] = a;
-            mine[WAVES + threadIdx.x % TEAM / kWaveLanes] = b;
-        }
-        __syncthreads();
-        a = mine[0];
-        b = mine[WAVES];
+// The sum over a team of LANES lanes (a part of a wave, waves == 1) or of `waves` whole waves; all teams of a block call it
+// together, turn after turn.  smem: two values per wave of the team, for even and odd turns, so that one barrier a turn is
+// enough.  VALUES sums at once.
+template <int LANES, int VALUES, typename C>
+__device__ __forceinline__ void teamSums(C (&v)[VALUES], C *smem, int waves, int &turn) {
 #pragma unroll
-        for (int w = 1; w < WAVES; w++) {
-            a += mine[w];
-            b += mine[WAVES + w];
-        }
+    for (int i = 0; i < VALUES; i++) v[i] = waveAll<LANES>(v[i], Add());
+    if (LANES < kWaveLanes || waves == 1) return;
+    C *mine = smem + (turn & 1) * VALUES * waves;
+    turn++;
+    const int wave = threadIdx.x / kWaveLanes % waves;
+    if (threadIdx.x % kWaveLanes == 0) {
+#pragma unroll
+        for (int i = 0; i < VALUES; i++) mine[wave * VALUES + i] = v[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < VALUES; i++) v[i] = mine[i];
+    for (int w = 1; w < waves; w++) {
+#pragma unroll
+        for (int i = 0; i < VALUES; i++) v[i] += mine[w * VALUES + i];
     }
 }
 __device__ __forceinline__ float fused(float a, float b, float c) { return __builtin_fmaf(a, b, c); }
