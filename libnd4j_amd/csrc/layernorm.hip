@@ -15,6 +15,26 @@ using namespace tr;
 
 constexpr int kRowThreads = 256;
 
+// Steps in a form that takes a half operand as it is: one instruction converts it, multiplies and adds, where a conversion of
+// its own and the two operations would be three.
+// acc + v
+template <typename T> __device__ __forceinline__ typename Compute<T>::type plus(typename Compute<T>::type acc, T v) {
+    if constexpr (sizeof(T) == 2) return fused(toCompute(v), 1.0f, acc);
+    else return acc + toCompute(v);
+}
+// (v - mu) s; offset = -mu s.  For halves as v s - mu s: it rounds mu s, 2^-24 of it, where the result keeps 2^-11 of itself.
+template <typename T>
+__device__ __forceinline__ typename Compute<T>::type normal(T v, typename Compute<T>::type mu, typename Compute<T>::type s,
+                                                            typename Compute<T>::type offset) {
+    if constexpr (sizeof(T) == 2) return fused(toCompute(v), s, offset);
+    else return (toCompute(v) - mu) * s;
+}
+// a b
+template <typename T> __device__ __forceinline__ typename Compute<T>::type times(T a, T b) {
+    if constexpr (sizeof(T) == 2) return fused(toCompute(a), toCompute(b), 0.0f);
+    else return toCompute(a) * toCompute(b);
+}
+
 // Any view: a block per row, element by element.
 template <typename T>
 __global__ void __launch_bounds__(kRowThreads) layerNormAnyKernel(const T *x, RowView xv, const T *gain, const T *bias, T *z, RowView zv,
@@ -51,15 +71,15 @@ __global__ void __launch_bounds__(kRowThreads) layerNormAnyKernel(const T *x, Ro
 // the row needs with PACKS vectors of 16 bytes a lane, and the elements behind the last whole vector go one a lane.  One
 // read of x, one write of z, the next row on its way while one is worked on; gain and bias stay in registers over the
 // team's rows (HELD).  Loads are unconditional (a vector that is not there re-reads the row's first place, see `at`).
-template <typename T, int LANES, int PACKS, int THREADS>
-__global__ void __launch_bounds__(THREADS)
+template <typename T, int LANES, int PACKS>
+__global__ void __launch_bounds__(1024)
     layerNormRowsKernel(const T *x, RowView xv, const T *gain, const T *bias, T *z, RowView zv, typename Compute<T>::type *mean,
                         typename Compute<T>::type *invStd, typename Compute<T>::type epsilon, int teamWaves) {
     typedef typename Compute<T>::type C;
     constexpr int N = Pack<T>::N;
     constexpr bool HELD = PACKS <= 2;  // a lane of a block of 1024 has 128 registers, which more of the row needs
-    __shared__ C sums[2 * (THREADS / kWaveLanes)];
-    const int size = LANES < kWaveLanes ? LANES : teamWaves * kWaveLanes, teams = THREADS / size;
+    __shared__ C sums[2 * (1024 / kWaveLanes)];
+    const int size = LANES < kWaveLanes ? LANES : teamWaves * kWaveLanes, teams = blockDim.x / size;
     const int team = threadIdx.x / size, lane = threadIdx.x - team * size;
     C *smem = sums + 2 * team * teamWaves;
     int turn = 0;
@@ -102,7 +122,7 @@ __global__ void __launch_bounds__(THREADS)
         for (int j = 0; j < PACKS; j++)
             if (lane + j * size < vectors) {
 #pragma unroll
-                for (int e = 0; e < N; e++) sum[0] += toCompute(v[j].v[e]);
+                for (int e = 0; e < N; e++) sum[0] = plus(sum[0], v[j].v[e]);
             }
         teamSums<LANES>(sum, smem, teamWaves, turn);
         const C mu = sum[0] * perLength;
@@ -112,12 +132,12 @@ __global__ void __launch_bounds__(THREADS)
             if (lane + j * size < vectors) {
 #pragma unroll
                 for (int e = 0; e < N; e++) {
-                    const C d = toCompute(v[j].v[e]) - mu;
+                    const C d = plus(-mu, v[j].v[e]);
                     squares[0] = fused(d, d, squares[0]);
                 }
             }
         teamSums<LANES>(squares, smem, teamWaves, turn);
-        const C s = (C)1 / sqrtOf(squares[0] * perLength + epsilon);
+        const C s = (C)1 / sqrtOf(squares[0] * perLength + epsilon), offset = -mu * s;
         if (!live) continue;
         if (lane == 0) {
             if (mean != nullptr) mean[r] = mu;
@@ -132,18 +152,15 @@ __global__ void __launch_bounds__(THREADS)
                 if (!HELD && bias != nullptr) b[j] = loadPackAnywhere(bias + at[j]);
 #pragma unroll
                 for (int e = 0; e < N; e++) {
-                    C h = (toCompute(v[j].v[e]) - mu) * s;
-                    if (gain != nullptr) h *= toCompute(g[j].v[e]);
-                    if (bias != nullptr) h += toCompute(b[j].v[e]);
+                    C h = normal(v[j].v[e], mu, s, offset);
+                    if (gain != nullptr) h = fused(h, toCompute(g[j].v[e]), bias != nullptr ? toCompute(b[j].v[e]) : (C)0);
+                    else if (bias != nullptr) h += toCompute(b[j].v[e]);
                     o.v[e] = fromCompute<T>(h);
                 }
                 storePackAnywhere(zr + at[j], o);
             }
         if (rest < length) {
-            C h = (vRest - mu) * s;
-            if (gain != nullptr) h *= gRest;
-            if (bias != nullptr) h += bRest;
-            zr[rest] = fromCompute<T>(h);
+            zr[rest] = fromCompute<T>(fused((vRest - mu) * s, gRest, bRest));
         }
     }
 }
@@ -244,6 +261,7 @@ __global__ void __launch_bounds__(kBpThreads)
         dRest = nextDRest;
         mu = nextMu;
         s = nextS;
+        const C offset = -mu * s;
         if (r0 + step < xv.rows) ask(r0 + step);
         C sum[2] = {(C)0, (C)0};  // of a and of a h
         if (live) {
@@ -252,12 +270,12 @@ __global__ void __launch_bounds__(kBpThreads)
                 if (lane + j * size < vectors) {
 #pragma unroll
                     for (int e = 0; e < N; e++) {
-                        const C dd = toCompute(d[j].v[e]), h = (toCompute(v[j].v[e]) - mu) * s;
-                        const C a = gain != nullptr ? dd * toCompute(g[j].v[e]) : dd;
+                        const C dd = toCompute(d[j].v[e]), h = normal(v[j].v[e], mu, s, offset);
+                        const C a = gain != nullptr ? times(d[j].v[e], g[j].v[e]) : dd;
                         sum[0] += a;
                         sum[1] = fused(a, h, sum[1]);
                         gainSum[j][e] = fused(dd, h, gainSum[j][e]);
-                        biasSum[j][e] += dd;
+                        biasSum[j][e] = plus(biasSum[j][e], d[j].v[e]);
                     }
                 }
             if (rest < length) {
@@ -279,10 +297,9 @@ __global__ void __launch_bounds__(kBpThreads)
                 Pack<T> o;
 #pragma unroll
                 for (int e = 0; e < N; e++) {
-                    const C h = (toCompute(v[j].v[e]) - mu) * s;
-                    C a = toCompute(d[j].v[e]);
-                    if (gain != nullptr) a *= toCompute(g[j].v[e]);
-                    o.v[e] = fromCompute<T>(s * fused(-h, meanAH, a - meanA));
+                    const C h = normal(v[j].v[e], mu, s, offset);
+                    const C a = gain != nullptr ? fused(toCompute(d[j].v[e]), toCompute(g[j].v[e]), -meanA) : plus(-meanA, d[j].v[e]);
+                    o.v[e] = fromCompute<T>(s * fused(-h, meanAH, a));
                 }
                 storePackAnywhere(dxr + at[j], o);
             }
@@ -405,7 +422,7 @@ int teamWaves(Long vectors, int packs) {
     const Long waves = (vectors + (Long)kWaveLanes * packs - 1) / ((Long)kWaveLanes * packs);
     return (int)(waves < 1 ? 1 : waves);
 }
-constexpr int kFullBlocks = 512;  // blocks of 1024 threads that the chip holds at once
+constexpr int kFullThreads = 256 * 2048;  // that the chip holds at once
 
 unsigned gridOf(Long blocks) { return (unsigned)(blocks < 1 ? 1 : (blocks > (1 << 20) ? (1 << 20) : blocks)); }
 
@@ -418,14 +435,16 @@ size_t layerNormBpScratch(Long rows, Long length) {
     return (size_t)2 * (any > held ? any : held) * length * sizeof(double);
 }
 
-template <typename T, int LANES, int PACKS, int THREADS>
+// Blocks of about four waves, whole teams: more teams in a block would wait for each other.
+template <typename T, int LANES, int PACKS>
 void runRows(hipStream_t s, const T *x, const RowView &xv, const T *gain, const T *bias, T *z, const RowView &zv,
              typename Compute<T>::type *mean, typename Compute<T>::type *invStd, double epsilon) {
     typedef typename Compute<T>::type C;
-    const int waves = teamWaves(xv.length / Pack<T>::N, PACKS), teams = LANES < kWaveLanes ? THREADS / LANES : THREADS / kWaveLanes / waves;
-    const unsigned blocks = (unsigned)gridFor(xv.rows, teams, kFullBlocks * 1024 / THREADS);
-    ND4J_LAUNCH((layerNormRowsKernel<T, LANES, PACKS, THREADS>), dim3(blocks), dim3(THREADS), 0, s, x, xv, gain, bias, z, zv, mean, invStd,
-                (C)epsilon, waves);
+    const int waves = teamWaves(xv.length / Pack<T>::N, PACKS), teams = LANES < kWaveLanes ? 256 / LANES : (waves >= 4 ? 1 : 4 / waves);
+    const int threads = LANES < kWaveLanes ? 256 : teams * waves * kWaveLanes;
+    const unsigned blocks = (unsigned)gridFor(xv.rows, teams, kFullThreads / threads);
+    ND4J_LAUNCH((layerNormRowsKernel<T, LANES, PACKS>), dim3(blocks), dim3(threads), 0, s, x, xv, gain, bias, z, zv, mean, invStd, (C)epsilon,
+                waves);
 }
 
 template <typename T>
@@ -434,15 +453,13 @@ void launchLayerNorm(hipStream_t s, const T *x, const RowView &xv, const T *gain
     typedef typename Compute<T>::type C;
     if (xv.el == 1 && zv.el == 1) {
         const Long vectors = xv.length / Pack<T>::N;
-#define ROWS(LANES, PACKS, THREADS) return runRows<T, LANES, PACKS, THREADS>(s, x, xv, gain, bias, z, zv, mean, invStd, epsilon)
-        if (vectors <= 16) ROWS(16, 1, 256);
-        if (vectors <= 32) ROWS(16, 2, 256);
-        if (vectors <= 64) ROWS(64, 1, 256);
-        if (vectors <= 256) ROWS(64, 2, 256);
-        if (vectors <= 1024) ROWS(64, 2, 512);
-        if (vectors <= 2048) ROWS(64, 2, 1024);
+#define ROWS(LANES, PACKS) return runRows<T, LANES, PACKS>(s, x, xv, gain, bias, z, zv, mean, invStd, epsilon)
+        if (vectors <= 16) ROWS(16, 1);
+        if (vectors <= 32) ROWS(16, 2);
+        if (vectors <= 64) ROWS(64, 1);
+        if (vectors <= 2048) ROWS(64, 2);
         if constexpr (sizeof(T) > 2)  // (32 halves a lane do not fit its 128 registers as floats)
-            if (vectors <= 4096) ROWS(64, 4, 1024);
+            if (vectors <= 4096) ROWS(64, 4);
 #undef ROWS
     }
     ND4J_LAUNCH((layerNormAnyKernel<T>), dim3(gridOf(xv.rows)), dim3(kRowThreads), 0, s, x, xv, gain, bias, z, zv, mean, invStd, (C)epsilon);
