@@ -35,34 +35,103 @@ template <typename T> __device__ __forceinline__ typename Compute<T>::type times
     else return toCompute(a) * toCompute(b);
 }
 
-// Any view: a block per row, element by element.
-template <typename T>
-__global__ void __launch_bounds__(kRowThreads) layerNormAnyKernel(const T *x, RowView xv, const T *gain, const T *bias, T *z, RowView zv,
-                                                                  typename Compute<T>::type *mean, typename Compute<T>::type *invStd,
-                                                                  typename Compute<T>::type epsilon) {
+// Rows too long for the kernel below, and views of any strides: a block per row, in three sweeps of which the second and
+// third find the row in the caches.  UNIT: contiguous elements, in vectors.
+constexpr int kLongThreads = 1024;
+template <typename T, bool UNIT, typename F> __device__ __forceinline__ void sweep(const T *row, Long el, Long length, F f) {
+    constexpr int N = Pack<T>::N;
+    if constexpr (UNIT) {
+        const Long whole = length / N * N;
+#pragma unroll 2
+        for (Long c = (Long)threadIdx.x * N; c < whole; c += kLongThreads * N) {
+            const Pack<T> v = loadPackAnywhere(row + c);
+#pragma unroll
+            for (int e = 0; e < N; e++) f(c + e, v.v[e]);
+        }
+        if (whole + threadIdx.x < length) f(whole + threadIdx.x, row[whole + threadIdx.x]);
+    } else {
+#pragma unroll 4
+        for (Long c = threadIdx.x; c < length; c += kLongThreads) f(c, row[c * el]);
+    }
+}
+template <typename T, bool UNIT>
+__global__ void __launch_bounds__(kLongThreads) layerNormAnyKernel(const T *x, RowView xv, const T *gain, const T *bias, T *z, RowView zv,
+                                                                   typename Compute<T>::type *mean, typename Compute<T>::type *invStd,
+                                                                   typename Compute<T>::type epsilon) {
     typedef typename Compute<T>::type C;
-    __shared__ C smem[kRowThreads / kWaveLanes];
+    __shared__ C smem[kLongThreads / kWaveLanes];
     for (Long r = blockIdx.x; r < xv.rows; r += gridDim.x) {
         const T *xr = x + r * xv.row;
         T *zr = z + r * zv.row;
         C sum = (C)0;
-        for (Long c = threadIdx.x; c < xv.length; c += kRowThreads) sum += toCompute(xr[c * xv.el]);
-        const C mu = blockAll<kRowThreads>(sum, Add(), smem) / (C)xv.length;
+        sweep<T, UNIT>(xr, xv.el, xv.length, [&](Long, T v) { sum += toCompute(v); });
+        const C mu = blockAll<kLongThreads>(sum, Add(), smem) / (C)xv.length;
         C squares = (C)0;
-        for (Long c = threadIdx.x; c < xv.length; c += kRowThreads) {
-            const C d = toCompute(xr[c * xv.el]) - mu;
+        sweep<T, UNIT>(xr, xv.el, xv.length, [&](Long, T v) {
+            const C d = toCompute(v) - mu;
             squares += d * d;
-        }
-        const C s = (C)1 / sqrtOf(blockAll<kRowThreads>(squares, Add(), smem) / (C)xv.length + epsilon);
+        });
+        const C s = (C)1 / sqrtOf(blockAll<kLongThreads>(squares, Add(), smem) / (C)xv.length + epsilon);
         if (threadIdx.x == 0) {
             if (mean != nullptr) mean[r] = mu;
             if (invStd != nullptr) invStd[r] = s;
         }
-        for (Long c = threadIdx.x; c < xv.length; c += kRowThreads) {
-            C v = (toCompute(xr[c * xv.el]) - mu) * s;
-            if (gain != nullptr) v *= toCompute(gain[c]);
-            if (bias != nullptr) v += toCompute(bias[c]);
-            zr[c * zv.el] = fromCompute<T>(v);
+        // (stores element by element, which the compiler may not join: z may be x)
+        sweep<T, UNIT>(xr, xv.el, xv.length, [&](Long c, T v) {
+            C h = (toCompute(v) - mu) * s;
+            if (gain != nullptr) h *= toCompute(gain[c]);
+            if (bias != nullptr) h += toCompute(bias[c]);
+            zr[c * zv.el] = fromCompute<T>(h);
+        });
+    }
+}
+
+// Views whose rows lie nearer to each other than a row's elements (an f-order matrix): lanes take neighbouring rows, the
+// waves of a block share the columns.
+constexpr int kAcrossThreads = 1024, kAcrossGroups = kAcrossThreads / kWaveLanes;
+template <typename C> __device__ __forceinline__ C acrossSum(C v, C (*smem)[kWaveLanes]) {
+    const int lane = threadIdx.x % kWaveLanes, group = threadIdx.x / kWaveLanes;
+    __syncthreads();
+    smem[group][lane] = v;
+    __syncthreads();
+    v = smem[0][lane];
+#pragma unroll
+    for (int g = 1; g < kAcrossGroups; g++) v += smem[g][lane];
+    return v;
+}
+template <typename T>
+__global__ void __launch_bounds__(kAcrossThreads) layerNormAcrossKernel(const T *x, RowView xv, const T *gain, const T *bias, T *z, RowView zv,
+                                                                        typename Compute<T>::type *mean, typename Compute<T>::type *invStd,
+                                                                        typename Compute<T>::type epsilon) {
+    typedef typename Compute<T>::type C;
+    __shared__ C smem[kAcrossGroups][kWaveLanes];
+    const int lane = threadIdx.x % kWaveLanes, group = threadIdx.x / kWaveLanes;
+    for (Long r0 = (Long)blockIdx.x * kWaveLanes; r0 < xv.rows; r0 += (Long)gridDim.x * kWaveLanes) {
+        const bool live = r0 + lane < xv.rows;
+        const Long r = live ? r0 + lane : r0;
+        const T *xr = x + r * xv.row;
+        C sum = (C)0;
+#pragma unroll 8
+        for (Long c = group; c < xv.length; c += kAcrossGroups) sum += toCompute(xr[c * xv.el]);
+        const C mu = acrossSum(sum, smem) / (C)xv.length;
+        C squares = (C)0;
+#pragma unroll 8
+        for (Long c = group; c < xv.length; c += kAcrossGroups) {
+            const C d = toCompute(xr[c * xv.el]) - mu;
+            squares += d * d;
+        }
+        const C s = (C)1 / sqrtOf(acrossSum(squares, smem) / (C)xv.length + epsilon);
+        if (!live) continue;
+        if (group == 0) {
+            if (mean != nullptr) mean[r] = mu;
+            if (invStd != nullptr) invStd[r] = s;
+        }
+#pragma unroll 4
+        for (Long c = group; c < xv.length; c += kAcrossGroups) {
+            C h = (toCompute(xr[c * xv.el]) - mu) * s;
+            if (gain != nullptr) h *= toCompute(gain[c]);
+            if (bias != nullptr) h += toCompute(bias[c]);
+            z[r * zv.row + c * zv.el] = fromCompute<T>(h);
         }
     }
 }
@@ -165,31 +234,83 @@ __global__ void __launch_bounds__(1024)
     }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kRowThreads) layerNormBpAnyKernel(const T *x, RowView xv, const T *gain,
-                                                                    const typename Compute<T>::type *mean,
-                                                                    const typename Compute<T>::type *invStd, const T *dz, RowView dzv, T *dx,
-                                                                    RowView dxv) {
+// The backward pass of the same views as layerNormAnyKernel's: dx alone, in two sweeps
+template <typename T, bool UNIT, typename F>
+__device__ __forceinline__ void sweepTwo(const T *one, Long el1, const T *two, Long el2, Long length, F f) {
+    constexpr int N = Pack<T>::N;
+    if constexpr (UNIT) {
+        const Long whole = length / N * N;
+#pragma unroll 2
+        for (Long c = (Long)threadIdx.x * N; c < whole; c += kLongThreads * N) {
+            const Pack<T> v = loadPackAnywhere(one + c), w = loadPackAnywhere(two + c);
+#pragma unroll
+            for (int e = 0; e < N; e++) f(c + e, v.v[e], w.v[e]);
+        }
+        if (whole + threadIdx.x < length) f(whole + threadIdx.x, one[whole + threadIdx.x], two[whole + threadIdx.x]);
+    } else {
+#pragma unroll 4
+        for (Long c = threadIdx.x; c < length; c += kLongThreads) f(c, one[c * el1], two[c * el2]);
+    }
+}
+template <typename T, bool UNIT>
+__global__ void __launch_bounds__(kLongThreads) layerNormBpAnyKernel(const T *x, RowView xv, const T *gain,
+                                                                     const typename Compute<T>::type *mean,
+                                                                     const typename Compute<T>::type *invStd, const T *dz, RowView dzv, T *dx,
+                                                                     RowView dxv) {
     typedef typename Compute<T>::type C;
-    __shared__ C smem[kRowThreads / kWaveLanes];
+    __shared__ C smem[kLongThreads / kWaveLanes];
     for (Long r = blockIdx.x; r < xv.rows; r += gridDim.x) {
         const T *xr = x + r * xv.row, *dzr = dz + r * dzv.row;
         T *dxr = dx + r * dxv.row;
         const C mu = mean[r], s = invStd[r];
         C sumA = (C)0, sumAH = (C)0;
-        for (Long c = threadIdx.x; c < xv.length; c += kRowThreads) {
+        sweepTwo<T, UNIT>(xr, xv.el, dzr, dzv.el, xv.length, [&](Long c, T v, T d) {
+            C a = toCompute(d);
+            if (gain != nullptr) a *= toCompute(gain[c]);
+            sumA += a;
+            sumAH += a * ((toCompute(v) - mu) * s);
+        });
+        const C meanA = blockAll<kLongThreads>(sumA, Add(), smem) / (C)xv.length;
+        const C meanAH = blockAll<kLongThreads>(sumAH, Add(), smem) / (C)xv.length;
+        sweepTwo<T, UNIT>(xr, xv.el, dzr, dzv.el, xv.length, [&](Long c, T v, T d) {
+            C a = toCompute(d);
+            if (gain != nullptr) a *= toCompute(gain[c]);
+            const C h = (toCompute(v) - mu) * s;
+            dxr[c * dxv.el] = fromCompute<T>(s * (a - meanA - h * meanAH));
+        });
+    }
+}
+
+// ... and of layerNormAcrossKernel's
+template <typename T>
+__global__ void __launch_bounds__(kAcrossThreads) layerNormBpAcrossKernel(const T *x, RowView xv, const T *gain,
+                                                                          const typename Compute<T>::type *mean,
+                                                                          const typename Compute<T>::type *invStd, const T *dz, RowView dzv,
+                                                                          T *dx, RowView dxv) {
+    typedef typename Compute<T>::type C;
+    __shared__ C smem[kAcrossGroups][kWaveLanes];
+    const int lane = threadIdx.x % kWaveLanes, group = threadIdx.x / kWaveLanes;
+    for (Long r0 = (Long)blockIdx.x * kWaveLanes; r0 < xv.rows; r0 += (Long)gridDim.x * kWaveLanes) {
+        const bool live = r0 + lane < xv.rows;
+        const Long r = live ? r0 + lane : r0;
+        const T *xr = x + r * xv.row, *dzr = dz + r * dzv.row;
+        const C mu = mean[r], s = invStd[r];
+        C sumA = (C)0, sumAH = (C)0;
+#pragma unroll 4
+        for (Long c = group; c < xv.length; c += kAcrossGroups) {
             C a = toCompute(dzr[c * dzv.el]);
             if (gain != nullptr) a *= toCompute(gain[c]);
             sumA += a;
             sumAH += a * ((toCompute(xr[c * xv.el]) - mu) * s);
         }
-        const C meanA = blockAll<kRowThreads>(sumA, Add(), smem) / (C)xv.length;
-        const C meanAH = blockAll<kRowThreads>(sumAH, Add(), smem) / (C)xv.length;
-        for (Long c = threadIdx.x; c < xv.length; c += kRowThreads) {
+        const C meanA = acrossSum(sumA, smem) / (C)xv.length, meanAH = acrossSum(sumAH, smem) / (C)xv.length;
+        if (!live) continue;
+#pragma unroll 4
+        for (Long c = group; c < xv.length; c += kAcrossGroups) {
             C a = toCompute(dzr[c * dzv.el]);
             if (gain != nullptr) a *= toCompute(gain[c]);
             const C h = (toCompute(xr[c * xv.el]) - mu) * s;
-            dxr[c * dxv.el] = fromCompute<T>(s * (a - meanA - h * meanAH));
+            dx[r * dxv.row + c * dxv.el] = fromCompute<T>(s * (a - meanA - h * meanAH));
         }
     }
 }
@@ -365,6 +486,7 @@ __global__ void __launch_bounds__(kRowThreads) layerNormBpColumnsKernel(const T 
         const Long c = work % tiles * kWaveLanes + lane, split = work / tiles;
         C gainSum = (C)0, biasSum = (C)0;
         if (c < xv.length)
+#pragma unroll 4
             for (Long r = split * WAVES + wave; r < xv.rows; r += (Long)splits * WAVES) {
                 const C d = toCompute(dz[r * dzv.row + c * dzv.el]);
                 gainSum += d * ((toCompute(x[r * xv.row + c * xv.el]) - mean[r]) * invStd[r]);
@@ -380,6 +502,30 @@ __global__ void __launch_bounds__(kRowThreads) layerNormBpColumnsKernel(const T 
             for (int w = 1; w < WAVES; w++) sum += smem[wave][w][lane];
             partial[((Long)wave * splits + split) * partialPitch(xv.length) + c] = sum;
         }
+    }
+}
+
+// The same for views whose rows are nearer to each other than a row's elements: a wave takes a column, its lanes neighbouring
+// rows of its split.
+template <typename T>
+__global__ void __launch_bounds__(kRowThreads) layerNormBpColumnsAcrossKernel(const T *x, RowView xv, const typename Compute<T>::type *mean,
+                                                                              const typename Compute<T>::type *invStd, const T *dz, RowView dzv,
+                                                                              typename Compute<T>::type *partial, int splits) {
+    typedef typename Compute<T>::type C;
+    constexpr int WAVES = kRowThreads / kWaveLanes;
+    const int lane = threadIdx.x % kWaveLanes, wave = threadIdx.x / kWaveLanes;
+    for (Long work = (Long)blockIdx.x * WAVES + wave; work < xv.length * splits; work += (Long)gridDim.x * WAVES) {
+        const Long c = work % xv.length, split = work / xv.length;
+        C gainSum = (C)0, biasSum = (C)0;
+#pragma unroll 4
+        for (Long r = split * kWaveLanes + lane; r < xv.rows; r += (Long)splits * kWaveLanes) {
+            const C d = toCompute(dz[r * dzv.row + c * dzv.el]);
+            gainSum += d * ((toCompute(x[r * xv.row + c * xv.el]) - mean[r]) * invStd[r]);
+            biasSum += d;
+        }
+        gainSum = waveAll<kWaveLanes>(gainSum, Add());
+        biasSum = waveAll<kWaveLanes>(biasSum, Add());
+        if (lane < 2) partial[((Long)lane * splits + split) * partialPitch(xv.length) + c] = lane == 0 ? gainSum : biasSum;
     }
 }
 
@@ -468,7 +614,14 @@ void launchLayerNorm(hipStream_t s, const T *x, const RowView &xv, const T *gain
             if (vectors <= 4096) ROWS(64, 4);
 #undef ROWS
     }
-    ND4J_LAUNCH((layerNormAnyKernel<T>), dim3(gridOf(xv.rows)), dim3(kRowThreads), 0, s, x, xv, gain, bias, z, zv, mean, invStd, (C)epsilon);
+    const dim3 grid(gridOf(xv.rows)), block(kLongThreads);
+    if (xv.el == 1 && zv.el == 1)
+        ND4J_LAUNCH((layerNormAnyKernel<T, true>), grid, block, 0, s, x, xv, gain, bias, z, zv, mean, invStd, (C)epsilon);
+    else if (rowsAreNear(xv) && rowsAreNear(zv))
+        ND4J_LAUNCH((layerNormAcrossKernel<T>), dim3(gridOf((xv.rows + kWaveLanes - 1) / kWaveLanes)), dim3(kAcrossThreads), 0, s, x, xv, gain,
+                    bias, z, zv, mean, invStd, (C)epsilon);
+    else
+        ND4J_LAUNCH((layerNormAnyKernel<T, false>), grid, block, 0, s, x, xv, gain, bias, z, zv, mean, invStd, (C)epsilon);
 }
 
 // runs the register kernel and returns the number of its blocks
@@ -507,11 +660,23 @@ void launchLayerNormBp(hipStream_t s, const T *x, const RowView &xv, const T *ga
     if (splits == 0) {  // any other view: the columns first, since dx may lie where dz or x does
         splits = columnSplits(xv.rows, xv.length);
         const Long tiles = (xv.length + kWaveLanes - 1) / kWaveLanes;
-        if (columns)
+        const bool across = rowsAreNear(xv) && rowsAreNear(dzv);
+        if (columns && across)
+            ND4J_LAUNCH((layerNormBpColumnsAcrossKernel<T>), dim3(gridOf(xv.length * splits / 4 + 1)), dim3(kRowThreads), 0, s, x, xv, mean, invStd, dz,
+                        dzv, partial, splits);
+        else if (columns)
             ND4J_LAUNCH((layerNormBpColumnsKernel<T>), dim3(gridOf(tiles * splits)), dim3(kRowThreads), 0, s, x, xv, mean, invStd, dz, dzv, partial,
                         splits);
-        if (dx != nullptr && xv.rows > 0)
-            ND4J_LAUNCH((layerNormBpAnyKernel<T>), dim3(gridOf(xv.rows)), dim3(kRowThreads), 0, s, x, xv, gain, mean, invStd, dz, dzv, dx, dxv);
+        if (dx != nullptr && xv.rows > 0) {
+            const dim3 grid(gridOf(xv.rows)), block(kLongThreads);
+            if (xv.el == 1 && dzv.el == 1 && dxv.el == 1)
+                ND4J_LAUNCH((layerNormBpAnyKernel<T, true>), grid, block, 0, s, x, xv, gain, mean, invStd, dz, dzv, dx, dxv);
+            else if (across && rowsAreNear(dxv))
+                ND4J_LAUNCH((layerNormBpAcrossKernel<T>), dim3(gridOf((xv.rows + kWaveLanes - 1) / kWaveLanes)), dim3(kAcrossThreads), 0, s, x, xv, gain,
+                            mean, invStd, dz, dzv, dx, dxv);
+            else
+                ND4J_LAUNCH((layerNormBpAnyKernel<T, false>), grid, block, 0, s, x, xv, gain, mean, invStd, dz, dzv, dx, dxv);
+        }
     }
     if (columns)
         ND4J_LAUNCH((layerNormBpFinishKernel<T>), dim3(gridOf((xv.length + kFinishColumns - 1) / kFinishColumns), 2), dim3(kFinishThreads), 0, s,

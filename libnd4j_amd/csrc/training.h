@@ -16,6 +16,12 @@ struct RowView {
     Long row = 0, el = 1;
 };
 
+// whether a view's rows lie nearer to each other than a row's elements (an f-order matrix): lanes then take rows
+inline bool rowsAreNear(const RowView &v) {
+    const Long row = v.row < 0 ? -v.row : v.row, el = v.el < 0 ? -v.el : v.el;
+    return v.rows > 1 && row < el;
+}
+
 // ---- layer norm (layernorm.hip) ----------------------------------------------------------------------------------------
 // z = (x - mean) / sqrt(variance + epsilon) * gain + bias over the rows; gain, bias, mean, invStd may be null
 template <typename T>
