@@ -20,14 +20,14 @@ using namespace tr;
 
 constexpr int kThreads = 256;
 
-// Any view: a thread per element.
+// Any view: a thread per element, neighbouring threads along the dimension in which z's elements are nearer to each other.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) embeddingAnyKernel(const T *table, RowView tv, const Long *tokens, T *z, RowView zv,
-                                                               typename Compute<T>::type scale) {
+                                                               typename Compute<T>::type scale, bool rowsFirst) {
     typedef typename Compute<T>::type C;
     const Long total = zv.rows * zv.length;
     for (Long i = (Long)blockIdx.x * kThreads + threadIdx.x; i < total; i += (Long)gridDim.x * kThreads) {
-        const Long r = i / zv.length, c = i - r * zv.length, t = tokens[r];
+        const Long r = rowsFirst ? i % zv.rows : i / zv.length, c = rowsFirst ? i / zv.rows : i - r * zv.length, t = tokens[r];
         C v = t < 0 ? (C)0 : notANumber<C>();
         if (t >= 0 && t < tv.rows) v = toCompute(table[t * tv.row + c * tv.el]) * scale;
         z[r * zv.row + c * zv.el] = fromCompute<T>(v);
@@ -557,7 +557,7 @@ void launchEmbedding(hipStream_t s, const T *table, const RowView &tv, const Lon
         return;
     }
     ND4J_LAUNCH((embeddingAnyKernel<T>), dim3(gridFor(zv.rows * zv.length, kThreads, kGridCap)), dim3(kThreads), 0, s, table, tv, tokens, z, zv,
-                (C)scale);
+                (C)scale, rowsAreNear(zv));
 }
 
 template <typename T>

@@ -28,7 +28,7 @@ template <typename C> struct Better {  // larger value first, then lower index; 
     }
 };
 
-// Any view: a block per row, element by element, and a sweep of the row for every alternative.
+// Views of any other strides: a block per row, element by element, and a sweep of the row for every alternative.
 template <typename T>
 __global__ void __launch_bounds__(kRowThreads) tokenProbsAnyKernel(const T *x, RowView xv, const Long *tokens, TokenProbsOut<T> out) {
     typedef typename Compute<T>::type C;
@@ -89,6 +89,94 @@ __global__ void __launch_bounds__(kRowThreads) tokenProbsAnyKernel(const T *x, R
                     if (out.topLogProbs != nullptr) out.topLogProbs[r * out.k + j] = notANumber<C>();
                 }
                 break;
+            }
+        }
+    }
+}
+
+// Views whose rows lie nearer to each other than a row's elements (an f-order matrix, as products of matrices often are):
+// lanes take neighbouring rows, the waves of a block share the columns; a sweep for every alternative here too.
+constexpr int kAcrossThreads = 1024, kAcrossGroups = kAcrossThreads / kWaveLanes;
+template <typename T>
+__global__ void __launch_bounds__(kAcrossThreads) tokenProbsAcrossKernel(const T *x, RowView xv, const Long *tokens, TokenProbsOut<T> out) {
+    typedef typename Compute<T>::type C;
+    __shared__ C one[kAcrossGroups][kWaveLanes], two[kAcrossGroups][kWaveLanes];
+    __shared__ int indexes[kAcrossGroups][kWaveLanes];
+    const int lane = threadIdx.x % kWaveLanes, group = threadIdx.x / kWaveLanes;
+    for (Long r0 = (Long)blockIdx.x * kWaveLanes; r0 < xv.rows; r0 += (Long)gridDim.x * kWaveLanes) {
+        const bool live = r0 + lane < xv.rows;
+        const Long r = live ? r0 + lane : r0;
+        const T *xr = x + r * xv.row;
+        C mx = -infinite<C>();
+#pragma unroll 8
+        for (Long c = group; c < xv.length; c += kAcrossGroups) mx = Largest()(mx, toCompute(xr[c * xv.el]));
+        __syncthreads();
+        one[group][lane] = mx;
+        __syncthreads();
+        for (int g = 0; g < kAcrossGroups; g++) mx = Largest()(mx, one[g][lane]);
+        if (mx == -infinite<C>()) mx = (C)0;
+        C sum = (C)0, weighted = (C)0;
+#pragma unroll 4
+        for (Long c = group; c < xv.length; c += kAcrossGroups) {
+            const C d = toCompute(xr[c * xv.el]) - mx, e = m::expSoft_(d);
+            sum += e;
+            if (d > -infinite<C>()) weighted -= d * e;
+        }
+        __syncthreads();
+        one[group][lane] = sum;
+        two[group][lane] = weighted;
+        __syncthreads();
+        sum = one[0][lane];
+        weighted = two[0][lane];
+        for (int g = 1; g < kAcrossGroups; g++) {
+            sum += one[g][lane];
+            weighted += two[g][lane];
+        }
+        const bool none = sum == (C)0;
+        const C logSum = m::logSoft_(sum);
+        if (live && group == 0) {
+            if (out.logSum != nullptr) out.logSum[r] = mx + logSum;
+            if (out.entropy != nullptr) out.entropy[r] = none ? (C)0 : logSum + weighted / sum;
+            if (out.logProbs != nullptr) {
+                const Long t = tokens[r];
+                C lp = (C)0;
+                if (t >= xv.length) lp = notANumber<C>();
+                else if (t >= 0) lp = none ? -infinite<C>() : (toCompute(xr[t * xv.el]) - mx) - logSum;
+                out.logProbs[r] = lp;
+            }
+        }
+        Entry<C> last;
+        last.value = infinite<C>();
+        last.index = -1;
+        bool more = true;  // (a lane whose row has no more numbers goes on with the others)
+        for (int k = 0; k < out.k; k++) {
+            Entry<C> best;
+            best.value = (C)0;
+            best.index = -1;
+#pragma unroll 4
+            for (Long c = group; c < xv.length; c += kAcrossGroups) {
+                Entry<C> e;
+                e.value = toCompute(xr[c * xv.el]);
+                e.index = (int)c;
+                const bool is = more && e.value == e.value && (k == 0 || e.value < last.value || (e.value == last.value && e.index > last.index));
+                if (is) best = Better<C>()(best, e);
+            }
+            __syncthreads();
+            one[group][lane] = best.value;
+            indexes[group][lane] = best.index;
+            __syncthreads();
+            for (int g = 0; g < kAcrossGroups; g++) {
+                Entry<C> e;
+                e.value = one[g][lane];
+                e.index = indexes[g][lane];
+                best = Better<C>()(best, e);
+            }
+            last = best;
+            more = more && last.index >= 0;
+            if (live && group == 0) {
+                out.top[r * out.k + k] = more ? last.index : -1;
+                if (out.topLogProbs != nullptr)
+                    out.topLogProbs[r * out.k + k] = !more ? notANumber<C>() : (none ? -infinite<C>() : (last.value - mx) - logSum);
             }
         }
     }
@@ -577,6 +665,38 @@ __global__ void __launch_bounds__(kRowThreads) tokenProbsBpAnyKernel(const T *x,
     }
 }
 
+// Views whose rows lie nearer to each other than a row's elements: lanes take neighbouring rows, a wave a stretch of columns.
+constexpr int kAcrossColumns = 64;
+template <typename T>
+__global__ void __launch_bounds__(kRowThreads) tokenProbsBpAcrossKernel(const T *x, RowView xv, const Long *tokens,
+                                                                        const typename Compute<T>::type *logSum,
+                                                                        const typename Compute<T>::type *entropy,
+                                                                        const typename Compute<T>::type *dLogProbs,
+                                                                        const typename Compute<T>::type *dEntropy, T *dx, RowView dxv,
+                                                                        Long rowTiles) {
+    typedef typename Compute<T>::type C;
+    constexpr int WAVES = kRowThreads / kWaveLanes;
+    const int lane = threadIdx.x % kWaveLanes, wave = threadIdx.x / kWaveLanes;
+    const Long stretches = (xv.length + kAcrossColumns - 1) / kAcrossColumns;
+    for (Long work = (Long)blockIdx.x * WAVES + wave; work < rowTiles * stretches; work += (Long)gridDim.x * WAVES) {
+        const Long r = work % rowTiles * kWaveLanes + lane, begin = work / rowTiles * kAcrossColumns;
+        const Long end = begin + kAcrossColumns < xv.length ? begin + kAcrossColumns : xv.length;
+        if (r >= xv.rows) continue;
+        const C ls = logSum[r];
+        const Long t = dLogProbs != nullptr ? tokens[r] : -1;
+        C a = t < 0 ? (C)0 : dLogProbs[r];
+        if (t >= xv.length) a = notANumber<C>();
+        const C b = dEntropy != nullptr ? dEntropy[r] : (C)0, h = dEntropy != nullptr ? entropy[r] : (C)0;
+#pragma unroll 4
+        for (Long c = begin; c < end; c++) {
+            const C lp = toCompute(x[r * xv.row + c * xv.el]) - ls, p = m::expSoft_(lp);
+            C d = (c == t ? a : (C)0) - a * p;
+            if (dEntropy != nullptr && p != (C)0) d -= b * p * (lp + h);
+            dx[r * dxv.row + c * dxv.el] = fromCompute<T>(ls == -infinite<C>() ? (C)0 : d);
+        }
+    }
+}
+
 // Rows of contiguous elements: a team of a wave or a block takes a stretch of a row, four vectors a lane and round.
 template <typename T, int TEAM, bool ENTROPY>
 __global__ void __launch_bounds__(kRowThreads) tokenProbsBpRowsKernel(const T *x, RowView xv, const Long *tokens,
@@ -718,6 +838,10 @@ void launchTokenLogProbs(hipStream_t s, const T *x, const RowView &xv, const Lon
         }
         return;
     }
+    if (rowsAreNear(xv)) {
+        ND4J_LAUNCH((tokenProbsAcrossKernel<T>), dim3(gridOf((xv.rows + kWaveLanes - 1) / kWaveLanes)), dim3(kAcrossThreads), 0, s, x, xv, tokens, out);
+        return;
+    }
     ND4J_LAUNCH((tokenProbsAnyKernel<T>), dim3(gridOf(xv.rows)), dim3(kRowThreads), 0, s, x, xv, tokens, out);
 }
 
@@ -742,6 +866,12 @@ void launchTokenLogProbsBp(hipStream_t s, const T *x, const RowView &xv, const L
             else RUN(kRowThreads, false);
         }
 #undef RUN
+        return;
+    }
+    if (rowsAreNear(xv) && rowsAreNear(dxv)) {
+        const Long rowTiles = (xv.rows + kWaveLanes - 1) / kWaveLanes, work = rowTiles * ((xv.length + kAcrossColumns - 1) / kAcrossColumns);
+        ND4J_LAUNCH((tokenProbsBpAcrossKernel<T>), dim3(gridOf((work + 3) / 4)), dim3(kRowThreads), 0, s, x, xv, tokens, logSum, entropy, dLogProbs,
+                    dEntropy, dx, dxv, rowTiles);
         return;
     }
     ND4J_LAUNCH((tokenProbsBpAnyKernel<T>), dim3(gridOf(xv.rows)), dim3(kRowThreads), 0, s, x, xv, tokens, logSum, entropy, dLogProbs, dEntropy,
