@@ -466,8 +466,9 @@ def test_token_log_probs_layouts(dev, S, layout):
 
 
 @pytest.mark.parametrize("S", SUFFIXES)
-@pytest.mark.parametrize("n", (70, 3001, 40000))
-def test_token_log_probs_of_masked_and_equal_rows(dev, S, n):
+@pytest.mark.parametrize("n,layout", [(70, "dense"), (70, "forder"), (70, "inner2"), (3001, "dense"), (3001, "forder"), (3001, "pitch3"),
+                                      (40000, "dense")])
+def test_token_log_probs_of_masked_and_equal_rows(dev, S, n, layout):
     """rows of equal values, of few values, ascending and descending rows, masks of -infinity and of the type's lowest value
     with nothing, one element, few and all but one left, the largest values, signed zeros, NaN and +infinity"""
     rs = np.random.RandomState(n)
@@ -499,7 +500,16 @@ def test_token_log_probs_of_masked_and_equal_rows(dev, S, n):
     x = np.array(rows).astype(STORAGE[S])
     for tokens in (np.arange(len(rows)) % n, np.full(len(rows), -1), np.full(len(rows), n - 1)):
         for k in (5, 64):
-            check_token_probs(run_token_probs(dev, S, x, tokens, k), token_probs_oracle(x, tokens, k, S))
+            check_token_probs(run_token_probs(dev, S, x, tokens, k, layout), token_probs_oracle(x, tokens, k, S))
+    # many rows at once: each of them is a block's (a wave's, where it is short) instead of being cut into slices
+    many = np.tile(x, (1024 // len(rows) + 1, 1)) if n <= 3001 else x[:0]
+    if len(many):
+        tokens = np.arange(len(many)) % n
+        got, few = run_token_probs(dev, S, many, tokens, 5, layout), token_probs_oracle(x, tokens[:len(rows)], 5, S)
+        want = {key: np.tile(v, (len(many) // len(rows),) + (1,) * (v.ndim - 1)) for key, v in few.items()}
+        for key in ("lp", "t_lp"):  # (the tokens differ from one copy of the rows to the next)
+            want[key] = np.concatenate([token_probs_oracle(x, tokens[i:i + len(rows)], 0, S)[key] for i in range(0, len(many), len(rows))])
+        check_token_probs(got, want)
 
 
 def test_token_log_probs_parts(dev):
