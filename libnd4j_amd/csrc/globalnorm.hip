@@ -2,12 +2,15 @@
 //
 //   norm = sqrt(sum of g^2),  f = maxNorm / norm where maxNorm < norm < infinity, else 1,  out = f g
 //
-// The tensors' elements count as one range, cut into tiles that the blocks take in turn, from the range's start for the norm
-// and from its end for the result, so that what the first launch read last - the most that the last-level cache holds of
-// it - is read first by the second.  A tile inside one tensor is walked in vectors (unaligned ones: tensors may begin
-// anywhere), a tile that holds ends of tensors vector by vector too, every thread looking the tensor up for its own
-// (a vector across tensors goes element by element): a thousand tensors of ten elements cost no more launches than one of
-// ten thousand.
+// The tensors' elements count as one range, cut into tiles that the blocks take in turn.  A tile inside one tensor is walked
+// in vectors (unaligned ones: tensors may begin anywhere), a tile that holds ends of tensors vector by vector too, every
+// thread looking the tensor up for its own (a vector across tensors goes element by element): a thousand tensors of ten
+// elements cost no more launches than one of ten thousand.
+//
+// Bound by memory: the elements are read twice and written once.  The first sweep reads with the ordinary policy, which
+// leaves what fits in the last-level cache, the second reads and writes with the streaming one: 60 tensors of 124M floats
+// 270 us, 5.5 TB/s of the 1.49 GB (streaming in the first sweep too took a tenth longer; ordinary loads in the second 6 %,
+// and ordinary stores 14 %; the second sweep from the end of the range is as fast).
 //
 // Squares are summed in double: the square of any float is finite there, and the order of the sum does not show in the
 // result's type.  (Squares of halves are exact in float; eight of them are added there first.)
@@ -139,11 +142,11 @@ __global__ void __launch_bounds__(kNormThreads) clipKernel(const T *const *given
     // (a NaN norm compares false, so it leaves the factor at 1 like one that is infinite)
     const C factor = value > maxNorm && value < infinite<double>() ? (C)(maxNorm / value) : (C)1;
     const Long whole = wholeLength(offsets, n, total);
-    int last = n - 1;  // (the tiles of a block descend)
-    for (Long left = (whole + tile - 1) / tile - blockIdx.x; left > 0; left -= gridDim.x) {
-        const Long t = (left - 1) * tile, end = t + tile < whole ? t + tile : whole;
-        const int low = tensorAt(offsets, 0, last, t), high = end <= offsets[low + 1] ? low : tensorAt(offsets, low, last, end - 1);
-        last = low;
+    int low = 0;
+    for (Long t = (Long)blockIdx.x * tile; t < whole; t += (Long)gridDim.x * tile) {
+        const Long end = t + tile < whole ? t + tile : whole;
+        low = tensorAt(offsets, low, n - 1, t);
+        const int high = end <= offsets[low + 1] ? low : tensorAt(offsets, low, n - 1, end - 1);
         if (low == high && end - t == tile && t >= offsets[low]) {
             const Long at = (t - offsets[low]) + threadIdx.x * N;
             const T *from = in[low] + at;
@@ -185,14 +188,15 @@ template <typename T>
 void launchClipByGlobalNorm(hipStream_t s, const T *const *in, T *const *out, const Long *offsets, int n, Long total, double maxNorm,
                             typename Compute<T>::type *norm, void *scratch) {
     double *partial = reinterpret_cast<double *>(scratch);
-    // Four vectors a thread where that leaves every block a tile; one where the tensors are small, for more blocks
-    const Long wide = (Long)kNormThreads * 4 * Pack<T>::N, narrow = (Long)kNormThreads * Pack<T>::N;
+    // Eight vectors a thread where that leaves every block a tile (four: 278 us where eight take 266, sixteen 280); one where
+    // the tensors are small, for more blocks
+    const Long wide = (Long)kNormThreads * 8 * Pack<T>::N, narrow = (Long)kNormThreads * Pack<T>::N;
     const bool isWide = total >= wide * kNormBlocks;
     const int blocks = gridFor(total, isWide ? wide : narrow, kNormBlocks);
     const dim3 grid(blocks), resultGrid(out != nullptr ? blocks : 1), block(kNormThreads);
     if (isWide) {
-        ND4J_LAUNCH((squaresKernel<T, 4>), grid, block, 0, s, in, offsets, n, total, partial);
-        ND4J_LAUNCH((clipKernel<T, 4>), resultGrid, block, 0, s, in, out, offsets, n, total, maxNorm, norm, partial, blocks);
+        ND4J_LAUNCH((squaresKernel<T, 8>), grid, block, 0, s, in, offsets, n, total, partial);
+        ND4J_LAUNCH((clipKernel<T, 8>), resultGrid, block, 0, s, in, out, offsets, n, total, maxNorm, norm, partial, blocks);
     } else {
         ND4J_LAUNCH((squaresKernel<T, 1>), grid, block, 0, s, in, offsets, n, total, partial);
         ND4J_LAUNCH((clipKernel<T, 1>), resultGrid, block, 0, s, in, out, offsets, n, total, maxNorm, norm, partial, blocks);
