@@ -139,7 +139,8 @@ __global__ void __launch_bounds__(kAcrossThreads) layerNormAcrossKernel(const T 
 // Rows of contiguous elements that a team holds in its registers: a team is LANES lanes of a wave or as many whole waves as
 // the row needs with PACKS vectors of 16 bytes a lane, and the elements behind the last whole vector go one a lane.  One
 // read of x, one write of z, the next row on its way while one is worked on; gain and bias stay in registers over the
-// team's rows (HELD).  Loads are unconditional (a vector that is not there re-reads the row's first place, see `at`).
+// team's rows (HELD).  Stores have the streaming policy ([16384, 1024] halves 15.4 us, 16.9 without; loads with it 16.7).
+// Loads are unconditional (a vector that is not there re-reads the row's first place, see `at`).
 template <typename T, int LANES, int PACKS>
 __global__ void __launch_bounds__(1024)
     layerNormRowsKernel(const T *x, RowView xv, const T *gain, const T *bias, T *z, RowView zv, typename Compute<T>::type *mean,
@@ -226,7 +227,7 @@ __global__ void __launch_bounds__(1024)
                     else if (bias != nullptr) h += toCompute(b[j].v[e]);
                     o.v[e] = fromCompute<T>(h);
                 }
-                storePackAnywhere(zr + at[j], o);
+                streamPackAnywhere(zr + at[j], o);
             }
         if (rest < length) {
             zr[rest] = fromCompute<T>(fused((vRest - mu) * s, gRest, bRest));
@@ -427,7 +428,7 @@ __global__ void __launch_bounds__(kBpThreads)
                     const C a = gain != nullptr ? fused(toCompute(d[j].v[e]), toCompute(g[j].v[e]), -meanA) : plus(-meanA, d[j].v[e]);
                     o.v[e] = fromCompute<T>(s * fused(-h, meanAH, a));
                 }
-                storePackAnywhere(dxr + at[j], o);
+                streamPackAnywhere(dxr + at[j], o);
             }
         if (rest < length) dxr[rest] = fromCompute<T>(s * (dRest * gRest - meanA - (vRest - mu) * s * meanAH));
     }
