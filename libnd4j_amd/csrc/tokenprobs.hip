@@ -402,8 +402,8 @@ __global__ void __launch_bounds__(THREADS) tokenProbsRowsKernel(const T *x, RowV
         const int tiles = (end - begin + TILE - 1) / TILE, spanTiles = (tiles + kSpans - 1) / kSpans;
         int span = 0, spanLeft = spanTiles;
         C spanLargest = -infinite<C>();
+        Pack<T> v[VECTORS];
         for (int t = begin; t < end; t += TILE) {
-            Pack<T> v[VECTORS];
             if (t + TILE <= end) {
 #pragma unroll
                 for (int j = 0; j < VECTORS; j++) v[j] = streamPackAnywhere(xr + t + (j * THREADS + (int)threadIdx.x) * N);
@@ -470,18 +470,21 @@ __global__ void __launch_bounds__(THREADS) tokenProbsRowsKernel(const T *x, RowV
 #pragma unroll
                 for (int w = 0; w < WAVES; w++) bound = Largest()(bound, bounds[w]);
             }
-            if (own >= bound) {
-                for (int k = 0; k * spanTiles < tiles; k++)
-                    if (maxima[k][threadIdx.x] >= bound) {
-                        const int place = atomicAdd(&hotCount, 1);
-                        if (place < THREADS) hot[place] = k * THREADS + (int)threadIdx.x;
-                    }
+            const bool held = VECTORS == 1 && tiles == 1;  // every thread's elements are in its registers still
+            if (!held) {
+                if (own >= bound) {
+                    for (int k = 0; k * spanTiles < tiles; k++)
+                        if (maxima[k][threadIdx.x] >= bound) {
+                            const int place = atomicAdd(&hotCount, 1);
+                            if (place < THREADS) hot[place] = k * THREADS + (int)threadIdx.x;
+                        }
+                }
+                __syncthreads();
             }
-            __syncthreads();
             // The vectors of the hot pairs - where there are too many of them, all vectors - are the items.  The elements that
             // reach the bound are gathered, and each counts those that come before it, which is its place.
             const int hots = hotCount, perPair = spanTiles * VECTORS;
-            const bool few = hots <= THREADS;
+            const bool few = !held && hots <= THREADS;
             const Long items = few ? (Long)hots * perPair : ((Long)end - begin + N - 1) / N;
             auto itemAt = [&](Long item, int &c, Pack<T> &v) {
                 c = end;
@@ -500,13 +503,10 @@ __global__ void __launch_bounds__(THREADS) tokenProbsRowsKernel(const T *x, RowV
                     for (int e = 0; e < N; e++) v.v[e] = c + e < end ? xr[c + e] : fromCompute<T>((C)0);
                 }
             };
-            for (Long i = wave * kWaveLanes; i < items; i += THREADS) {
-                int c;
-                Pack<T> v;
-                itemAt(i + lane, c, v);
+            auto gather = [&](int c, const Pack<T> &from) {
 #pragma unroll
                 for (int e = 0; e < N; e++) {
-                    const C value = toCompute(v.v[e]);
+                    const C value = toCompute(from.v[e]);
                     const bool is = c + e < end && value >= bound;
                     const unsigned long long which = __ballot(is);
                     if (which == 0ull) continue;
@@ -518,7 +518,17 @@ __global__ void __launch_bounds__(THREADS) tokenProbsRowsKernel(const T *x, RowV
                         candidateIndexes[place] = c + e;
                     }
                 }
-                if (*(volatile int *)&found > THREADS) break;
+            };
+            if (held) {
+                gather(begin + (int)threadIdx.x * N, v[0]);
+            } else {
+                for (Long i = wave * kWaveLanes; i < items; i += THREADS) {
+                    int c;
+                    Pack<T> item;
+                    itemAt(i + lane, c, item);
+                    gather(c, item);
+                    if (*(volatile int *)&found > THREADS) break;
+                }
             }
             __syncthreads();
             const int count = found;
@@ -533,7 +543,7 @@ __global__ void __launch_bounds__(THREADS) tokenProbsRowsKernel(const T *x, RowV
                     for (int j = 0; j < count; j++) {
                         const C other = candidates[j];
                         const int otherIndex = candidateIndexes[j];
-                        place += other > value || (other == value && otherIndex < index);
+                        place += (int)(other > value) | ((int)(other == value) & (int)(otherIndex < index));
                     }
                 }
                 if (place < out.k) {
@@ -549,12 +559,12 @@ __global__ void __launch_bounds__(THREADS) tokenProbsRowsKernel(const T *x, RowV
                 best.clear(out.k);
                 for (Long i = wave * kWaveLanes; i < items; i += THREADS) {
                     int c;
-                    Pack<T> v;
-                    itemAt(i + lane, c, v);
+                    Pack<T> item;
+                    itemAt(i + lane, c, item);
                     unsigned offers = 0;  // a bit per element
 #pragma unroll
                     for (int e = 0; e < N; e++) {
-                        const C value = toCompute(v.v[e]);
+                        const C value = toCompute(item.v[e]);
                         if (c + e < end && value >= bound && best.beats(value, c + e)) offers |= 1u << e;
                     }
                     while (__ballot(offers != 0u) != 0ull) {
@@ -562,7 +572,7 @@ __global__ void __launch_bounds__(THREADS) tokenProbsRowsKernel(const T *x, RowV
                         C value = -infinite<C>();
 #pragma unroll
                         for (int e = 0; e < N; e++)
-                            if (e == which) value = toCompute(v.v[e]);
+                            if (e == which) value = toCompute(item.v[e]);
                         best.offer(value, c + which, offers != 0u);
                         offers &= offers - 1;
                     }
@@ -596,7 +606,8 @@ __global__ void __launch_bounds__(THREADS) tokenProbsRowsKernel(const T *x, RowV
     }
 }
 
-// A wave takes a row and joins its slices, of which there are at most kMostSlices: one a lane.
+// A wave takes a row and joins its slices, of which there are at most kMostSlices: one a lane.  (Of 200 list entries the best
+// eight by merging take 2.4 us; counting, as above, took 10.)
 constexpr int kMostSlices = kWaveLanes;
 template <typename T, bool TOP>
 __global__ void __launch_bounds__(kWaveLanes) tokenProbsJoinKernel(const T *x, RowView xv, const Long *tokens, TokenProbsOut<T> out,
