@@ -537,9 +537,10 @@ Layout layoutOf(Long n, Long length) {
 
 }  // namespace
 
+// (a launch holds fewer than 2^32 threads)
 bool embeddingBpFits(Long n, Long length) {
     const Long chunk = chunkOf(n), tiles = length / (kWaveLanes * Pack<double>::N) + 1;
-    return n / chunk + 1 < ((Long)1 << 30) / tiles;
+    return n / chunk + 1 < ((Long)1 << 22) / tiles;
 }
 size_t embeddingBpScratch(Long n, Long length) { return layoutOf(n, length).bytes; }
 

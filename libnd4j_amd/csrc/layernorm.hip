@@ -154,7 +154,6 @@ __global__ void __launch_bounds__(1024)
     C *smem = sums + 2 * team * teamWaves;
     int turn = 0;
     const int length = (int)xv.length, vectors = length / N, rest = vectors * N + lane;
-    const C perLength = (C)1 / (C)length;
     int at[PACKS];
     Pack<T> g[PACKS], b[PACKS];
     C gRest = (C)1, bRest = (C)0;
@@ -195,7 +194,7 @@ __global__ void __launch_bounds__(1024)
                 for (int e = 0; e < N; e++) sum[0] = plus(sum[0], v[j].v[e]);
             }
         teamSums<LANES>(sum, smem, teamWaves, turn);
-        const C mu = sum[0] * perLength;
+        const C mu = sum[0] / (C)length;
         C squares[1] = {rest < length ? (vRest - mu) * (vRest - mu) : (C)0};
 #pragma unroll
         for (int j = 0; j < PACKS; j++)
@@ -207,7 +206,7 @@ __global__ void __launch_bounds__(1024)
                 }
             }
         teamSums<LANES>(squares, smem, teamWaves, turn);
-        const C s = (C)1 / sqrtOf(squares[0] * perLength + epsilon), offset = -mu * s;
+        const C s = (C)1 / sqrtOf(squares[0] / (C)length + epsilon), offset = -mu * s;
         if (!live) continue;
         if (lane == 0) {
             if (mean != nullptr) mean[r] = mu;
@@ -229,9 +228,7 @@ __global__ void __launch_bounds__(1024)
                 }
                 streamPackAnywhere(zr + at[j], o);
             }
-        if (rest < length) {
-            zr[rest] = fromCompute<T>(fused((vRest - mu) * s, gRest, bRest));
-        }
+        if (rest < length) zr[rest] = fromCompute<T>(fused((vRest - mu) * s, gRest, bRest));
     }
 }
 
@@ -336,13 +333,12 @@ __global__ void __launch_bounds__(kBpThreads)
     constexpr int N = Pack<T>::N;
     extern __shared__ __align__(16) char dynamicLds[];
     C *columns = reinterpret_cast<C *>(dynamicLds);  // [half of the teams][columns of a row]
-    __shared__ C sums[4 * (kBpThreads / kWaveLanes)];
+    __shared__ C sums[8 * (kBpThreads / kWaveLanes)];  // (the waves behind the last whole team have places too)
     const int size = LANES < kWaveLanes ? LANES : teamWaves * kWaveLanes, teams = kBpThreads / size;
     const int team = threadIdx.x / size, lane = threadIdx.x - team * size;
     C *smem = sums + 4 * team * teamWaves;
     int turn = 0;
     const int length = (int)xv.length, vectors = length / N, rest = vectors * N + lane;
-    const C perLength = (C)1 / (C)length;
     int at[PACKS];
     Pack<T> g[PACKS];
     C gainSum[PACKS][N], biasSum[PACKS][N], gainRest = (C)0, biasRest = (C)0, gRest = (C)1;
@@ -415,7 +411,7 @@ __global__ void __launch_bounds__(kBpThreads)
         }
         if (dx == nullptr) continue;
         teamSums<LANES>(sum, smem, teamWaves, turn);
-        const C meanA = sum[0] * perLength, meanAH = sum[1] * perLength;
+        const C meanA = sum[0] / (C)length, meanAH = sum[1] / (C)length;
         if (!live) continue;
         T *dxr = dx + r * dxv.row;
 #pragma unroll
@@ -636,7 +632,8 @@ int runBpRows(hipStream_t s, const T *x, const RowView &xv, const T *gain, const
     // as many turns as the most blocks would take, the rows spread evenly over them
     const Long most = PACKS == 1 ? 2 * kBpBlocks : kBpBlocks, turns = (xv.rows + most * teams - 1) / (most * teams);
     const int blocks = gridFor(xv.rows, turns * teams, (int)most);
-    const size_t lds = partial != nullptr ? (size_t)(teams / 2) * (Pack<T>::N * PACKS * (LANES < kWaveLanes ? LANES : waves * kWaveLanes) + Pack<T>::N) * sizeof(C) : 0;
+    const int size = LANES < kWaveLanes ? LANES : waves * kWaveLanes;
+    const size_t lds = partial != nullptr ? (size_t)(teams / 2) * (Pack<T>::N * PACKS * size + Pack<T>::N) * sizeof(C) : 0;
     ND4J_LAUNCH((layerNormBpRowsKernel<T, LANES, PACKS>), dim3(blocks), dim3(kBpThreads), lds, s, x, xv, gain, mean, invStd, dz, dzv, dx, dxv,
                 partial, waves);
     return blocks;
