@@ -514,11 +514,16 @@ template <typename T> static void transformStrided(int op, T *x, Long xs, T *z, 
         for (Long i = start; i < end; i++) transformOp<T>(op, x[i * xs], extra, z[i * zs]);
     }
 }
+// What sums over long ranges are held in: floats in double, the other types in their own.
+template <typename T> struct LongSum { typedef T type; };
+template <> struct LongSum<float> { typedef double type; };
 // Whole-array special transforms (include/ops/special_ops.h): SoftMax 38 (1483-1568), SoftMaxDerivative 39
 // (1806-1937), LogSoftMax 40 (1635-1726) over each row of a matrix or over a vector; IsMax 41 (1951-2260): one-hot of
 // the first maximum of the whole array, or of every TAD along the dimensions listed in extraParams
 // ([0] = count, [1..] = dimensions).  Restated as what the routines compute when called in place (x == z), which is
-// how the reference's vector branches of 39 / 40 and the matrix branch of 39 read their input.
+// how the reference's vector branches of 39 / 40 and the matrix branch of 39 read their input.  A row of floats is summed
+// in double (LongSum): the compiled loops add many partial sums of a row, which one float that takes 100000 values in turn
+// is further from than the bar of the comparisons (1.1e-4 against 1e-5).
 template <typename T> static void specialTransform(int op, T *x, Long *xi, T *z, Long *zi, T *extra) {
     const int rank = siRank(xi);
     const Long n = siNumel(xi);
@@ -543,8 +548,9 @@ template <typename T> static void specialTransform(int op, T *x, Long *xi, T *z,
             T *xr = x + r * xRow, *zr = z + r * zRow;
             T mx = xr[0];
             for (Long c = 1; c < len; c++) mx = m_max(mx, xr[c * xEl]);
-            T sum = (T)0.0f;
-            for (Long c = 0; c < len; c++) { T e = m_exp(xr[c * xEl] - mx); zr[c * zEl] = e; sum += e; }
+            typename LongSum<T>::type total = (T)0.0f;
+            for (Long c = 0; c < len; c++) { T e = m_exp(xr[c * xEl] - mx); zr[c * zEl] = e; total += e; }
+            const T sum = (T)total;
             for (Long c = 0; c < len; c++) {
                 T v = zr[c * zEl] / sum;
                 if (op == 39) v = v * ((T)1.0f - v);
@@ -887,25 +893,38 @@ template <typename T> static inline T r3Post(int op, const R3<T> &a, Long n) {
     }
 }
 // whole arrays (reduce3.h:838-916): memory-linear pairing when both arrays have an element-wise stride and the
-// same order, C-order logical pairing otherwise; one sequential pass
+// same order, C-order logical pairing otherwise; one sequential pass, its sums in LongSum's type with each term rounded to T
 template <typename T> static T reduce3Scalar(int op, T *x, Long *xi, T *extra, T *y, Long *yi) {
     if (op < 0 || op > 7) { printf("[ERROR] Unknown opNum=%d (oracle reduce3)\n", op); return (T)0.0f; }
     const T eps = extra != nullptr ? extra[0] : (T)0.0f;
     const Long n = siNumel(xi);
     const Long xe = siEws(xi), ye = siEws(yi);
-    R3<T> a;
-    a.r = a.e0 = a.e1 = (T)0.0f;
+    typedef typename LongSum<T>::type S;
+    R3<S> sums;
+    sums.r = sums.e0 = sums.e1 = (T)0.0f;
+    auto add = [&](T d1, T d2) {
+        R3<T> one;
+        one.r = one.e0 = one.e1 = (T)0.0f;
+        r3Op<T>(op, one, d1, d2, eps);
+        sums.r = sums.r + one.r;
+        sums.e0 = sums.e0 + one.e0;
+        sums.e1 = sums.e1 + one.e1;
+    };
     if (siOrder(xi) == siOrder(yi) && xe >= 1 && ye >= 1) {
-        for (Long i = 0; i < n; i++) r3Op<T>(op, a, x[i * xe], y[i * ye], eps);
+        for (Long i = 0; i < n; i++) add(x[i * xe], y[i * ye]);
     } else {
         Long cx[kMaxRank], cy[kMaxRank];
         for (Long i = 0; i < n; i++) {
             ind2subC(siRank(xi), siShape(xi), (int)i, cx);
             ind2subC(siRank(yi), siShape(yi), (int)i, cy);
-            r3Op<T>(op, a, x[getOffset(0, siShape(xi), siStride(xi), cx, siRank(xi))],
-                    y[getOffset(0, siShape(yi), siStride(yi), cy, siRank(yi))], eps);
+            add(x[getOffset(0, siShape(xi), siStride(xi), cx, siRank(xi))],
+                y[getOffset(0, siShape(yi), siStride(yi), cy, siRank(yi))]);
         }
     }
+    R3<T> a;
+    a.r = (T)sums.r;
+    a.e0 = (T)sums.e0;
+    a.e1 = (T)sums.e1;
     return r3Post<T>(op, a, n);
 }
 // one run of `n` pairs: element f of each operand is found from its linear index in the given order
