@@ -17,10 +17,15 @@ constexpr int kRowThreads = 256;
 
 // Steps in a form that takes a half operand as it is: one instruction converts it, multiplies and adds, where a conversion of
 // its own and the two operations would be three.
-// acc + v
+// acc + v (times a 1 that the compiler does not see: of the constant it makes a conversion and an addition)
 template <typename T> __device__ __forceinline__ typename Compute<T>::type plus(typename Compute<T>::type acc, T v) {
-    if constexpr (sizeof(T) == 2) return fused(toCompute(v), 1.0f, acc);
-    else return acc + toCompute(v);
+    if constexpr (sizeof(T) == 2) {
+        float one = 1.0f;
+        asm("" : "+s"(one));
+        return fused(toCompute(v), one, acc);
+    } else {
+        return acc + toCompute(v);
+    }
 }
 // (v - mu) s; offset = -mu s.  For halves as v s - mu s: it rounds mu s, 2^-24 of it, where the result keeps 2^-11 of itself.
 template <typename T>
@@ -28,6 +33,12 @@ __device__ __forceinline__ typename Compute<T>::type normal(T v, typename Comput
                                                             typename Compute<T>::type offset) {
     if constexpr (sizeof(T) == 2) return fused(toCompute(v), s, offset);
     else return (toCompute(v) - mu) * s;
+}
+// what is known to be no NaN
+__device__ __forceinline__ float16 fromNumber(float v) {
+    float16 h;
+    h.x = __builtin_bit_cast(unsigned short, (_Float16)v);
+    return h;
 }
 // a b
 template <typename T> __device__ __forceinline__ typename Compute<T>::type times(T a, T b) {
@@ -345,9 +356,12 @@ __global__ void __launch_bounds__(kBpThreads)
 #pragma unroll
     for (int j = 0; j < PACKS; j++) {
         at[j] = lane + j * size < vectors ? (lane + j * size) * N : 0;
-        if (vectors > 0 && gain != nullptr) g[j] = loadPackAnywhere(gain + at[j]);
 #pragma unroll
-        for (int e = 0; e < N; e++) gainSum[j][e] = biasSum[j][e] = (C)0;
+        for (int e = 0; e < N; e++) {
+            gainSum[j][e] = biasSum[j][e] = (C)0;
+            g[j].v[e] = fromCompute<T>((C)1);  // no gain: dz times 1, which is dz
+        }
+        if (vectors > 0 && gain != nullptr) g[j] = loadPackAnywhere(gain + at[j]);
     }
     if (rest < length && gain != nullptr) gRest = toCompute(gain[rest]);
     // the next row is on its way while this one is worked on
@@ -394,7 +408,7 @@ __global__ void __launch_bounds__(kBpThreads)
 #pragma unroll
                     for (int e = 0; e < N; e++) {
                         const C dd = toCompute(d[j].v[e]), h = normal(v[j].v[e], mu, s, offset);
-                        const C a = gain != nullptr ? times(d[j].v[e], g[j].v[e]) : dd;
+                        const C a = times(d[j].v[e], g[j].v[e]);
                         sum[0] += a;
                         sum[1] = fused(a, h, sum[1]);
                         gainSum[j][e] = fused(dd, h, gainSum[j][e]);
@@ -414,18 +428,29 @@ __global__ void __launch_bounds__(kBpThreads)
         const C meanA = sum[0] / (C)length, meanAH = sum[1] / (C)length;
         if (!live) continue;
         T *dxr = dx + r * dxv.row;
+        auto store = [&](auto convert) {
 #pragma unroll
-        for (int j = 0; j < PACKS; j++)
-            if (lane + j * size < vectors) {
-                Pack<T> o;
+            for (int j = 0; j < PACKS; j++)
+                if (lane + j * size < vectors) {
+                    Pack<T> o;
 #pragma unroll
-                for (int e = 0; e < N; e++) {
-                    const C h = normal(v[j].v[e], mu, s, offset);
-                    const C a = gain != nullptr ? fused(toCompute(d[j].v[e]), toCompute(g[j].v[e]), -meanA) : plus(-meanA, d[j].v[e]);
-                    o.v[e] = fromCompute<T>(s * fused(-h, meanAH, a));
+                    for (int e = 0; e < N; e++) {
+                        const C h = normal(v[j].v[e], mu, s, offset), a = fused(toCompute(d[j].v[e]), toCompute(g[j].v[e]), -meanA);
+                        o.v[e] = convert(s * fused(-h, meanAH, a));
+                    }
+                    streamPackAnywhere(dxr + at[j], o);
                 }
-                streamPackAnywhere(dxr + at[j], o);
-            }
+        };
+        if constexpr (sizeof(T) == 2) {
+            // Finite sums have finite terms, a and h then are finite too, and what an infinite product adds up to is no NaN: so
+            // is no element of dx, unless s is 0 (a NaN's own bits take a compare and a select an element).
+            if (::fabsf(sum[0]) < infinite<C>() && ::fabsf(sum[1]) < infinite<C>() && s != (C)0)
+                store([](C o) { return fromNumber(o); });
+            else
+                store([](C o) { return fromCompute<T>(o); });
+        } else {
+            store([](C o) { return fromCompute<T>(o); });
+        }
         if (rest < length) dxr[rest] = fromCompute<T>(s * (dRest * gRest - meanA - (vRest - mu) * s * meanAH));
     }
     if (partial == nullptr) return;
