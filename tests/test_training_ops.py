@@ -221,6 +221,36 @@ def test_layer_norm_bp_parts_and_in_place(dev, S, rows, n):
         close(got[k], want[k], want[3 + k])
 
 
+@pytest.mark.parametrize("S", SUFFIXES)
+@pytest.mark.parametrize("n", (40, 300, 5003))
+def test_layer_norm_bp_of_nan_infinity_and_overflow(dev, S, n):
+    """a row's NaN and infinities stay in the row, and come out as the formula has them; so does what passes the type's range"""
+    x, gain, mean, inv, dz = bp_inputs(S, 9, n, 3)
+    dz[1, 5] = np.nan
+    dz[2, n - 1] = np.inf
+    x[3, 7] = np.nan
+    inv[4] = 0
+    inv[5] = np.nan
+    inv[6] = 1e6  # beyond a half's range in every element of dx, and far inside a float's
+    x[7, 0] = -np.inf
+    for g in (gain, None):
+        got = run_layer_norm_bp(dev, S, x, g, mean, inv, dz, wants=("dx",))[0]
+        with np.errstate(all="ignore"):
+            want, _, _, tol, _, _ = layer_norm_bp_oracle(x, g, mean, inv, dz, S)
+            rounded = want.astype(STORAGE[S])
+        assert np.array_equal(np.isnan(got), np.isnan(rounded))
+        if S == "Half":
+            assert (got[np.isnan(got)].view(np.uint16) == 0x7fff).all()
+        far = np.isinf(rounded) & np.isinf(got)
+        assert np.array_equal(got[far], rounded[far])
+        near = ~far & ~np.isnan(rounded)
+        near[6] &= S != "Half"  # (the row that the half rounds to infinity but near zeros of dx)
+        assert not np.isinf(got[near]).any()
+        close(got[near], want[near], tol[near])
+        assert np.isnan(got[1]).all() and not got[4].any() and np.isfinite(got[[0, 8]]).all()
+        assert np.isinf(got[6]).any() == (S == "Half")
+
+
 def test_layer_norm_bp_without_rows(dev):
     x = np.zeros((0, 33), np.float32)
     got = run_layer_norm_bp(dev, "Float", x, None, np.zeros(0), np.zeros(0), x)
