@@ -261,8 +261,9 @@ void nd4j_amd_execReduceFloatNoAlloc(Nd4jPointer *extraPointers, int opNum, floa
  * leading dimensions merge into rows a common distance apart (a matrix of either order, a padded or sliced matrix,
  * a dense array of any rank; a rank-1 array is one row).  Host copies travel in extraPointers as usual - [0] for the
  * first shapeInfo argument, [8] for the last, [7] for the one between - or the argument itself is a host pointer;
- * otherwise the shapeInfo is read back from the device, which synchronises the stream.  Gains, biases and per-row
- * values are dense vectors.  Per-row statistics, log probabilities and norms have the compute type: float for Half.
+ * otherwise the shapeInfo is read back from the device, which synchronises the stream (refused while it is captured).
+ * Views that are read may repeat elements (strides of 0); in results no two elements share a place.  Gains, biases and
+ * per-row values are dense vectors.  Per-row statistics, log probabilities and norms have the compute type: float for Half.
  *
  * Execution.  Every call is enqueued on the stream of extraPointers[1], returns without waiting, allocates nothing
  * but scratch, gives the same bits for the same inputs, and may be captured into a graph.  Calls with a `scratch`

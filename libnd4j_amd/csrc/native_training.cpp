@@ -3,6 +3,7 @@
 // reached through the C ABI (include/nd4j_native_c.h), which documents them.  Everything a kernel takes for granted is
 // checked here, before anything is enqueued; what cannot be checked on the host (token values, offsets) the kernels bound.
 #include <cmath>
+#include <numeric>
 #include <stdexcept>
 #include <string>
 
@@ -21,6 +22,9 @@ const Long kMostLength = ((Long)1 << 31) - ((Long)1 << 20);  // columns fit an i
 
 // The rows of a view: its last dimension, at every position of the others, which have to lie a common distance apart.
 RowView rowsOf(const char *op, const char *name, Nd4jPointer *extra, int slot, const Long *arg, std::vector<Long> &storage, hipStream_t s) {
+    // (a read-back synchronises the stream, which would end a capture)
+    if (slotOf(extra, slot) == nullptr && arg != nullptr && streamIsCapturing(s) && isDeviceMemory(arg))
+        refuse(op, std::string("the stream is being captured, which needs a host copy of the shapeInfo of ") + name);
     const Long *info = hostShapeInfo(extra, slot, arg, storage, s);
     if (info == nullptr) refuse(op, std::string("no shapeInfo of ") + name);
     const int rank = siRank(info);
@@ -48,6 +52,13 @@ RowView rowsOf(const char *op, const char *name, Nd4jPointer *extra, int slot, c
     if (v.length < 1) refuse(op, std::string(name) + " has rows without elements");
     if (v.length > kMostLength) refuse(op, std::string(name) + " has rows of more than 2^31 - 2^20 elements");
     return v;
+}
+
+// A result's elements have places of their own: d rows further and e elements on is the same place where d row = e el.
+void apart(const char *op, const char *name, const RowView &v) {
+    const Long row = v.row < 0 ? -v.row : v.row, el = v.el < 0 ? -v.el : v.el, common = std::gcd(row, el);
+    const bool meet = common == 0 ? v.rows > 1 || v.length > 1 : el / common < v.rows && row / common < v.length;
+    if (v.rows > 0 && meet) refuse(op, std::string("elements of ") + name + " share places");
 }
 
 template <typename P> void need(const char *op, const char *name, const P *p, size_t alignment) {
@@ -89,6 +100,7 @@ void layerNorm(Nd4jPointer *extra, T *x, Long *xInfo, T *gain, T *bias, T *z, Lo
     std::vector<Long> sx, sz;
     const RowView xv = rowsOf(op, "x", extra, X_HOST_X_SHAPE, xInfo, sx, s), zv = rowsOf(op, "z", extra, X_HOST_Z_SHAPE, zInfo, sz, s);
     sameShape(op, "x", xv, "z", zv);
+    apart(op, "z", zv);
     if (!(epsilon >= 0.0)) refuse(op, "epsilon is negative or not a number");
     if (xv.rows == 0) return;
     must(op, "x", x);
@@ -113,6 +125,7 @@ void layerNormBp(Nd4jPointer *extra, T *x, Long *xInfo, T *gain, typename Comput
     if (dx != nullptr) {
         dxv = rowsOf(op, "dx", extra, X_HOST_Z_SHAPE, dxInfo, sz, s);
         sameShape(op, "x", xv, "dx", dxv);
+        apart(op, "dx", dxv);
     }
     mayBe(op, "dx", dx);
     mayBe(op, "dGain", dGain);
@@ -143,6 +156,7 @@ void embedding(Nd4jPointer *extra, T *table, Long *tableInfo, Long *tokens, Long
     if (n == 0) return;
     const RowView zv = rowsOf(op, "z", extra, X_HOST_Z_SHAPE, zInfo, sz, s);
     if (zv.rows != n || zv.length != tv.length) refuse(op, "z is not a row of the table's length for every token");
+    apart(op, "z", zv);
     if (n > ((Long)1 << 56) / tv.length) refuse(op, "too many elements");
     must(op, "the table", table);
     must(op, "tokens", tokens);
@@ -164,6 +178,7 @@ void embeddingBp(Nd4jPointer *extra, T *dz, Long *dzInfo, Long *tokens, Long n, 
     if (n > 0) dzv = rowsOf(op, "dz", extra, X_HOST_X_SHAPE, dzInfo, sx, s);
     if (dzv.rows != n || dzv.length != tv.length) refuse(op, "dz is not a row of the table's length for every token");
     if (tv.rows == 0 || (n == 0 && accumulate != 0)) return;
+    apart(op, "dTable", tv);
     // (tokens are sorted as 32-bit keys with 32-bit positions)
     if (n > kMostLength || tv.rows > kMostLength) refuse(op, "more than 2^31 - 2^20 tokens or rows of the table are not supported");
     if (!embeddingBpFits(n, tv.length)) refuse(op, "too many elements");
@@ -216,6 +231,7 @@ void tokenLogProbsBp(Nd4jPointer *extra, T *x, Long *xInfo, Long *tokens, typena
     std::vector<Long> sx, sz;
     const RowView xv = rowsOf(op, "x", extra, X_HOST_X_SHAPE, xInfo, sx, s), dxv = rowsOf(op, "dx", extra, X_HOST_Z_SHAPE, dxInfo, sz, s);
     sameShape(op, "x", xv, "dx", dxv);
+    apart(op, "dx", dxv);
     if (dLogProbs == nullptr && dEntropy == nullptr) refuse(op, "neither the log probabilities' gradient nor the entropies' is given");
     if (xv.rows == 0) return;
     must(op, "x", x);

@@ -228,6 +228,36 @@ def test_calls_in_captured_graphs(dev):
             hip.hipGraphDestroy(g)
 
 
+def test_a_captured_call_needs_host_copies(dev):
+    """without one the shapeInfo would be read back, which ends a capture: refused, and the capture goes on"""
+    hip = ctypes.CDLL("libamdhip64.so")
+    ops, stream, graph = dev.ops, ctypes.c_void_p(dev.stream), ctypes.c_void_p()
+    rs = np.random.RandomState(2)
+    x = rs.randn(6, 40).astype(np.float32)
+    X, Z = View(dev, 6, 40, "dense", np.float32, x), View(dev, 6, 40, "dense", np.float32)
+    full, bare = (ctypes.c_void_p * 20)(), (ctypes.c_void_p * 20)()
+    full[0], full[1], full[8] = X.info.ctypes.data, dev.stream, Z.info.ctypes.data
+    bare[1] = dev.stream
+    infos = dev.upload(X.info), dev.upload(Z.info)
+    args = (X.ptr, infos[0].ptr, None, None, Z.ptr, infos[1].ptr, None, None, 1e-5)
+    dev.sync()
+    assert hip.hipStreamBeginCapture(stream, 1) == 0  # 1: thread-local capture mode
+    try:
+        with pytest.raises(Nd4jError, match="host copy"):
+            ops.amd_execLayerNormFloat(bare, *args)
+        ops.amd_execLayerNormFloat(full, *args)
+    finally:
+        status = hip.hipStreamEndCapture(stream, ctypes.byref(graph))
+    assert status == 0 and graph.value
+    hip.hipGraphDestroy(graph)
+    ops.amd_execLayerNormFloat(bare, *args)  # outside of a capture it is read back
+    dev.sync()
+    want = (x - x.mean(1, keepdims=True)) / np.sqrt(x.var(1, keepdims=True) + 1e-5)
+    assert np.abs(Z.get() - want).max() < 1e-5  # (values below 4, a dozen roundings of 2^-24 of them)
+    for v in (X, Z) + infos:
+        v.free()
+
+
 def test_calls_from_threads_on_streams_of_their_own(dev):
     """four threads, a stream and the library's scratch each: the results of one thread alone; then the streams are released"""
     ops = dev.ops

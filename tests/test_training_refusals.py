@@ -113,6 +113,30 @@ def test_clip_by_global_norm(ops, S, why, args):
                                                      g("w", None), g("wb", 0))
 
 
+@pytest.mark.parametrize("S", SUFFIXES)
+@pytest.mark.parametrize("strides", [[0, 1], [8, 0], [0, 0], [1, 1], [7, 1], [2, 4], [-2, 6], [1, 3]])
+def test_results_whose_elements_share_places(ops, S, strides):
+    shared, whole = info(4, 8, strides=strides), info(4, 8)
+    with pytest.raises(Nd4jError, match="share places"):
+        getattr(ops, "amd_execLayerNorm" + S)(extra(x=whole, z=shared), P, None, P, P, P, None, P, P, 1e-5)
+    with pytest.raises(Nd4jError, match="share places"):
+        getattr(ops, "amd_execLayerNormBp" + S)(extra(whole, whole, shared), P, None, P, P, P, P, None, P, None, P, P, None, 0)
+    with pytest.raises(Nd4jError, match="share places"):
+        getattr(ops, "amd_execEmbedding" + S)(extra(x=whole, z=shared), P, None, P, 4, P, None, 1.0)
+    with pytest.raises(Nd4jError, match="share places"):
+        getattr(ops, "amd_execEmbeddingBp" + S)(extra(x=whole, z=shared), P, None, P, 4, P, None, 1.0, 0, None, 0)
+    with pytest.raises(Nd4jError, match="share places"):
+        getattr(ops, "amd_execTokenLogProbsBp" + S)(extra(x=whole, z=shared), P, None, P, P, P, P, P, P, None)
+
+
+@pytest.mark.parametrize("S", SUFFIXES)
+@pytest.mark.parametrize("strides", [[8, 1], [1, 4], [9, 1], [-8, 1], [8, -1], [1, 5], [16, 2], [3, 4]])
+def test_results_whose_elements_do_not(ops, S, strides):
+    """refused for another reason, which is looked at later"""
+    with pytest.raises(Nd4jError, match="x is null"):
+        getattr(ops, "amd_execLayerNorm" + S)(extra(x=info(4, 8), z=info(4, 8, strides=strides)), None, None, P, P, P, None, P, P, 1e-5)
+
+
 def test_scratch_sizes(ops):
     assert ops.amd_scratchLayerNormBp(0, 1) > 0
     assert ops.amd_scratchLayerNormBp(16384, 1024) < 1 << 26
