@@ -9,7 +9,9 @@
 //
 // The sort's launches are a few small blocks that wait for memory; unless the gradient is added onto what the table holds,
 // the rest of the chip clears the table meanwhile, the rows that get sums later among them (they are few where clearing
-// takes long: clearing only the others, behind the sort, made [16384 of 32000, 768] floats 65 us).
+// takes long: clearing only the others, behind the sort, made [16384 of 32000, 768] floats 65 us).  Those take 40 us: the sort's
+// four launches 23, of which clearing 98 MB needs 15, the sums 14, the join 4, all with a launch's latency in them.  Up to 4096
+// tokens it is three launches, 14 us for 257 tokens.
 #include "launch.h"
 #include "training.cuh"
 
@@ -36,7 +38,7 @@ __global__ void __launch_bounds__(kThreads) embeddingAnyKernel(const T *table, R
 
 // Rows of contiguous elements: a thread takes vectors of 16 bytes of the rows as they lie behind each other, kInFlight of
 // them at a time, since each waits for its token first and for the table then.  Bound by memory: 32768 rows of 1024 halves
-// 16.8 us, 8 TB/s of what it reads and writes, of which the frequent rows come from the caches (eight at a time: 19.1 us).
+// 16.3 us, 8.2 TB/s of what it reads and writes, of which the frequent rows come from the caches (eight at a time: 19.1 us).
 constexpr int kInFlight = 2;
 template <typename T>
 __global__ void __launch_bounds__(kThreads) embeddingRowsKernel(const T *table, RowView tv, const Long *tokens, T *z, RowView zv,

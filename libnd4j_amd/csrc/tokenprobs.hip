@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(kAcrossThreads) tokenProbsAcrossKernel(const T
 // their places by counting.  Where rows are few they are cut into slices, whose sums and lists a second launch joins.
 //
 // (Keeping the best elements during the sweep, as the first form did, took 118 us over [4096, 32000] floats at k = 5, where
-// the sweep alone takes 81.)
+// the sweep alone takes 81.  This form takes 86, 6.1 TB/s.  One row of 50257 halves takes 11 us, which is two launches.)
 
 // exp for the sums: the relative error grows with |d| (a rounding of d log2 e), on terms whose share is exp(d)
 __device__ __forceinline__ float expOf(float d) { return __builtin_amdgcn_exp2f(d * 1.44269502162933349609375f); }
