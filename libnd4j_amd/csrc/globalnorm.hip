@@ -9,7 +9,7 @@
 //
 // Bound by memory: the elements are read twice and written once.  The first sweep reads with the ordinary policy, which
 // leaves what fits in the last-level cache, the second reads and writes with the streaming one: 60 tensors of 124M floats
-// 270 us, 5.5 TB/s of the 1.49 GB (streaming in the first sweep too took a tenth longer; ordinary loads in the second 6 %,
+// 245 us, 6.1 TB/s of the 1.49 GB (streaming in the first sweep too took a tenth longer; ordinary loads in the second 6 %,
 // and ordinary stores 14 %; the second sweep from the end of the range is as fast).  20 tensors of 100003 halves in all
 // take 12.5 us, which is two launches.
 //
@@ -24,7 +24,7 @@ namespace {
 using namespace tr;
 
 constexpr int kNormThreads = 512;
-constexpr int kNormBlocks = 1024;  // four a compute unit: all waves that it holds
+constexpr int kNormBlocks = 512;  // of the first sweep, whose sums every block of the second adds up (1024: 250 us where these take 245)
 
 // The elements of the range: what the offsets say, and no more than the host was told.
 __device__ __forceinline__ Long wholeLength(const Long *offsets, int n, Long total) {
@@ -189,18 +189,20 @@ template <typename T>
 void launchClipByGlobalNorm(hipStream_t s, const T *const *in, T *const *out, const Long *offsets, int n, Long total, double maxNorm,
                             typename Compute<T>::type *norm, void *scratch) {
     double *partial = reinterpret_cast<double *>(scratch);
-    // Eight vectors a thread where that leaves every block a tile (four: 278 us where eight take 266, sixteen 280); one where
-    // the tensors are small, for more blocks
-    const Long wide = (Long)kNormThreads * 8 * Pack<T>::N, narrow = (Long)kNormThreads * Pack<T>::N;
-    const bool isWide = total >= wide * kNormBlocks;
-    const int blocks = gridFor(total, isWide ? wide : narrow, kNormBlocks);
-    const dim3 grid(blocks), resultGrid(out != nullptr ? blocks : 1), block(kNormThreads);
-    if (isWide) {
-        ND4J_LAUNCH((squaresKernel<T, 8>), grid, block, 0, s, in, offsets, n, total, partial);
-        ND4J_LAUNCH((clipKernel<T, 8>), resultGrid, block, 0, s, in, out, offsets, n, total, maxNorm, norm, partial, blocks);
+    // From 25 MB on the first sweep takes tiles of eight vectors a thread and the second tiles of four, a block each (as many blocks
+    // as the first, tile after tile: 270 us where these take 245; eight vectors 250, two 294, since every block adds up the sums
+    // first).  Smaller ones go in tiles of one vector, for more blocks: 6M floats 26.3 us, 27.0 in large tiles, but 8M 35.9 and 30.5.
+    const Long wide = (Long)kNormThreads * 8 * Pack<T>::N, half = wide / 2, narrow = (Long)kNormThreads * Pack<T>::N;
+    const dim3 block(kNormThreads);
+    if (total >= wide * (kNormBlocks * 3 / 4)) {
+        const int parts = gridFor(total, wide, kNormBlocks);
+        ND4J_LAUNCH((squaresKernel<T, 8>), dim3(parts), block, 0, s, in, offsets, n, total, partial);
+        ND4J_LAUNCH((clipKernel<T, 4>), dim3(out != nullptr ? gridFor(total, half, 1 << 20) : 1), block, 0, s, in, out, offsets, n, total, maxNorm,
+                    norm, partial, parts);
     } else {
-        ND4J_LAUNCH((squaresKernel<T, 1>), grid, block, 0, s, in, offsets, n, total, partial);
-        ND4J_LAUNCH((clipKernel<T, 1>), resultGrid, block, 0, s, in, out, offsets, n, total, maxNorm, norm, partial, blocks);
+        const int parts = gridFor(total, narrow, kNormBlocks);
+        ND4J_LAUNCH((squaresKernel<T, 1>), dim3(parts), block, 0, s, in, offsets, n, total, partial);
+        ND4J_LAUNCH((clipKernel<T, 1>), dim3(out != nullptr ? parts : 1), block, 0, s, in, out, offsets, n, total, maxNorm, norm, partial, parts);
     }
 }
 

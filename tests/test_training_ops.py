@@ -738,6 +738,23 @@ def test_clip_of_many_tensors(dev, S):
 
 
 @pytest.mark.parametrize("S", SUFFIXES)
+@pytest.mark.parametrize("apart", (True, False))
+def test_clip_of_large_tensors(dev, S, apart):
+    """beyond 25 MB, where the tiles are larger: ends of tensors inside them, and a last tile that is not whole"""
+    rs = np.random.RandomState(4)
+    n = 30000000 // STORAGE[S]().itemsize
+    lengths = [n // 2 + 1, 7, 0, 16384, n // 4 + 3, 3, n // 4 + 101]
+    whole = (rs.randint(-64, 65, sum(lengths)) / 64).astype(STORAGE[S])
+    tensors = np.split(whole, np.cumsum(lengths)[:-1])
+    got, value = run_clip(dev, S, tensors, 1.0, apart)
+    check_clip(got, value, tensors, 1.0, S)
+    same, _ = run_clip(dev, S, tensors, 1.0, apart, inplace=True)
+    assert all(np.array_equal(a, b) for a, b in zip(same, got))
+    got, value = run_clip(dev, S, tensors, 0.0, apart, results=False)
+    check_clip(tensors, value, tensors, 1e30, S)
+
+
+@pytest.mark.parametrize("S", SUFFIXES)
 def test_clip_of_extremes(dev, S):
     """no tensors; all zero; squares beyond the type's range; NaN and infinities, which change nothing but the norm"""
     got, value = run_clip(dev, S, [np.zeros(0)], 1.0)
