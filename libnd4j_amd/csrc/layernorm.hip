@@ -150,8 +150,8 @@ __global__ void __launch_bounds__(kAcrossThreads) layerNormAcrossKernel(const T 
 // Rows of contiguous elements that a team holds in its registers: a team is LANES lanes of a wave or as many whole waves as
 // the row needs with PACKS vectors of 16 bytes a lane, and the elements behind the last whole vector go one a lane.  One
 // read of x, one write of z, the next row on its way while one is worked on; gain and bias stay in registers over the
-// team's rows (HELD).  [16384, 1024] halves 14.7 us, 4.6 TB/s; what it has beyond the copy's 10.5 are the two sums of a row, one
-// after the other.  Stores have the streaming policy (measured side by side 15.4 us, 16.9 without; loads with it 16.7).
+// team's rows (HELD).  [16384, 1024] halves 13.3 us, 5.1 TB/s; what it has beyond the copy's 10.5 are the two sums of a row, one
+// after the other.  Stores have the streaming policy (a tenth longer without it, and with it for the loads too).
 // Loads are unconditional (a vector that is not there re-reads the row's first place, see `at`).
 template <typename T, int LANES, int PACKS>
 __global__ void __launch_bounds__(1024)
@@ -604,7 +604,16 @@ int teamWaves(Long vectors, int packs) {
     const Long waves = (vectors + (Long)kWaveLanes * packs - 1) / ((Long)kWaveLanes * packs);
     return (int)(waves < 1 ? 1 : waves);
 }
-constexpr int kFullThreads = 256 * 2048;  // that the chip holds at once
+// The blocks of the forward kernel.  Halves, and teams of more than eight waves: as many as the 256 compute units hold at once
+// (32 waves a unit at one vector a lane, by registers 20 at two and 16 at four), each going on from row to row: [16384, 1024]
+// halves 14.4 us, 15.4 with 32 waves a unit throughout and 16.4 with a block for every row; [4096, 8192] floats 52 and 68.  Smaller
+// teams of floats and doubles: three times the 32, which spreads what is left at the end: [16384, 1024] floats 21.0 us, 23.5
+// with 32 and 20.8 with a block for every row, [65536, 256] 21.7, 23.4 and 25.5.
+int rowBlocks(int packs, int size, int blockWaves, int teamWaves) {
+    if (size > 2 && teamWaves <= 8) return 256 * 96 / blockWaves;
+    const int held = (packs == 1 ? 32 : (packs == 2 ? 20 : 16)) / blockWaves;
+    return 256 * (held < 1 ? 1 : held);
+}
 
 unsigned gridOf(Long blocks) { return (unsigned)(blocks < 1 ? 1 : (blocks > (1 << 20) ? (1 << 20) : blocks)); }
 
@@ -624,7 +633,7 @@ void runRows(hipStream_t s, const T *x, const RowView &xv, const T *gain, const 
     typedef typename Compute<T>::type C;
     const int waves = teamWaves(xv.length / Pack<T>::N, PACKS), teams = LANES < kWaveLanes ? 256 / LANES : (waves >= 4 ? 1 : 4 / waves);
     const int threads = LANES < kWaveLanes ? 256 : teams * waves * kWaveLanes;
-    const unsigned blocks = (unsigned)gridFor(xv.rows, teams, kFullThreads / threads);
+    const unsigned blocks = (unsigned)gridFor(xv.rows, teams, rowBlocks(PACKS, (int)sizeof(T), threads / kWaveLanes, waves));
     ND4J_LAUNCH((layerNormRowsKernel<T, LANES, PACKS>), dim3(blocks), dim3(threads), 0, s, x, xv, gain, bias, z, zv, mean, invStd, (C)epsilon,
                 waves);
 }
