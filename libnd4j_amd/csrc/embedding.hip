@@ -40,6 +40,7 @@ __global__ void __launch_bounds__(kThreads) embeddingAnyKernel(const T *table, R
 // them at a time, since each waits for its token first and for the table then.  Bound by memory: 32768 rows of 1024 halves
 // 16.3 us, 8.2 TB/s of what it reads and writes, of which the frequent rows come from the caches (eight at a time: 19.1 us).
 constexpr int kInFlight = 2;
+constexpr int kRowBlocks = 1 << 22;  // (as many as there are turns: with at most 8192 blocks 65536 rows of 4096 floats took 319 us, now 284)
 template <typename T>
 __global__ void __launch_bounds__(kThreads) embeddingRowsKernel(const T *table, RowView tv, const Long *tokens, T *z, RowView zv,
                                                                 typename Compute<T>::type scale, FastDiv perRow, unsigned units) {
@@ -555,7 +556,7 @@ void launchEmbedding(hipStream_t s, const T *table, const RowView &tv, const Lon
         for (Long r = 0; r < zv.rows; r += most) {
             const Long rows = zv.rows - r < most ? zv.rows - r : most;
             const unsigned units = (unsigned)(rows * perRow);
-            ND4J_LAUNCH((embeddingRowsKernel<T>), dim3(gridFor(units, (Long)kThreads * kInFlight, kGridCap)), dim3(kThreads), 0, s, table, tv,
+            ND4J_LAUNCH((embeddingRowsKernel<T>), dim3(gridFor(units, (Long)kThreads * kInFlight, kRowBlocks)), dim3(kThreads), 0, s, table, tv,
                         tokens + r, z + r * zv.row, zv, (C)scale, FastDiv((unsigned)perRow), units);
         }
         return;
