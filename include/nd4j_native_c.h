@@ -233,7 +233,8 @@ void nd4j_amd_forderTileCopy(Nd4jPointer *extraPointers, float *dst, const float
 /* No counterpart in the reference (its scratch belongs to the caller).  The library keeps a workspace, reduction slots
  * and a pinned scalar block per (device, stream), allocated at the stream's first call that needs them.  A host that
  * destroys a stream calls this first, with the stream's device current: it waits for the stream to drain and frees them
- * (13 MiB of device memory and 256 bytes of pinned host memory a stream); a later call on the same handle allocates
+ * (13 MiB of device memory and 256 bytes of pinned host memory a stream, and the scratch of the operators around a
+ * language model's matrix products, if they were given none); a later call on the same handle allocates
  * afresh.  Without it they stay until the process ends. */
 void nd4j_amd_releaseStream(Nd4jPointer stream);
 /* test aid: sets the counter from which the launches on extraPointers[1]'s stream draw the tickets that tag their

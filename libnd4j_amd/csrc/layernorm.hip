@@ -333,7 +333,7 @@ __global__ void __launch_bounds__(kAcrossThreads) layerNormBpAcrossKernel(const 
 // which is why there are no more of them, and 16 waves hide the loads of each other.  (Blocks of a single team, which need not
 // wait for others but leave three times the partial sums, took 50 us where these take 35.)
 //
-// [16384, 1024] floats 40 us, 5.0 TB/s of x, dz and dx: bound by memory.  [4097, 5003] halves 35 us, of which the sums of the
+// [16384, 1024] floats 40 us, 5.0 TB/s of x, dz and dx: bound by memory.  [4097, 5003] halves 34 us, of which the sums of the
 // columns by the kernel below are 5: about 20 vector instructions an element, six rows for every team where 5.3 would be even, and 9 MB of
 // partial sums written and read again.
 constexpr int kBpThreads = 1024;
