@@ -402,28 +402,47 @@ __global__ void __launch_bounds__(THREADS) tokenProbsRowsKernel(const T *x, RowV
         const int tiles = (end - begin + TILE - 1) / TILE, spanTiles = (tiles + kSpans - 1) / kSpans;
         int span = 0, spanLeft = spanTiles;
         C spanLargest = -infinite<C>();
+        int lastShift = 0;  // by which the first vector of the last tile lies in front of its place
         Pack<T> v[VECTORS];
         for (int t = begin; t < end; t += TILE) {
             if (t + TILE <= end) {
 #pragma unroll
                 for (int j = 0; j < VECTORS; j++) v[j] = streamPackAnywhere(xr + t + (j * THREADS + (int)threadIdx.x) * N);
+            } else if (end - begin >= N) {
+                // a vector that passes the end is the last whole one: its elements that are another lane's add nothing
+                int shift[VECTORS];
+#pragma unroll
+                for (int j = 0; j < VECTORS; j++) {
+                    const int c = t + (j * THREADS + (int)threadIdx.x) * N, at = c < end - N ? c : end - N;
+                    shift[j] = c - at;
+                    v[j] = loadPackAnywhere(xr + at);
+                }
+#pragma unroll
+                for (int j = 0; j < VECTORS; j++)
+                    if (shift[j] > 0) {
+#pragma unroll
+                        for (int e = 0; e < N; e++)
+                            if (e < shift[j]) v[j].v[e] = fromCompute<T>(-infinite<C>());
+                    }
+                lastShift = shift[0];
             } else {
 #pragma unroll
                 for (int j = 0; j < VECTORS; j++) {
                     const int c = t + (j * THREADS + (int)threadIdx.x) * N;
-                    if (c + N <= end) {
-                        v[j] = loadPackAnywhere(xr + c);
-                    } else {
 #pragma unroll
-                        for (int e = 0; e < N; e++) v[j].v[e] = c + e < end ? xr[c + e] : fromCompute<T>(-infinite<C>());  // adds nothing
-                    }
+                    for (int e = 0; e < N; e++) v[j].v[e] = c + e < end ? xr[c + e] : fromCompute<T>(-infinite<C>());
                 }
             }
+            // the wave's vectors with elements of the row: in a last tile most may have none, which shows where the arithmetic takes as
+            // long as the memory ([20000, 5000] halves 70 -> 53 us; floats 2 % longer)
+            const int here = end - t - wave * kWaveLanes * N, packs = sizeof(T) == 2 ? (here + ROUND - 1) / ROUND : VECTORS;
             C tileLargest = -infinite<C>();
 #pragma unroll
             for (int j = 0; j < VECTORS; j++)
+                if (j < packs) {
 #pragma unroll
-                for (int e = 0; e < N; e++) tileLargest = Largest()(tileLargest, toCompute(v[j].v[e]));
+                    for (int e = 0; e < N; e++) tileLargest = Largest()(tileLargest, toCompute(v[j].v[e]));
+                }
             if (TOP) {
                 spanLargest = Largest()(spanLargest, tileLargest);
                 maxima[span][threadIdx.x] = spanLargest;
@@ -437,12 +456,14 @@ __global__ void __launch_bounds__(THREADS) tokenProbsRowsKernel(const T *x, RowV
             const C from = s.largest > -infinite<C>() ? s.largest : (C)0;
 #pragma unroll
             for (int j = 0; j < VECTORS; j++)
+                if (j < packs) {
 #pragma unroll
-                for (int e = 0; e < N; e++) {
-                    const C d = toCompute(v[j].v[e]) - from, p = expOf(d);
-                    s.sum += p;
-                    // (0 for an element of -infinity, where d p is not a number)
-                    if (ENTROPY) s.weighted = fma_(Largest()(d, (C)-1e30f), -p, s.weighted);
+                    for (int e = 0; e < N; e++) {
+                        const C d = toCompute(v[j].v[e]) - from, p = expOf(d);
+                        s.sum += p;
+                        // (0 for an element of -infinity, where d p is not a number)
+                        if (ENTROPY) s.weighted = fma_(Largest()(d, (C)-1e30f), -p, s.weighted);
+                    }
                 }
         }
         const C own = s.largest;
@@ -503,11 +524,11 @@ __global__ void __launch_bounds__(THREADS) tokenProbsRowsKernel(const T *x, RowV
                     for (int e = 0; e < N; e++) v.v[e] = c + e < end ? xr[c + e] : fromCompute<T>((C)0);
                 }
             };
-            auto gather = [&](int c, const Pack<T> &from) {
+            auto gather = [&](int c, int first, const Pack<T> &from) {
 #pragma unroll
                 for (int e = 0; e < N; e++) {
                     const C value = toCompute(from.v[e]);
-                    const bool is = c + e < end && value >= bound;
+                    const bool is = e >= first && c + e < end && value >= bound;
                     const unsigned long long which = __ballot(is);
                     if (which == 0ull) continue;
                     int place = 0;
@@ -520,13 +541,13 @@ __global__ void __launch_bounds__(THREADS) tokenProbsRowsKernel(const T *x, RowV
                 }
             };
             if (held) {
-                gather(begin + (int)threadIdx.x * N, v[0]);
+                gather(begin + (int)threadIdx.x * N - lastShift, lastShift, v[0]);
             } else {
                 for (Long i = wave * kWaveLanes; i < items; i += THREADS) {
                     int c;
                     Pack<T> item;
                     itemAt(i + lane, c, item);
-                    gather(c, item);
+                    gather(c, 0, item);
                     if (*(volatile int *)&found > THREADS) break;
                 }
             }
