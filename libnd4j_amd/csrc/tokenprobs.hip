@@ -483,13 +483,30 @@ __global__ void __launch_bounds__(THREADS) tokenProbsRowsKernel(const T *x, RowV
             C bound = bounds[0];
 #pragma unroll
             for (int w = 1; w < WAVES; w++) bound = bounds[w] < bound ? bounds[w] : bound;
-            if (WAVES > 1 && bound == -infinite<C>()) {  // a wave without as many elements: the k-th largest of any other will do
-                const C other = kthLargest(own, out.k, LAST);
+            if (WAVES > 1 && bound == -infinite<C>()) {
+                // A wave without as many elements, as at a row's end: the waves that have one in every lane share k, and the k-th
+                // largest of any one wave will do too.  (The second alone lets half of a short slice pass at k = 64.)
+                const bool full = __ballot(own > -infinite<C>()) == ~0ull;
+                const C alone = kthLargest(own, out.k, LAST);
                 __syncthreads();
-                if (lane == 0) bounds[wave] = other;
+                if (lane == 0) bounds[wave] = full ? (C)1 : (C)0;
+                __syncthreads();
+                int fulls = 0;
+#pragma unroll
+                for (int w = 0; w < WAVES; w++) fulls += bounds[w] > (C)0 ? 1 : 0;
+                const C shared = full ? kthLargest(own, (out.k + fulls - 1) / fulls, LAST) : infinite<C>();
+                __syncthreads();
+                if (lane == 0) bounds[wave] = shared;
+                __syncthreads();
+                C least = bounds[0];
+#pragma unroll
+                for (int w = 1; w < WAVES; w++) least = bounds[w] < least ? bounds[w] : least;
+                __syncthreads();
+                if (lane == 0) bounds[wave] = alone;
                 __syncthreads();
 #pragma unroll
                 for (int w = 0; w < WAVES; w++) bound = Largest()(bound, bounds[w]);
+                if (fulls > 0) bound = Largest()(bound, least);
             }
             const bool held = VECTORS == 1 && tiles == 1;  // every thread's elements are in its registers still
             if (!held) {
