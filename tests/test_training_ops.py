@@ -486,6 +486,21 @@ def test_token_log_probs_lengths(dev, S, n):
 
 
 @pytest.mark.parametrize("S", SUFFIXES)
+@pytest.mark.parametrize("more", (1, 5, 81, 200, 512, 904, 1105, 2047))
+def test_token_log_probs_at_a_rows_end(dev, S, more):
+    """the last slice of a row with few elements in its waves, and fewer than the alternatives; the largest ones lie there"""
+    rs = np.random.RandomState(more)
+    n = 8192 + more
+    for k in (8, 17, 33, 64):
+        x = (rs.randn(3, n) * 4).astype(STORAGE[S])
+        x[1, 8192:] += 16
+        x[2] = np.round(x[2])
+        x[2, :8192 - 7] = -np.inf
+        tokens = rs.randint(0, n, 3)
+        check_token_probs(run_token_probs(dev, S, x, tokens, k), token_probs_oracle(x, tokens, k, S))
+
+
+@pytest.mark.parametrize("S", SUFFIXES)
 @pytest.mark.parametrize("layout", LAYOUTS)
 def test_token_log_probs_layouts(dev, S, layout):
     rs = np.random.RandomState(6)
