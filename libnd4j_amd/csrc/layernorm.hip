@@ -27,13 +27,9 @@ template <typename T> __device__ __forceinline__ typename Compute<T>::type plus(
         return acc + toCompute(v);
     }
 }
-// (v - mu) s; offset = -mu s.  For halves as v s - mu s: it rounds mu s, 2^-24 of it, where the result keeps 2^-11 of itself.
-template <typename T>
-__device__ __forceinline__ typename Compute<T>::type normal(T v, typename Compute<T>::type mu, typename Compute<T>::type s,
-                                                            typename Compute<T>::type offset) {
-    if constexpr (sizeof(T) == 2) return fused(toCompute(v), s, offset);
-    else return (toCompute(v) - mu) * s;
-}
+// v - mu, which is taken before anything else is: where a row's values are near each other v s and mu s are far larger than
+// their difference, and a rounding of mu s on its own is an error of that size (a constant row of 30000 came out as 0.5).
+template <typename T> __device__ __forceinline__ typename Compute<T>::type less(T v, typename Compute<T>::type mu) { return plus(-mu, v); }
 // what is known to be no NaN
 __device__ __forceinline__ float16 fromNumber(float v) {
     float16 h;
@@ -213,12 +209,12 @@ __global__ void __launch_bounds__(1024)
             if (lane + j * size < vectors) {
 #pragma unroll
                 for (int e = 0; e < N; e++) {
-                    const C d = plus(-mu, v[j].v[e]);
+                    const C d = less(v[j].v[e], mu);
                     squares[0] = fused(d, d, squares[0]);
                 }
             }
         teamSums<LANES>(squares, smem, teamWaves, turn);
-        const C s = (C)1 / sqrtOf(squares[0] / (C)length + epsilon), offset = -mu * s;
+        const C s = (C)1 / sqrtOf(squares[0] / (C)length + epsilon);
         if (!live) continue;
         if (lane == 0) {
             if (mean != nullptr) mean[r] = mu;
@@ -233,7 +229,7 @@ __global__ void __launch_bounds__(1024)
                 if (!HELD && bias != nullptr) b[j] = loadPackAnywhere(bias + at[j]);
 #pragma unroll
                 for (int e = 0; e < N; e++) {
-                    C h = normal(v[j].v[e], mu, s, offset);
+                    C h = less(v[j].v[e], mu) * s;
                     if (gain != nullptr) h = fused(h, toCompute(g[j].v[e]), bias != nullptr ? toCompute(b[j].v[e]) : (C)0);
                     else if (bias != nullptr) h += toCompute(b[j].v[e]);
                     o.v[e] = fromCompute<T>(h);
@@ -351,6 +347,7 @@ __global__ void __launch_bounds__(kBpThreads)
     // Long rows of floats and doubles are read with the streaming policy: [16384, 1024] floats 40.0 us, 41.6 with the ordinary one.
     // (Short ones, [100000, 64] floats, 22.0 and 19.7; [4097, 5003] halves 40.0 and 35.2.)
     constexpr bool STREAM = sizeof(T) > 2 && PACKS > 1;
+    constexpr bool LATE = sizeof(T) == 2;  // s multiplied in where it costs least, an instruction an element instead of three
     extern __shared__ __align__(16) char dynamicLds[];
     C *columns = reinterpret_cast<C *>(dynamicLds);  // [half of the teams][columns of a row]
     __shared__ C sums[8 * (kBpThreads / kWaveLanes)];  // (the waves behind the last whole team have places too)
@@ -408,34 +405,39 @@ __global__ void __launch_bounds__(kBpThreads)
         dRest = nextDRest;
         mu = nextMu;
         s = nextS;
-        const C offset = -mu * s;
         if (r0 + step < xv.rows) ask(r0 + step);
-        C sum[2] = {(C)0, (C)0};  // of a and of a h
+        C sum[2] = {(C)0, (C)0};  // of a and of a h (halves: of a (x - mean), which cannot leave a float's range, and s behind the row)
         if (live) {
 #pragma unroll
             for (int j = 0; j < PACKS; j++)
                 if (lane + j * size < vectors) {
 #pragma unroll
                     for (int e = 0; e < N; e++) {
-                        const C dd = toCompute(d[j].v[e]), h = normal(v[j].v[e], mu, s, offset);
+                        const C dd = toCompute(d[j].v[e]), m = less(v[j].v[e], mu);
                         const C a = times(d[j].v[e], g[j].v[e]);
                         sum[0] += a;
-                        sum[1] = fused(a, h, sum[1]);
-                        gainSum[j][e] = fused(dd, h, gainSum[j][e]);
+                        if constexpr (LATE) {
+                            sum[1] = fused(a, m, sum[1]);
+                            gainSum[j][e] = fused(dd * s, m, gainSum[j][e]);
+                        } else {
+                            sum[1] = fused(a, m * s, sum[1]);
+                            gainSum[j][e] = fused(dd, m * s, gainSum[j][e]);
+                        }
                         biasSum[j][e] = plus(biasSum[j][e], d[j].v[e]);
                     }
                 }
             if (rest < length) {
                 const C h = (vRest - mu) * s, a = dRest * gRest;
                 sum[0] += a;
-                sum[1] = fused(a, h, sum[1]);
+                sum[1] = fused(a, LATE ? vRest - mu : h, sum[1]);
                 gainRest = fused(dRest, h, gainRest);
                 biasRest += dRest;
             }
         }
         if (dx == nullptr) continue;
         teamSums<LANES>(sum, smem, teamWaves, turn);
-        const C meanA = sum[0] / (C)length, meanAH = sum[1] / (C)length;
+        if (LATE) sum[1] *= s;
+        const C meanA = sum[0] / (C)length, meanAH = sum[1] / (C)length, share = s * meanAH;  // (of x - mean: h meanAH)
         if (!live) continue;
         T *dxr = dx + r * dxv.row;
         auto store = [&](auto convert) {
@@ -445,17 +447,17 @@ __global__ void __launch_bounds__(kBpThreads)
                     Pack<T> o;
 #pragma unroll
                     for (int e = 0; e < N; e++) {
-                        const C h = normal(v[j].v[e], mu, s, offset), a = fused(toCompute(d[j].v[e]), toCompute(g[j].v[e]), -meanA);
-                        o.v[e] = convert(s * fused(-h, meanAH, a));
+                        const C m = less(v[j].v[e], mu), a = fused(toCompute(d[j].v[e]), toCompute(g[j].v[e]), -meanA);
+                        o.v[e] = convert(s * (LATE ? fused(-m, share, a) : fused(-(m * s), meanAH, a)));
                     }
                     streamPackAnywhere(dxr + at[j], o);
                 }
         };
         if constexpr (sizeof(T) == 2) {
-            // Finite sums have finite terms, a and h then are finite too, and what an infinite product adds up to is no NaN: so
-            // is no element of dx, unless s is 0.  (A NaN's own bits take a compare and a select an element: 39 us where this
+            // Finite sums have finite terms, a and x - mean then are finite too, and what an infinite product adds up to is no NaN:
+            // so is no element of dx, unless s is 0.  (A NaN's own bits take a compare and a select an element: 39 us where this
             // takes 35, a select for a missing gain among them, which is a gain of 1 now.)
-            if (::fabsf(sum[0]) < infinite<C>() && ::fabsf(sum[1]) < infinite<C>() && s != (C)0)
+            if (::fabsf(sum[0]) < infinite<C>() && ::fabsf(share) < infinite<C>() && s != (C)0)
                 store([](C o) { return fromNumber(o); });
             else
                 store([](C o) { return fromCompute<T>(o); });
