@@ -358,8 +358,8 @@ void nd4j_amd_execTokenLogProbsBpDouble(Nd4jPointer *extraPointers, double *x, N
                                         double *dEntropy, double *dx, Nd4jLong *dxShapeInfo);
 
 /* norm[0] = the square root of the sum of the squares of all elements of n tensors, and dz = dx * maxNorm / norm where
- * the norm is finite and greater than maxNorm, dz = dx otherwise (a norm of infinity or NaN changes nothing, so that the
- * caller can look at it and skip the step).  dx and dz are device tables of n device pointers, dense tensors of
+ * the norm is greater than maxNorm and finite in the type of norm[0], dz = dx otherwise (a norm of infinity or NaN changes
+ * nothing, so that the caller can look at it and skip the step).  dx and dz are device tables of n device pointers, dense tensors of
  * offsets[i + 1] - offsets[i] elements (offsets: n + 1 entries on the device, from 0, ascending); dz may be the table dx,
  * or name the same tensors: clipping in place.  total is offsets[n], known to the host.  norm may be null; with dz null
  * the norm alone is computed and maxNorm is not looked at. */

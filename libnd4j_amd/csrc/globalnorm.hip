@@ -2,6 +2,9 @@
 //
 //   norm = sqrt(sum of g^2),  f = maxNorm / norm where maxNorm < norm < infinity, else 1,  out = f g
 //
+// A norm counts as infinite where the type that the caller gets it in does not hold it, so that what the caller reads and what
+// was done to the tensors agree.
+//
 // The tensors' elements count as one range, cut into tiles that the blocks take in turn.  A tile inside one tensor is walked
 // in vectors (unaligned ones: tensors may begin anywhere), a tile that holds ends of tensors vector by vector too, every
 // thread looking the tensor up for its own (a vector across tensors goes element by element): a thousand tensors of ten
@@ -141,7 +144,7 @@ __global__ void __launch_bounds__(kNormThreads) clipKernel(const T *const *given
     if (norm != nullptr && blockIdx.x == 0 && threadIdx.x == 0) norm[0] = (C)value;
     if (out == nullptr) return;
     // (a NaN norm compares false, so it leaves the factor at 1 like one that is infinite)
-    const C factor = value > maxNorm && value < infinite<double>() ? (C)(maxNorm / value) : (C)1;
+    const C factor = value > maxNorm && (C)value < infinite<C>() ? (C)(maxNorm / value) : (C)1;
     const Long whole = wholeLength(offsets, n, total);
     int low = 0;
     for (Long t = (Long)blockIdx.x * tile; t < whole; t += (Long)gridDim.x * tile) {
