@@ -47,6 +47,7 @@ __device__ __forceinline__ int tensorAt(const Long *offsets, int low, int high, 
 // Searches wait for one offset after the other, and for the tensor's address then, a trip to the cache each: of up to
 // kStaged - 1 tensors a block copies both tables into LDS first.
 constexpr int kStaged = 1024;
+template <typename C> __device__ __forceinline__ C smallestNormal() { return sizeof(C) == 4 ? (C)0x1p-126 : (C)0x1p-1022; }
 template <typename T> struct Tables {
     const Long *offsets;
     const T *const *in;
@@ -146,42 +147,54 @@ __global__ void __launch_bounds__(kNormThreads) clipKernel(const T *const *given
     // (a NaN norm compares false, so it leaves the factor at 1 like one that is infinite)
     const C factor = value > maxNorm && (C)value < infinite<C>() ? (C)(maxNorm / value) : (C)1;
     const Long whole = wholeLength(offsets, n, total);
-    int low = 0;
-    for (Long t = (Long)blockIdx.x * tile; t < whole; t += (Long)gridDim.x * tile) {
-        const Long end = t + tile < whole ? t + tile : whole;
-        low = tensorAt(offsets, low, n - 1, t);
-        const int high = end <= offsets[low + 1] ? low : tensorAt(offsets, low, n - 1, end - 1);
-        if (low == high && end - t == tile && t >= offsets[low]) {
-            const Long at = (t - offsets[low]) + threadIdx.x * N;
-            const T *from = in[low] + at;
-            T *to = out[low] + at;
-            Pack<T> v[VECTORS];
+    auto walk = [&](auto scaled) {
+        int low = 0;
+        for (Long t = (Long)blockIdx.x * tile; t < whole; t += (Long)gridDim.x * tile) {
+            const Long end = t + tile < whole ? t + tile : whole;
+            low = tensorAt(offsets, low, n - 1, t);
+            const int high = end <= offsets[low + 1] ? low : tensorAt(offsets, low, n - 1, end - 1);
+            if (low == high && end - t == tile && t >= offsets[low]) {
+                const Long at = (t - offsets[low]) + threadIdx.x * N;
+                const T *from = in[low] + at;
+                T *to = out[low] + at;
+                Pack<T> v[VECTORS];
 #pragma unroll
-            for (int j = 0; j < VECTORS; j++) v[j] = streamPackAnywhere(from + j * (kNormThreads * N));
+                for (int j = 0; j < VECTORS; j++) v[j] = streamPackAnywhere(from + j * (kNormThreads * N));
 #pragma unroll
-            for (int j = 0; j < VECTORS; j++) {
+                for (int j = 0; j < VECTORS; j++) {
 #pragma unroll
-                for (int e = 0; e < N; e++) v[j].v[e] = fromCompute<T>(toCompute(v[j].v[e]) * factor);
-                streamPackAnywhere(to + j * (kNormThreads * N), v[j]);
-            }
-        } else {
-            for (Long i = t + threadIdx.x * N; i < end; i += kNormThreads * N) {
-                int k = tensorAt(offsets, low, high, i);
-                if (i >= offsets[k] && i + N <= end && i + N <= offsets[k + 1]) {
-                    Pack<T> v = loadPackAnywhere(in[k] + (i - offsets[k]));
-#pragma unroll
-                    for (int e = 0; e < N; e++) v.v[e] = fromCompute<T>(toCompute(v.v[e]) * factor);
-                    storePackAnywhere(out[k] + (i - offsets[k]), v);
-                    continue;
+                    for (int e = 0; e < N; e++) v[j].v[e] = fromCompute<T>(scaled(toCompute(v[j].v[e])));
+                    streamPackAnywhere(to + j * (kNormThreads * N), v[j]);
                 }
-                for (Long j = i; j < i + N && j < end; j++) {
-                    while (k < high && j >= offsets[k + 1]) k++;
-                    if (j < offsets[k]) continue;
-                    out[k][j - offsets[k]] = fromCompute<T>(toCompute(in[k][j - offsets[k]]) * factor);
+            } else {
+                for (Long i = t + threadIdx.x * N; i < end; i += kNormThreads * N) {
+                    int k = tensorAt(offsets, low, high, i);
+                    if (i >= offsets[k] && i + N <= end && i + N <= offsets[k + 1]) {
+                        Pack<T> v = loadPackAnywhere(in[k] + (i - offsets[k]));
+#pragma unroll
+                        for (int e = 0; e < N; e++) v.v[e] = fromCompute<T>(scaled(toCompute(v.v[e])));
+                        storePackAnywhere(out[k] + (i - offsets[k]), v);
+                        continue;
+                    }
+                    for (Long j = i; j < i + N && j < end; j++) {
+                        while (k < high && j >= offsets[k + 1]) k++;
+                        if (j < offsets[k]) continue;
+                        out[k][j - offsets[k]] = fromCompute<T>(scaled(toCompute(in[k][j - offsets[k]])));
+                    }
                 }
             }
         }
+    };
+    if constexpr (sizeof(T) > 2) {
+        // Of a factor below the type's normal range few bits are left, or none: it goes in two steps then, in double.  (Halves are
+        // far below their range with such a factor.)
+        if (factor < smallestNormal<C>()) {
+            const double down = 0x1p-600, rest = maxNorm / (value * down);
+            walk([=](C v) { return (C)((double)v * down * rest); });
+            return;
+        }
     }
+    walk([=](C v) { return v * factor; });
 }
 
 }  // namespace

@@ -47,3 +47,15 @@ def test_floats_whose_norm_no_float_holds(dev, apart):
         check(dev, "Float", [np.array(values, np.float32)], 1.0, apart=apart, inplace=True)
     for values in ([3.4e38], [2e38, -2e38], [1e38] * 11):  # these are held
         check(dev, "Float", [np.array(values, np.float32), np.ones(77, np.float32)], 1.0, apart=apart)
+
+
+@pytest.mark.parametrize("S", ("Float",))
+@pytest.mark.parametrize("n", (3, 700))
+def test_factors_below_the_normal_range(dev, S, n):
+    """large gradients and a small bound: the factor has few bits in the type, or none, and the product all"""
+    rs = np.random.RandomState(n)
+    big, small = (1e37, (1e-2, 1e-4, 1e-9)) if S == "Float" else (1e306, (1e-3, 1e-8, 1e-20))
+    tensors = [(rs.randn(n) * big / 8).astype(STORAGE[S]), rs.randn(n).astype(STORAGE[S])]
+    for most in small:
+        check(dev, S, tensors, most)
+        check(dev, S, tensors, most, inplace=True)
