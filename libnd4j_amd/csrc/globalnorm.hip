@@ -17,7 +17,9 @@
 // take 12.5 us, which is two launches.
 //
 // Squares are summed in double: the square of any float is finite there, and the order of the sum does not show in the
-// result's type.  (Squares of halves are exact in float; eight of them are added there first.)
+// result's type.  (Squares of halves are exact in float; eight of them are added there first.)  Squares of doubles have three
+// sums, of elements around 1 and of those far above and below it, scaled by a power of two, so that any norm that a double holds
+// comes out.
 #include "launch.h"
 #include "training.cuh"
 
@@ -47,7 +49,6 @@ __device__ __forceinline__ int tensorAt(const Long *offsets, int low, int high, 
 // Searches wait for one offset after the other, and for the tensor's address then, a trip to the cache each: of up to
 // kStaged - 1 tensors a block copies both tables into LDS first.
 constexpr int kStaged = 1024;
-template <typename C> __device__ __forceinline__ C smallestNormal() { return sizeof(C) == 4 ? (C)0x1p-126 : (C)0x1p-1022; }
 template <typename T> struct Tables {
     const Long *offsets;
     const T *const *in;
@@ -68,33 +69,103 @@ __device__ __forceinline__ Tables<T> stagedTables(const T *const *in, const Long
     return t;
 }
 
-template <typename T> __device__ __forceinline__ double squaresOf(const Pack<T> &v) {
-    constexpr int N = Pack<T>::N;
-    if constexpr (sizeof(T) == 2) {
-        float sum = 0.0f;
-#pragma unroll
-        for (int e = 0; e < N; e++) sum += toCompute(v.v[e]) * toCompute(v.v[e]);
-        return (double)sum;
-    } else {
-        double sum = 0.0;
-#pragma unroll
-        for (int e = 0; e < N; e++) sum = __builtin_fma((double)toCompute(v.v[e]), (double)toCompute(v.v[e]), sum);
-        return sum;
+template <typename C> __device__ __forceinline__ C smallestNormal() { return sizeof(C) == 4 ? (C)0x1p-126 : (C)0x1p-1022; }
+
+// A sum of squares
+template <typename T> struct Squares {
+    double sum;
+    __device__ __forceinline__ void clear() { sum = 0.0; }
+    __device__ __forceinline__ void join(const Squares &o) { sum += o.sum; }
+    __device__ __forceinline__ void add(T v) {
+        const double d = (double)toCompute(v);
+        sum += d * d;
     }
-}
+    template <int VECTORS> __device__ __forceinline__ void add(const Pack<T> (&v)[VECTORS]) {
+#pragma unroll
+        for (int j = 0; j < VECTORS; j++) add(v[j]);
+    }
+    __device__ __forceinline__ void add(const Pack<T> &v) {
+        constexpr int N = Pack<T>::N;
+        if constexpr (sizeof(T) == 2) {
+            float eight = 0.0f;
+#pragma unroll
+            for (int e = 0; e < N; e++) eight += toCompute(v.v[e]) * toCompute(v.v[e]);
+            sum += (double)eight;
+        } else {
+            double four = 0.0;
+#pragma unroll
+            for (int e = 0; e < N; e++) four = __builtin_fma((double)toCompute(v.v[e]), (double)toCompute(v.v[e]), four);
+            sum += four;
+        }
+    }
+    __device__ __forceinline__ bool sumIsAll() const { return true; }
+    __device__ __forceinline__ double root() const { return ::sqrt(sum); }
+};
+// Elements beyond 2^480 are squared as 2^-600 of themselves (2^56 of the largest squares that are not scaled, 2^960, are a double
+// still), those below 2^-400 as 2^600 of themselves (what is not scaled has normal squares).  NaN counts as usual, infinity as large.
+template <> struct Squares<double> {
+    double sum, large, small;
+    __device__ __forceinline__ void clear() { sum = large = small = 0.0; }
+    __device__ __forceinline__ void join(const Squares &o) {
+        sum += o.sum;
+        large += o.large;
+        small += o.small;
+    }
+    __device__ __forceinline__ void add(double v) {
+        const double size = ::fabs(v);
+        if (size > 0x1p480) large = __builtin_fma(v * 0x1p-600, v * 0x1p-600, large);
+        else if (size < 0x1p-400) small = __builtin_fma(v * 0x1p600, v * 0x1p600, small);
+        else sum = __builtin_fma(v, v, sum);
+    }
+    // Several at once: squared as they are, if the sum says that none was large and none small that counts (looked at element by
+    // element, 50M doubles took 203 us instead of 195).
+    template <int VECTORS> __device__ __forceinline__ void add(const Pack<double> (&v)[VECTORS]) {
+        double all = 0.0;
+#pragma unroll
+        for (int j = 0; j < VECTORS; j++) all = __builtin_fma(v[j].v[0], v[j].v[0], __builtin_fma(v[j].v[1], v[j].v[1], all));
+        if (all >= 0x1p-740 && all <= 0x1p960) {
+            sum += all;
+        } else {
+#pragma unroll
+            for (int j = 0; j < VECTORS; j++) {
+                add(v[j].v[0]);
+                add(v[j].v[1]);
+            }
+        }
+    }
+    __device__ __forceinline__ bool sumIsAll() const { return large == 0.0 && small == 0.0; }
+    __device__ __forceinline__ double root() const {
+        if (large != 0.0) return ::sqrt(large + sum * 0x1p-600 * 0x1p-600) * 0x1p600;  // (what is small is lost beside it)
+        if (sum != 0.0) return ::sqrt(sum + small * 0x1p-600 * 0x1p-600);
+        return ::sqrt(small) * 0x1p-600;
+    }
+};
+// What the blocks of the first sweep leave: their sums, and of doubles all three, NaN as the sum saying that they are needed (to
+// read and add up three for every block of the second sweep took 4 % longer over 50M doubles).
+template <typename T> struct Partial {
+    double sums[kNormBlocks];
+    Squares<double> whole[sizeof(T) == 8 ? kNormBlocks : 1];
+};
+struct JoinSquares {
+    template <typename S> __device__ __forceinline__ S operator()(S a, S b) const {
+        a.join(b);
+        return a;
+    }
+};
 
 template <typename T, int VECTORS>
-__global__ void __launch_bounds__(kNormThreads) squaresKernel(const T *const *givenIn, const Long *givenOffsets, int n, Long total, double *partial) {
+__global__ void __launch_bounds__(kNormThreads) squaresKernel(const T *const *givenIn, const Long *givenOffsets, int n, Long total, Partial<T> *partial) {
     constexpr int N = Pack<T>::N;
     constexpr Long tile = (Long)kNormThreads * VECTORS * N;
-    __shared__ double smem[kNormThreads / kWaveLanes];
+    __shared__ Squares<T> smem[kNormThreads / kWaveLanes];
     __shared__ Long stagedOffsets[kStaged];
     __shared__ const T *stagedIn[kStaged];
     const Tables<T> tables = stagedTables<T>(givenIn, givenOffsets, n, stagedOffsets, stagedIn);
     const Long *offsets = tables.offsets;
     const T *const *in = tables.in;
     const Long whole = wholeLength(offsets, n, total);
-    double sum = 0.0;
+    Squares<T> sum;
+    sum.clear();
     int low = 0;  // (the tiles of a block ascend)
     for (Long t = (Long)blockIdx.x * tile; t < whole; t += (Long)gridDim.x * tile) {
         const Long end = t + tile < whole ? t + tile : whole;
@@ -105,31 +176,33 @@ __global__ void __launch_bounds__(kNormThreads) squaresKernel(const T *const *gi
             Pack<T> v[VECTORS];
 #pragma unroll
             for (int j = 0; j < VECTORS; j++) v[j] = loadPackAnywhere(from + j * (kNormThreads * N));
-#pragma unroll
-            for (int j = 0; j < VECTORS; j++) sum += squaresOf<T>(v[j]);
+            sum.add(v);
         } else {
             for (Long i = t + threadIdx.x * N; i < end; i += kNormThreads * N) {
                 int k = tensorAt(offsets, low, high, i);
                 if (i >= offsets[k] && i + N <= end && i + N <= offsets[k + 1]) {
-                    sum += squaresOf<T>(loadPackAnywhere(in[k] + (i - offsets[k])));
+                    const Pack<T> one[1] = {loadPackAnywhere(in[k] + (i - offsets[k]))};
+                    sum.add(one);
                     continue;
                 }
                 for (Long j = i; j < i + N && j < end; j++) {
                     while (k < high && j >= offsets[k + 1]) k++;
                     if (j < offsets[k]) continue;
-                    const double v = (double)toCompute(in[k][j - offsets[k]]);
-                    sum += v * v;
+                    sum.add(in[k][j - offsets[k]]);
                 }
             }
         }
     }
-    sum = blockAll<kNormThreads>(sum, Add(), smem);
-    if (threadIdx.x == 0) partial[blockIdx.x] = sum;
+    sum = blockAll<kNormThreads>(sum, JoinSquares(), smem);
+    if (threadIdx.x == 0) {
+        partial->sums[blockIdx.x] = sum.sumIsAll() ? sum.sum : (double)notANumber<float>();
+        if constexpr (sizeof(T) == 8) partial->whole[blockIdx.x] = sum;
+    }
 }
 
 template <typename T, int VECTORS>
 __global__ void __launch_bounds__(kNormThreads) clipKernel(const T *const *givenIn, T *const *out, const Long *givenOffsets, int n, Long total,
-                                                           double maxNorm, typename Compute<T>::type *norm, const double *partial, int parts) {
+                                                           double maxNorm, typename Compute<T>::type *norm, const Partial<T> *partial, int parts) {
     typedef typename Compute<T>::type C;
     constexpr int N = Pack<T>::N;
     constexpr Long tile = (Long)kNormThreads * VECTORS * N;
@@ -140,8 +213,17 @@ __global__ void __launch_bounds__(kNormThreads) clipKernel(const T *const *given
     const Long *offsets = tables.offsets;
     const T *const *in = tables.in;
     double sum = 0.0;
-    for (int i = threadIdx.x; i < parts; i += kNormThreads) sum += partial[i];
-    const double value = ::sqrt(blockAll<kNormThreads>(sum, Add(), smem));
+    for (int i = threadIdx.x; i < parts; i += kNormThreads) sum += partial->sums[i];
+    double value = ::sqrt(blockAll<kNormThreads>(sum, Add(), smem));
+    if constexpr (sizeof(T) == 8) {
+        if (value != value) {  // (of all threads of the block, which have the same one)
+            __shared__ Squares<T> wholes[kNormThreads / kWaveLanes];
+            Squares<T> whole;
+            whole.clear();
+            for (int i = threadIdx.x; i < parts; i += kNormThreads) whole.join(partial->whole[i]);
+            value = blockAll<kNormThreads>(whole, JoinSquares(), wholes).root();
+        }
+    }
     if (norm != nullptr && blockIdx.x == 0 && threadIdx.x == 0) norm[0] = (C)value;
     if (out == nullptr) return;
     // (a NaN norm compares false, so it leaves the factor at 1 like one that is infinite)
@@ -199,12 +281,12 @@ __global__ void __launch_bounds__(kNormThreads) clipKernel(const T *const *given
 
 }  // namespace
 
-size_t clipByGlobalNormScratch(Long) { return kNormBlocks * sizeof(double); }
+size_t clipByGlobalNormScratch(Long) { return sizeof(Partial<double>); }
 
 template <typename T>
 void launchClipByGlobalNorm(hipStream_t s, const T *const *in, T *const *out, const Long *offsets, int n, Long total, double maxNorm,
                             typename Compute<T>::type *norm, void *scratch) {
-    double *partial = reinterpret_cast<double *>(scratch);
+    Partial<T> *partial = reinterpret_cast<Partial<T> *>(scratch);
     // From 25 MB on the first sweep takes tiles of eight vectors a thread and the second tiles of four, a block each (as many blocks
     // as the first, tile after tile: 270 us where these take 245; eight vectors 250, two 294, since every block adds up the sums
     // first).  Smaller ones go in tiles of one vector, for more blocks: 6M floats 26.3 us, 27.0 in large tiles, but 8M 35.9 and 30.5.

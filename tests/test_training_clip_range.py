@@ -49,7 +49,7 @@ def test_floats_whose_norm_no_float_holds(dev, apart):
         check(dev, "Float", [np.array(values, np.float32), np.ones(77, np.float32)], 1.0, apart=apart)
 
 
-@pytest.mark.parametrize("S", ("Float",))
+@pytest.mark.parametrize("S", ("Float", "Double"))
 @pytest.mark.parametrize("n", (3, 700))
 def test_factors_below_the_normal_range(dev, S, n):
     """large gradients and a small bound: the factor has few bits in the type, or none, and the product all"""
@@ -59,3 +59,21 @@ def test_factors_below_the_normal_range(dev, S, n):
     for most in small:
         check(dev, S, tensors, most)
         check(dev, S, tensors, most, inplace=True)
+
+
+@pytest.mark.parametrize("apart", (True, False))
+def test_doubles_whose_squares_no_double_holds(dev, apart):
+    rs = np.random.RandomState(2)
+    rows = rs.randn(600)
+    for scale in (1e200, 1e153, 1e155, 1e306, 1e-153, 1e-155, 1e-163, 1e-200, 1e-300, 1e-310):
+        check(dev, "Double", [rows * scale, -rows[:5] * scale], 1.0, apart=apart)
+        check(dev, "Double", [rows * scale, rows[:77] * 1e-3], 0.5, apart=apart)
+        check(dev, "Double", [rows * scale, rows[:77] * 1e-170, rows[:9] * 1e150], scale / 4, apart=apart)
+    check(dev, "Double", [np.array([1.7e308])], 1.0, apart=apart)
+    check(dev, "Double", [np.array([1.7e308, 1e308])], 1.0, apart=apart)  # the norm is beyond the range
+    check(dev, "Double", [np.array([5e-324, 0.0, -5e-324])], 1.0, apart=apart)
+    for bad in (np.nan, np.inf):
+        t = np.array([1e200, bad, 1e-200, 1.0])
+        got, value = run_clip(dev, "Double", [t], 1.0, apart)
+        assert np.array_equal(got[0], t, equal_nan=True)
+        assert np.isnan(value) if np.isnan(bad) else np.isposinf(value)
