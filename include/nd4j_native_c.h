@@ -268,9 +268,9 @@ void nd4j_amd_execReduceFloatNoAlloc(Nd4jPointer *extraPointers, int opNum, floa
  *
  * Execution.  Every call is enqueued on the stream of extraPointers[1], returns without waiting, allocates nothing
  * but scratch, gives the same bits for the same inputs, and may be captured into a graph.  Calls with a `scratch`
- * argument take null for it (the library then keeps a block per device and stream, freed by
- * nd4j_amd_releaseStream) or scratchBytes bytes of the caller's at a 16-byte boundary, at least what the
- * nd4j_amd_scratch... function of that call says for the sizes.  On a stream under capture null is refused: a graph
+ * argument take null for it (the library then keeps blocks per device and stream, each twice as large at least as the
+ * one before, freed by nd4j_amd_releaseStream) or scratchBytes bytes of the caller's at a 16-byte boundary, at least what
+ * the nd4j_amd_scratch... function of that call says for the sizes.  On a stream under capture null is refused: a graph
  * needs scratch that no other graph and no other stream uses while it runs.  Arguments that do not fit are refused
  * (nd4j_lastError) before anything is enqueued; results are then left untouched.  Results must not overlap inputs
  * unless a call says so. */

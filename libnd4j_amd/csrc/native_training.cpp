@@ -74,15 +74,18 @@ void sameShape(const char *op, const char *a, const RowView &x, const char *b, c
     if (x.rows != z.rows || x.length != z.length) refuse(op, std::string(a) + " and " + b + " differ in shape");
 }
 
-// The caller's scratch when it is given one, else the stream's.  A stream under capture gets none of the library's: two
-// graphs captured on it would share the block, and a later call that outgrows it would free it under them.
-void *scratchFor(const char *op, hipStream_t s, void *given, Long givenBytes, size_t bytes) {
-    if (bytes == 0) return nullptr;
+// The caller's scratch when it is given one, else the stream's, kept until the call's launches are enqueued.  A stream under
+// capture gets none of the library's: two graphs captured on it would share the block, and a later call that outgrows it would
+// free it under them.
+OperatorScratch scratchFor(const char *op, hipStream_t s, void *given, Long givenBytes, size_t bytes) {
+    OperatorScratch scratch;
+    if (bytes == 0) return scratch;
     if (given != nullptr) {
         if (givenBytes < 0 || (size_t)givenBytes < bytes)
             refuse(op, "the scratch holds " + std::to_string(givenBytes) + " bytes, " + std::to_string(bytes) + " are needed");
         if (reinterpret_cast<uintptr_t>(given) % 16 != 0) refuse(op, "the scratch is not aligned to 16 bytes");
-        return given;
+        scratch.ptr = given;
+        return scratch;
     }
     if (streamIsCapturing(s))
         throw std::runtime_error(std::string(op) + ": the stream is being captured, which needs scratch of the graph's own (" +
@@ -141,8 +144,8 @@ void layerNormBp(Nd4jPointer *extra, T *x, Long *xInfo, T *gain, typename Comput
         return;
     }
     const bool columns = dGain != nullptr || dBias != nullptr;
-    void *work = scratchFor(op, s, scratch, scratchBytes, columns ? layerNormBpScratch(xv.rows, xv.length) : 0);
-    launchLayerNormBp<T>(s, x, xv, gain, mean, invStd, dz, dzv, dx, dxv, dGain, dBias, work);
+    const OperatorScratch work = scratchFor(op, s, scratch, scratchBytes, columns ? layerNormBpScratch(xv.rows, xv.length) : 0);
+    launchLayerNormBp<T>(s, x, xv, gain, mean, invStd, dz, dzv, dx, dxv, dGain, dBias, work.ptr);
     checkLaunch(op, s);
 }
 
@@ -187,8 +190,8 @@ void embeddingBp(Nd4jPointer *extra, T *dz, Long *dzInfo, Long *tokens, Long n, 
         must(op, "dz", dz);
         must(op, "tokens", tokens);
     }
-    void *work = scratchFor(op, s, scratch, scratchBytes, n > 0 ? embeddingBpScratch(n, tv.length) : 0);
-    launchEmbeddingBp<T>(s, dz, dzv, tokens, dTable, tv, scale, accumulate != 0, work);
+    const OperatorScratch work = scratchFor(op, s, scratch, scratchBytes, n > 0 ? embeddingBpScratch(n, tv.length) : 0);
+    launchEmbeddingBp<T>(s, dz, dzv, tokens, dTable, tv, scale, accumulate != 0, work.ptr);
     checkLaunch(op, s);
 }
 
@@ -218,8 +221,8 @@ void tokenLogProbs(Nd4jPointer *extra, T *x, Long *xInfo, Long *tokens, typename
     out.k = k;
     out.top = top;
     out.topLogProbs = k > 0 ? topLogProbs : nullptr;
-    void *work = scratchFor(op, s, scratch, scratchBytes, tokenLogProbsScratch(xv.rows, xv.length, k));
-    launchTokenLogProbs<T>(s, x, xv, tokens, out, work);
+    const OperatorScratch work = scratchFor(op, s, scratch, scratchBytes, tokenLogProbsScratch(xv.rows, xv.length, k));
+    launchTokenLogProbs<T>(s, x, xv, tokens, out, work.ptr);
     checkLaunch(op, s);
 }
 
@@ -265,9 +268,9 @@ void clipByGlobalNorm(Nd4jPointer *extra, Nd4jPointer *dx, Nd4jPointer *dz, Long
         must(op, "offsets", offsets);
         mayBe(op, "the table of results", dz);
     }
-    void *work = scratchFor(op, s, scratch, scratchBytes, clipByGlobalNormScratch(total));
+    const OperatorScratch work = scratchFor(op, s, scratch, scratchBytes, clipByGlobalNormScratch(total));
     launchClipByGlobalNorm<T>(s, reinterpret_cast<const T *const *>(dx), reinterpret_cast<T *const *>(dz), offsets, n, total, maxNorm, norm,
-                              work);
+                              work.ptr);
     checkLaunch(op, s);
 }
 

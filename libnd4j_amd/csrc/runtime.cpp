@@ -173,30 +173,48 @@ Workspace workspaceFor(hipStream_t s, size_t minBytes) {
 }
 
 namespace {
-std::map<std::pair<int, hipStream_t>, std::pair<void *, size_t> > gOperatorScratch;
+struct OperatorBlocks {
+    std::mutex mutex;  // taken without gMutex
+    std::vector<void *> blocks;  // the last one is in use
+    size_t bytes = 0;            // of that
+};
+std::map<std::pair<int, hipStream_t>, OperatorBlocks> gOperatorBlocks;  // nodes stay, without memory once they are released
 }  // namespace
 
-void *operatorScratchFor(hipStream_t s, size_t bytes) {
+OperatorScratch operatorScratchFor(hipStream_t s, size_t bytes) {
     int dev = 0;
     (void)hipGetDevice(&dev);
-    std::lock_guard<std::mutex> lock(gMutex);
-    std::pair<void *, size_t> &block = gOperatorScratch[std::make_pair(dev, s)];
-    if (block.first != nullptr && block.second >= bytes) return block.first;
-    size_t want = (size_t)1 << 20;  // powers of two, so that a growing batch does not allocate at every step
-    while (want < bytes) want <<= 1;
-    if (block.first != nullptr) {
-        (void)hipStreamSynchronize(s);  // earlier work on this stream may still use the old block
-        (void)hipFree(block.first);
-        block = std::pair<void *, size_t>(nullptr, 0);
+    OperatorBlocks *own = nullptr;
+    {
+        std::lock_guard<std::mutex> lock(gMutex);
+        own = &gOperatorBlocks[std::make_pair(dev, s)];
     }
-    void *p = nullptr;
-    hipError_t e = hipMalloc(&p, want);
-    if (e != hipSuccess) {
-        (void)hipGetLastError();
-        throwHip("operator scratch allocation", e);
+    OperatorScratch scratch;
+    scratch.held = std::unique_lock<std::mutex>(own->mutex);
+    if (own->blocks.empty() || own->bytes < bytes) {
+        size_t want = (size_t)1 << 20;  // powers of two, so that a growing batch does not allocate at every step
+        while (want < bytes) want <<= 1;
+        own->blocks.reserve(own->blocks.size() + 1);
+        void *p = nullptr;
+        hipError_t e = hipMalloc(&p, want);
+        if (e != hipSuccess && !own->blocks.empty()) {  // without the blocks outgrown, once nothing uses them any more
+            (void)hipGetLastError();
+            e = hipStreamSynchronize(s);
+            if (e != hipSuccess) throwHip("operator scratch", e);
+            for (void *old : own->blocks) (void)hipFree(old);
+            own->blocks.clear();
+            own->bytes = 0;
+            e = hipMalloc(&p, want);
+        }
+        if (e != hipSuccess) {
+            (void)hipGetLastError();
+            throwHip("operator scratch allocation", e);
+        }
+        own->blocks.push_back(p);
+        own->bytes = want;
     }
-    block = std::make_pair(p, want);
-    return p;
+    scratch.ptr = own->blocks.back();
+    return scratch;
 }
 
 namespace {
@@ -353,24 +371,31 @@ void releaseStreamResources(hipStream_t s) {
     const auto key = std::make_pair(dev, s);
     Workspace w;
     w.ptr = nullptr;
-    void *slots = nullptr, *pinned = nullptr, *scratch = nullptr;
+    void *slots = nullptr, *pinned = nullptr;
+    OperatorBlocks *own = nullptr;
     {
         std::lock_guard<std::mutex> lock(gMutex);
         auto wi = gWorkspaces.find(key);
         if (wi != gWorkspaces.end()) { w = wi->second; gWorkspaces.erase(wi); }
         auto fi = gFlatSlots.find(key);
         if (fi != gFlatSlots.end()) { slots = fi->second.block; gFlatSlots.erase(fi); }
-        auto si = gOperatorScratch.find(key);
-        if (si != gOperatorScratch.end()) { scratch = si->second.first; gOperatorScratch.erase(si); }
+        auto bi = gOperatorBlocks.find(key);
+        if (bi != gOperatorBlocks.end()) own = &bi->second;
         auto pi = gPinnedSlots.find(key);
         if (pi != gPinnedSlots.end()) { pinned = pi->second.block; gPinnedSlots.erase(pi); }
     }
-    if (w.ptr == nullptr && slots == nullptr && pinned == nullptr && scratch == nullptr) return;
+    std::vector<void *> scratch;
+    if (own != nullptr) {
+        std::lock_guard<std::mutex> lock(own->mutex);
+        scratch.swap(own->blocks);
+        own->bytes = 0;
+    }
+    if (w.ptr == nullptr && slots == nullptr && pinned == nullptr && scratch.empty()) return;
     hipError_t e = hipStreamSynchronize(s);  // what is queued on the stream may still use them
     if (e != hipSuccess) throwHip("releaseStreamResources", e);
     if (w.ptr != nullptr) (void)hipFree(w.ptr);
     if (slots != nullptr) (void)hipFree(slots);
-    if (scratch != nullptr) (void)hipFree(scratch);
+    for (void *block : scratch) (void)hipFree(block);
     if (pinned != nullptr) (void)hipHostFree(pinned);
 }
 

@@ -7,6 +7,7 @@
 #include <atomic>
 #include <cstdio>
 #include <memory>
+#include <mutex>
 #include <stdexcept>
 #include <string>
 #include <vector>
@@ -75,8 +76,15 @@ void reportUnknownOp(const char *family, int opNum);
 // Device scratch owned by the library, one per (device, stream), allocated on first use and kept.
 Workspace workspaceFor(hipStream_t s, size_t minBytes);
 // Device scratch of the operators of training.h, one block per (device, stream) beside the workspace above, so that
-// growing it never frees what a captured graph of another call holds.  Not for streams under capture.
-void *operatorScratchFor(hipStream_t s, size_t bytes);
+// growing it never frees what a captured graph of another call holds.  Not for streams under capture.  The block is the
+// caller's until `held` goes: a call keeps it until all of its launches are enqueued, so that those of another thread on the
+// same stream come before or behind them.  A call that needs more than the block has gets another one without a wait; the old
+// one, which queued work may still use, is kept until the stream is released (all of them together are smaller than the last).
+struct OperatorScratch {
+    void *ptr = nullptr;
+    std::unique_lock<std::mutex> held;
+};
+OperatorScratch operatorScratchFor(hipStream_t s, size_t bytes);
 // Adds the slots, counter and ticket of the one-launch whole-array reduction to `w`: a block of device memory per
 // (device, stream) that only those reductions use, cleared when it is allocated.  Calls on one stream run one after the
 // other, so they may share it (one host thread per stream: the ticket source is not synchronised).

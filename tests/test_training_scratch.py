@@ -1,0 +1,132 @@
+"""The library's own scratch of the operators around a language model's matrix products: blocks that grow while work is queued,
+several threads on streams of their own and on one stream."""
+import ctypes
+import threading
+
+import pytest
+
+from libnd4j_amd import harness
+from test_training_path import Calls, same
+
+pytestmark = pytest.mark.gpu
+
+SIZES = ((5, 100), (37, 300), (230, 900), (600, 2400), (100, 5003))  # rows and width, with scratch from less than 1 MiB to 20
+
+
+@pytest.fixture(scope="module")
+def dev():
+    return harness.Device()
+
+
+def prepared(dev, stream, sizes, seed):
+    """calls without scratch of their own on `stream`, and what they give with it, one after the other"""
+    calls, want = [], []
+    for k, (rows, width) in enumerate(sizes):
+        ours, theirs = Calls(dev, dev.stream, "Float", rows, width, 300, seed + k), Calls(dev, stream, "Float", rows, width, 300, seed + k, False)
+        ours.fresh()
+        theirs.fresh()
+        ours.run()
+        dev.sync()
+        want.append(ours.results())
+        calls.append(theirs)
+    return calls, want
+
+
+def at_once(works):
+    failures = []
+
+    def guarded(work):
+        try:
+            work()
+        except Exception as e:  # reported below, by the thread that asserts
+            failures.append(e)
+
+    threads = [threading.Thread(target=guarded, args=(w,)) for w in works]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failures, failures
+
+
+def test_blocks_that_grow_behind_queued_work(dev):
+    stream = dev.ops.createStream()
+    calls, want = prepared(dev, stream, SIZES, 0)
+    for _ in range(2):
+        for c in calls + calls[::-1]:
+            c.run()
+        dev.ops.streamSynchronize(stream)
+        for c, w in zip(calls, want):
+            assert same(c.results(), w)
+        dev.ops.amd_releaseStream(stream)
+
+
+def test_threads_whose_blocks_grow(dev):
+    streams = [dev.ops.createStream() for _ in range(4)]
+    held = [prepared(dev, s, SIZES[k % 2:], 10 * k) for k, s in enumerate(streams)]
+
+    def work(calls, stream):
+        for _ in range(5):
+            for c in calls:
+                c.run()
+        dev.ops.streamSynchronize(stream)
+
+    at_once([lambda c=c, s=s: work(c, s) for (c, _), s in zip(held, streams)])
+    for (calls, want), s in zip(held, streams):
+        for c, w in zip(calls, want):
+            assert same(c.results(), w)
+        dev.ops.amd_releaseStream(s)
+
+
+@pytest.mark.parametrize("plain", (False, True))
+def test_threads_on_one_stream(dev, plain):
+    """a call's launches are not mixed with another thread's that use the same block; plain: the stream of null"""
+    stream = None if plain else dev.ops.createStream()
+    held = [prepared(dev, stream if stream is not None else 0, SIZES[:4][::1 - 2 * (k % 2)], 10 * k) for k in range(4)]
+    wait = dev.ops.streamSynchronize
+
+    def work(calls):
+        for _ in range(10):
+            for c in calls:
+                c.run()
+        wait(stream)
+
+    at_once([lambda c=c: work(c) for c, _ in held])
+    for calls, want in held:
+        for c, w in zip(calls, want):
+            assert same(c.results(), w)
+    dev.ops.amd_releaseStream(stream)
+
+
+def test_a_block_grows_without_a_wait(dev):
+    """The stream waits for a function of the host's; a call on it that needs a larger block returns all the same, and so does a
+    call on another stream.  (The function ends by itself after 20 seconds.)"""
+    hip = ctypes.CDLL("libamdhip64.so")
+    stream, other = dev.ops.createStream(), dev.ops.createStream()
+    (small, large), (want, more) = prepared(dev, stream, (SIZES[0], SIZES[3]), 3)
+    (beside,), _ = prepared(dev, other, SIZES[2:3], 5)
+    small.run()
+    dev.ops.streamSynchronize(stream)
+    go, returned = threading.Event(), threading.Event()
+    waiting = ctypes.CFUNCTYPE(None, ctypes.c_void_p)(lambda _: go.wait(20) and None)
+
+    def work():
+        small.run()
+        large.run()
+        beside.run()
+        returned.set()
+
+    try:
+        assert hip.hipLaunchHostFunc(ctypes.c_void_p(stream), waiting, None) == 0
+        thread = threading.Thread(target=work)
+        thread.start()
+        in_time = returned.wait(10)
+    finally:
+        go.set()
+    thread.join()
+    dev.ops.streamSynchronize(stream)
+    dev.ops.streamSynchronize(other)
+    assert in_time
+    assert same(small.results(), want) and same(large.results(), more)
+    for s in (stream, other):
+        dev.ops.amd_releaseStream(s)
