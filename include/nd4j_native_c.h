@@ -344,9 +344,9 @@ void nd4j_amd_execTokenLogProbsDouble(Nd4jPointer *extraPointers, double *x, Nd4
                                       double *topLogProbs, Nd4jPointer scratch, Nd4jLong scratchBytes);
 Nd4jLong nd4j_amd_scratchTokenLogProbs(Nd4jLong rows, Nd4jLong length, int k);
 /* dx = dLogProbs (delta(token) - p) - dEntropy p (log p + entropy) with the logSum and entropy of the forward call.
- * dLogProbs or dEntropy may be null (tokens and entropy then too).  A negative token's dLogProbs counts as 0, a token
- * behind the row's end makes the row of dx NaN, a row without a distribution (logSum -infinity) gets zeros.  The
- * alternatives are not differentiated.  dx may be x (the same view). */
+ * dLogProbs or dEntropy may be null (tokens and entropy then too).  A negative token's dLogProbs is not looked at and has
+ * no share of dx, whatever the row holds; a token behind the row's end makes the row of dx NaN, a row without a
+ * distribution (logSum -infinity) gets zeros.  The alternatives are not differentiated.  dx may be x (the same view). */
 void nd4j_amd_execTokenLogProbsBpFloat(Nd4jPointer *extraPointers, float *x, Nd4jLong *xShapeInfo, Nd4jLong *tokens,
                                        float *logSum, float *entropy, float *dLogProbs, float *dEntropy, float *dx,
                                        Nd4jLong *dxShapeInfo);

@@ -690,6 +690,8 @@ __global__ void __launch_bounds__(kWaveLanes) tokenProbsJoinKernel(const T *x, R
 }
 
 // ---- backward ----------------------------------------------------------------------------------------------------------
+// A row is zero if it has no distribution, or if its token is padding and no entropy is differentiated: padded places may hold
+// anything, NaN too, which 0 times p would let through.
 template <typename T>
 __global__ void __launch_bounds__(kRowThreads) tokenProbsBpAnyKernel(const T *x, RowView xv, const Long *tokens,
                                                                      const typename Compute<T>::type *logSum,
@@ -705,11 +707,12 @@ __global__ void __launch_bounds__(kRowThreads) tokenProbsBpAnyKernel(const T *x,
         C a = t < 0 ? (C)0 : dLogProbs[r];
         if (t >= xv.length) a = notANumber<C>();
         const C b = dEntropy != nullptr ? dEntropy[r] : (C)0, h = dEntropy != nullptr ? entropy[r] : (C)0;
+        const bool zero = ls == -infinite<C>() || (t < 0 && dEntropy == nullptr);
         for (Long c = threadIdx.x; c < xv.length; c += kRowThreads) {
             const C lp = toCompute(xr[c * xv.el]) - ls, p = m::expSoft_(lp);
             C d = (c == t ? a : (C)0) - a * p;
             if (dEntropy != nullptr && p != (C)0) d -= b * p * (lp + h);
-            dxr[c * dxv.el] = fromCompute<T>(ls == -infinite<C>() ? (C)0 : d);
+            dxr[c * dxv.el] = fromCompute<T>(zero ? (C)0 : d);
         }
     }
 }
@@ -736,12 +739,13 @@ __global__ void __launch_bounds__(kRowThreads) tokenProbsBpAcrossKernel(const T 
         C a = t < 0 ? (C)0 : dLogProbs[r];
         if (t >= xv.length) a = notANumber<C>();
         const C b = dEntropy != nullptr ? dEntropy[r] : (C)0, h = dEntropy != nullptr ? entropy[r] : (C)0;
+        const bool zero = ls == -infinite<C>() || (t < 0 && dEntropy == nullptr);
 #pragma unroll 4
         for (Long c = begin; c < end; c++) {
             const C lp = toCompute(x[r * xv.row + c * xv.el]) - ls, p = m::expSoft_(lp);
             C d = (c == t ? a : (C)0) - a * p;
             if (dEntropy != nullptr && p != (C)0) d -= b * p * (lp + h);
-            dx[r * dxv.row + c * dxv.el] = fromCompute<T>(ls == -infinite<C>() ? (C)0 : d);
+            dx[r * dxv.row + c * dxv.el] = fromCompute<T>(zero ? (C)0 : d);
         }
     }
 }
@@ -769,15 +773,15 @@ __global__ void __launch_bounds__(kRowThreads) tokenProbsBpRowsKernel(const T *x
         C a = t < 0 ? (C)0 : dLogProbs[r];
         if (t >= xv.length) a = notANumber<C>();
         const C b = ENTROPY ? dEntropy[r] : (C)0, h = ENTROPY ? entropy[r] : (C)0;
-        const bool none = ls == -infinite<C>();
+        const bool zero = ls == -infinite<C>() || (t < 0 && !ENTROPY);
         auto gradient = [&](C v) {
             const C lp = v - ls, p = expOf(lp);
             C d = -a * p;
             if (ENTROPY) d -= p != (C)0 ? b * p * (lp + h) : (C)0;
-            return none ? (C)0 : d;
+            return zero ? (C)0 : d;
         };
         for (int c0 = begin; c0 < end; c0 += ROUND) {
-            const bool hasToken = t >= c0 && t < (Long)c0 + ROUND && !none;
+            const bool hasToken = t >= c0 && t < (Long)c0 + ROUND && !zero;
             if (c0 + (Long)ROUND <= end) {
                 Pack<T> v[VECTORS];
 #pragma unroll

@@ -1,0 +1,45 @@
+"""The gradient of log probabilities of tokens: padding over rows that hold anything."""
+import numpy as np
+import pytest
+
+from libnd4j_amd import harness
+from test_training_ops import run_token_probs, run_token_probs_bp, token_probs_bp_oracle
+from training_views import COMPUTE, STORAGE, SUFFIXES, close
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def dev():
+    return harness.Device()
+
+
+@pytest.mark.parametrize("S", SUFFIXES)
+@pytest.mark.parametrize("lx,ldx", [("dense", "dense"), ("pitch3", "offset1"), ("forder", "forder"), ("inner2", "dense")])
+@pytest.mark.parametrize("n", (40, 3000, 9001))
+def test_padding_has_no_gradient_whatever_the_row_holds(dev, S, lx, ldx, n):
+    """a negative token: the row's log probability is 0 by definition, and zeros come back for rows of NaN and infinities too"""
+    rs = np.random.RandomState(n)
+    C = COMPUTE[S]
+    x = rs.randn(7, n).astype(STORAGE[S])
+    x[0] = np.nan
+    x[1, n // 2] = np.nan
+    x[2, 3] = np.inf
+    x[3] = np.inf
+    x[4] = -np.inf
+    tokens = np.array([-1, -5, -1, -1, -1, -1, n // 3])
+    out = run_token_probs(dev, S, x, tokens, 0)
+    assert not out["lp"][:6].any()
+    a = rs.randn(7).astype(C)
+    a[1], a[2] = np.nan, np.inf  # (nor does what stands in a padded place count)
+    for inplace in (False, True):
+        got = run_token_probs_bp(dev, S, x, tokens, out["ls"], None, a, None, lx, ldx, inplace)
+        assert not got[:6].any()
+        want, tol = token_probs_bp_oracle(x[6:], tokens[6:], out["ls"][6:], None, a[6:], None, S)
+        close(got[6:], want, tol)
+    # with entropies the row's NaN are those of the entropy's gradient, and a row of numbers has that alone
+    b = (rs.randn(7) / 4).astype(C)
+    got = run_token_probs_bp(dev, S, x, tokens, out["ls"], out["h"], a, b, lx, ldx)
+    want, tol = token_probs_bp_oracle(x[5:], tokens[5:], out["ls"][5:], out["h"][5:], a[5:], b[5:], S)
+    close(got[5:], want, tol)
+    assert not got[4].any() and np.isnan(got[1]).all()
