@@ -775,7 +775,9 @@ __global__ void __launch_bounds__(kRowThreads) tokenProbsBpRowsKernel(const T *x
         const C b = ENTROPY ? dEntropy[r] : (C)0, h = ENTROPY ? entropy[r] : (C)0;
         const bool zero = ls == -infinite<C>() || (t < 0 && !ENTROPY);
         auto gradient = [&](C v) {
-            const C lp = v - ls, p = expOf(lp);
+            // (a half keeps 2^-11 of it; of what is stored in more bits, expOf would be 15 x 2^-24 off at a log probability of -20, and
+            // 0 where p is subnormal: [4096,32000] floats 168 us with the exact one, 165 with expOf)
+            const C lp = v - ls, p = sizeof(T) == 2 ? expOf(lp) : m::expSoft_(lp);
             C d = -a * p;
             if (ENTROPY) d -= p != (C)0 ? b * p * (lp + h) : (C)0;
             return zero ? (C)0 : d;
