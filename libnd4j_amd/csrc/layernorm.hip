@@ -625,10 +625,19 @@ unsigned gridOf(Long blocks) { return (unsigned)(blocks < 1 ? 1 : (blocks > (1 <
 }  // namespace
 
 constexpr int kBpBlocks = 256;  // of the register kernel; twice as many where a lane holds one vector
+constexpr Long kBpOnePack = 64, kBpTwoPacks = 2048;  // vectors of a row that its lanes hold one and two of; longer rows go elsewhere
 
+// the most blocks of the register kernel for rows of this many vectors (0: they are not its)
+static Long mostBpBlocks(Long vectors) { return vectors <= kBpOnePack ? 2 * kBpBlocks : (vectors <= kBpTwoPacks ? kBpBlocks : 0); }
+template <typename T> static size_t bpScratch(Long rows, Long length) {
+    // (views that are not dense go by columnSplits whatever their length; no kernel has more blocks than rows)
+    const Long any = columnSplits(rows, length), most = mostBpBlocks(length / Pack<T>::N), held = rows < most ? rows : most;
+    return (size_t)2 * (any > held ? any : held) * partialPitch(length) * sizeof(typename Compute<T>::type);
+}
 size_t layerNormBpScratch(Long rows, Long length) {
-    const Long any = columnSplits(rows, length), held = rows < 2 * kBpBlocks ? (rows < 1 ? 1 : rows) : 2 * kBpBlocks;
-    return (size_t)2 * (any > held ? any : held) * partialPitch(length) * sizeof(double);
+    const size_t half = bpScratch<float16>(rows, length), single = bpScratch<float>(rows, length), twice = bpScratch<double>(rows, length);
+    const size_t most = half > single ? half : single;
+    return most > twice ? most : twice;
 }
 
 // Blocks of about four waves, whole teams: more teams in a block would wait for each other.
@@ -677,7 +686,7 @@ int runBpRows(hipStream_t s, const T *x, const RowView &xv, const T *gain, const
     const int waves = teamWaves(xv.length / Pack<T>::N, PACKS);
     const int teams = LANES < kWaveLanes ? kBpThreads / LANES : kBpThreads / kWaveLanes / waves;
     // as many turns as the most blocks would take, the rows spread evenly over them
-    const Long most = PACKS == 1 ? 2 * kBpBlocks : kBpBlocks, turns = (xv.rows + most * teams - 1) / (most * teams);
+    const Long most = mostBpBlocks(xv.length / Pack<T>::N), turns = (xv.rows + most * teams - 1) / (most * teams);
     const int blocks = gridFor(xv.rows, turns * teams, (int)most);
     const int size = LANES < kWaveLanes ? LANES : waves * kWaveLanes;
     const size_t lds = partial != nullptr ? (size_t)(teams / 2) * (Pack<T>::N * PACKS * size + Pack<T>::N) * sizeof(C) : 0;
@@ -698,8 +707,8 @@ void launchLayerNormBp(hipStream_t s, const T *x, const RowView &xv, const T *ga
         const Long vectors = xv.length / Pack<T>::N;
 #define ROWS(LANES, PACKS) splits = runBpRows<T, LANES, PACKS>(s, x, xv, gain, mean, invStd, dz, dzv, dx, dxv, partial)
         if (vectors <= 16) ROWS(16, 1);
-        else if (vectors <= 64) ROWS(64, 1);
-        else if (vectors <= 2048) ROWS(64, 2);
+        else if (vectors <= kBpOnePack) ROWS(64, 1);
+        else if (vectors <= kBpTwoPacks) ROWS(64, 2);
 #undef ROWS
     }
     if (splits == 0) {  // any other view: the columns first, since dx may lie where dz or x does

@@ -1,12 +1,15 @@
 """The library's own scratch of the operators around a language model's matrix products: blocks that grow while work is queued,
-several threads on streams of their own and on one stream."""
+several threads on streams of their own and on one stream; and scratch of the callers', of the sizes that they are told."""
 import ctypes
 import threading
 
+import numpy as np
 import pytest
 
 from libnd4j_amd import harness
+from test_training_ops import bp_inputs
 from test_training_path import Calls, same
+from training_views import COMPUTE, STORAGE, SUFFIXES, Vec, View, extra
 
 pytestmark = pytest.mark.gpu
 
@@ -130,3 +133,60 @@ def test_a_block_grows_without_a_wait(dev):
     assert same(small.results(), want) and same(large.results(), more)
     for s in (stream, other):
         dev.ops.amd_releaseStream(s)
+
+
+BP_SIZES = ((1, 1), (1, 5003), (3, 40), (511, 64), (513, 65), (700, 512), (700, 513), (3000, 1024), (300, 4097), (300, 4098), (260, 8195), (260, 8196),
+            (257, 16391), (257, 16392), (100, 70001))
+
+
+@pytest.mark.parametrize("S", SUFFIXES)
+@pytest.mark.parametrize("rows,n", BP_SIZES)
+def test_scratch_of_the_size_that_is_asked_for(dev, S, rows, n):
+    """what a call is told to bring is enough, and nothing behind it is written"""
+    ops, T, C = dev.ops, STORAGE[S], COMPUTE[S]
+    rs = np.random.RandomState(rows + n)
+    x, gain, mean, inv, dz = bp_inputs(S, rows, n, rows + n)
+    tokens = rs.randint(-1, 50, rows)
+
+    def guarded(size):
+        return size, dev.upload(np.full(size + 4096, 0x5a, np.uint8))
+
+    def whole(size, buf):
+        assert (buf.download(np.uint8)[size:] == 0x5a).all()
+        buf.free()
+
+    for layout in ("dense", "inner2", "forder"):
+        X, DZ, DX = View(dev, rows, n, layout, T, x), View(dev, rows, n, layout, T, dz), View(dev, rows, n, layout, T)
+        M, I, DG, DB = Vec(dev, mean, C), Vec(dev, inv, C), Vec(dev, np.zeros(n), T), Vec(dev, np.zeros(n), T)
+        size, buf = guarded(ops.amd_scratchLayerNormBp(rows, n))
+        getattr(ops, "amd_execLayerNormBp" + S)(extra(dev, x=X, y=DZ, z=DX), X.ptr, X.info_ptr, None, M.ptr, I.ptr, DZ.ptr, DZ.info_ptr, DX.ptr, DX.info_ptr,
+                                                DG.ptr, DB.ptr, buf.ptr, size)
+        whole(size, buf)
+        W, K = View(dev, 50, n, layout, T), Vec(dev, tokens, np.int64)
+        size, buf = guarded(ops.amd_scratchEmbeddingBp(rows, 50, n))
+        getattr(ops, "amd_execEmbeddingBp" + S)(extra(dev, x=DZ, z=W), DZ.ptr, DZ.info_ptr, K.ptr, rows, W.ptr, W.info_ptr, 1.0, 0, buf.ptr, size)
+        whole(size, buf)
+        k = min(n, 64)
+        top, top_lp, lp = Vec(dev, np.zeros(rows * k), np.int64), Vec(dev, np.zeros(rows * k), C), Vec(dev, np.zeros(rows), C)
+        size, buf = guarded(ops.amd_scratchTokenLogProbs(rows, n, k))
+        getattr(ops, "amd_execTokenLogProbs" + S)(extra(dev, x=X), X.ptr, X.info_ptr, K.ptr, lp.ptr, None, None, k, top.ptr, top_lp.ptr, buf.ptr if size else None, size)
+        whole(size, buf)
+        for v in (X, DZ, DX, M, I, DG, DB, W, K, top, top_lp, lp):
+            v.free()
+
+
+@pytest.mark.parametrize("S", SUFFIXES)
+@pytest.mark.parametrize("count", (1, 60))
+def test_scratch_of_clipping_of_the_size_that_is_asked_for(dev, S, count):
+    ops, total = dev.ops, 20000003
+    flat = dev.empty(total * STORAGE[S]().itemsize)
+    ops.memset(flat.ptr, 0, total * STORAGE[S]().itemsize, 0, None)
+    ends = np.linspace(0, total, count + 1).astype(np.int64)
+    tables, offsets = dev.upload(flat.ptr + ends[:-1] * STORAGE[S]().itemsize), Vec(dev, ends, np.int64)
+    norm = Vec(dev, [1.0], COMPUTE[S])
+    size = ops.amd_scratchClipByGlobalNorm(total)
+    buf = dev.upload(np.full(size + 4096, 0x5a, np.uint8))
+    getattr(ops, "amd_execClipByGlobalNorm" + S)(extra(dev), tables.ptr, tables.ptr, offsets.ptr, count, total, 1.0, norm.ptr, buf.ptr, size)
+    assert (buf.download(np.uint8)[size:] == 0x5a).all() and norm.get()[0] == 0
+    for v in (flat, tables, offsets, norm, buf):
+        v.free()
