@@ -242,8 +242,8 @@ __global__ void __launch_bounds__(kSortThreads) sortPlaceKernel(const Long *toke
     }
 }
 
-// Up to kSmallSort tokens of fewer than 2^18: one block does all passes in LDS, in one launch instead of two a pass, each
-// token as one word of its key and, below it, its position.  (A round of 1024 tokens takes about 1 us a pass: 16384 tokens took
+// Up to kSmallSort tokens of a vocabulary below 2^(32 - kSmallBits): one block does all passes in LDS, in one launch instead of
+// two a pass, each token as one word of its key (the key `vocabulary` among them) and, below it, its position.  (A round of 1024 tokens takes about 1 us a pass: 16384 tokens took
 // 35 us this way.)
 constexpr int kSmallThreads = 1024, kSmallBits = 12, kSmallSort = 1 << kSmallBits, kSmallRounds = kSmallSort / kSmallThreads;
 __global__ void __launch_bounds__(kSmallThreads) sortSmallKernel(const Long *tokens, unsigned n, unsigned vocabulary, int passes, unsigned *keysOut,
