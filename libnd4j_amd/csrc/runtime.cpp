@@ -179,6 +179,14 @@ struct OperatorBlocks {
     size_t bytes = 0;            // of that
 };
 std::map<std::pair<int, hipStream_t>, OperatorBlocks> gOperatorBlocks;  // nodes stay, without memory once they are released
+
+// While another stream is captured (by this thread, or by any in the global mode) an allocation is refused and ends that capture,
+// unless the thread says that it is not part of it.
+struct OutsideCaptures {
+    hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+    OutsideCaptures() { (void)hipThreadExchangeStreamCaptureMode(&mode); }
+    ~OutsideCaptures() { (void)hipThreadExchangeStreamCaptureMode(&mode); }
+};
 }  // namespace
 
 OperatorScratch operatorScratchFor(hipStream_t s, size_t bytes) {
@@ -194,6 +202,7 @@ OperatorScratch operatorScratchFor(hipStream_t s, size_t bytes) {
     if (own->blocks.empty() || own->bytes < bytes) {
         size_t want = (size_t)1 << 20;  // powers of two, so that a growing batch does not allocate at every step
         while (want < bytes) want <<= 1;
+        const OutsideCaptures outside;
         own->blocks.reserve(own->blocks.size() + 1);
         void *p = nullptr;
         hipError_t e = hipMalloc(&p, want);

@@ -135,6 +135,43 @@ def test_a_block_grows_without_a_wait(dev):
         dev.ops.amd_releaseStream(s)
 
 
+@pytest.mark.parametrize("mode", (0, 1, 2))  # global, thread-local, relaxed
+def test_eager_calls_beside_a_capture(dev, mode):
+    """a stream that is not captured gets its block, and larger ones, while another one is; the graph replays as it should"""
+    hip = ctypes.CDLL("libamdhip64.so")
+    stream, other = dev.ops.createStream(), dev.ops.createStream()
+    captured, twin = Calls(dev, stream, "Float", 37, 300, 300, 7), Calls(dev, stream, "Float", 37, 300, 300, 7)
+    beside, want = prepared(dev, other, SIZES[:4], 20)
+    for c in (captured, twin):
+        c.fresh()
+    dev.sync()
+    graph, executable = ctypes.c_void_p(), ctypes.c_void_p()
+    assert hip.hipStreamBeginCapture(ctypes.c_void_p(stream), mode) == 0
+    try:
+        for c in beside:
+            c.run()
+        captured.run()
+    finally:
+        status = hip.hipStreamEndCapture(ctypes.c_void_p(stream), ctypes.byref(graph))
+    assert status == 0 and graph.value
+    dev.ops.streamSynchronize(other)
+    for c, w in zip(beside, want):
+        assert same(c.results(), w)
+    assert hip.hipGraphInstantiate(ctypes.byref(executable), graph, None, None, ctypes.c_size_t(0)) == 0
+    for _ in range(3):
+        assert hip.hipGraphLaunch(executable, ctypes.c_void_p(stream)) == 0
+        twin.run()
+        dev.ops.streamSynchronize(stream)
+        assert same(captured.results(), twin.results())
+        for c in (captured, twin):
+            c.fresh()
+        dev.sync()
+    hip.hipGraphExecDestroy(executable)
+    hip.hipGraphDestroy(graph)
+    for s in (stream, other):
+        dev.ops.amd_releaseStream(s)
+
+
 BP_SIZES = ((1, 1), (1, 5003), (3, 40), (511, 64), (513, 65), (700, 512), (700, 513), (3000, 1024), (300, 4097), (300, 4098), (260, 8195), (260, 8196),
             (257, 16391), (257, 16392), (100, 70001))
 
