@@ -22,10 +22,15 @@ const Long kMostLength = ((Long)1 << 31) - ((Long)1 << 20);  // columns fit an i
 
 // The rows of a view: its last dimension, at every position of the others, which have to lie a common distance apart.
 RowView rowsOf(const char *op, const char *name, Nd4jPointer *extra, int slot, const Long *arg, std::vector<Long> &storage, hipStream_t s) {
-    // (a read-back synchronises the stream, which would end a capture)
-    if (slotOf(extra, slot) == nullptr && arg != nullptr && streamIsCapturing(s) && isDeviceMemory(arg))
-        refuse(op, std::string("the stream is being captured, which needs a host copy of the shapeInfo of ") + name);
-    const Long *info = hostShapeInfo(extra, slot, arg, storage, s);
+    // (a read-back synchronises the stream, which would end its capture)
+    const Long *info = nullptr;
+    if (slotOf(extra, slot) == nullptr && arg != nullptr && isDeviceMemory(arg)) {
+        if (streamIsCapturing(s)) refuse(op, std::string("the stream is being captured, which needs a host copy of the shapeInfo of ") + name);
+        const OutsideCaptures outside;
+        info = hostShapeInfo(extra, slot, arg, storage, s);
+    } else {
+        info = hostShapeInfo(extra, slot, arg, storage, s);
+    }
     if (info == nullptr) refuse(op, std::string("no shapeInfo of ") + name);
     const int rank = siRank(info);
     if (rank < 1 || rank > kMaxRank) refuse(op, std::string(name) + " needs a rank between 1 and 32");

@@ -179,14 +179,6 @@ struct OperatorBlocks {
     size_t bytes = 0;            // of that
 };
 std::map<std::pair<int, hipStream_t>, OperatorBlocks> gOperatorBlocks;  // nodes stay, without memory once they are released
-
-// While another stream is captured (by this thread, or by any in the global mode) an allocation is refused and ends that capture,
-// unless the thread says that it is not part of it.
-struct OutsideCaptures {
-    hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
-    OutsideCaptures() { (void)hipThreadExchangeStreamCaptureMode(&mode); }
-    ~OutsideCaptures() { (void)hipThreadExchangeStreamCaptureMode(&mode); }
-};
 }  // namespace
 
 OperatorScratch operatorScratchFor(hipStream_t s, size_t bytes) {

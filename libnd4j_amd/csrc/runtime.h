@@ -75,6 +75,14 @@ void reportUnknownOp(const char *family, int opNum);
 
 // Device scratch owned by the library, one per (device, stream), allocated on first use and kept.
 Workspace workspaceFor(hipStream_t s, size_t minBytes);
+// While another stream is captured (by this thread, or by any in the global mode) allocations and waits are refused and end
+// that capture, unless the thread says that they are no part of it: for as long as one of these lives.
+struct OutsideCaptures {
+    hipStreamCaptureMode mode = hipStreamCaptureModeRelaxed;
+    OutsideCaptures() { (void)hipThreadExchangeStreamCaptureMode(&mode); }
+    ~OutsideCaptures() { (void)hipThreadExchangeStreamCaptureMode(&mode); }
+    OutsideCaptures(const OutsideCaptures &) = delete;
+};
 // Device scratch of the operators of training.h, one block per (device, stream) beside the workspace above, so that
 // growing it never frees what a captured graph of another call holds.  Not for streams under capture.  The block is the
 // caller's until `held` goes: a call keeps it until all of its launches are enqueued, so that those of another thread on the

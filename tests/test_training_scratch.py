@@ -172,6 +172,32 @@ def test_eager_calls_beside_a_capture(dev, mode):
         dev.ops.amd_releaseStream(s)
 
 
+@pytest.mark.parametrize("mode", (0, 1, 2))
+def test_shapes_read_back_beside_a_capture(dev, mode):
+    """a call without host copies of its shapeInfo, on a stream that is not captured, while another one is"""
+    hip = ctypes.CDLL("libamdhip64.so")
+    stream, other = dev.ops.createStream(), dev.ops.createStream()
+    x = np.random.RandomState(0).randn(6, 40).astype(np.float32)
+    X, Z, Y = (View(dev, 6, 40, "dense", np.float32, x) for _ in range(3))
+    infos = dev.upload(X.info), dev.upload(Z.info)
+    bare = (ctypes.c_void_p * 20)()
+    bare[1] = other
+    graph = ctypes.c_void_p()
+    dev.sync()
+    assert hip.hipStreamBeginCapture(ctypes.c_void_p(stream), mode) == 0
+    try:
+        dev.ops.amd_execLayerNormFloat(bare, X.ptr, infos[0].ptr, None, None, Z.ptr, infos[1].ptr, None, None, 1e-5)
+        dev.ops.amd_execLayerNormFloat(extra(dev, x=X, z=Y, stream=stream), X.ptr, None, None, None, Y.ptr, None, None, None, 1e-5)
+    finally:
+        status = hip.hipStreamEndCapture(ctypes.c_void_p(stream), ctypes.byref(graph))
+    assert status == 0 and graph.value
+    hip.hipGraphDestroy(graph)
+    dev.ops.streamSynchronize(other)
+    assert np.array_equal(Y.get(), x)  # (captured, and never launched)
+    dev.ops.amd_execLayerNormFloat(extra(dev, x=X, z=Y), X.ptr, None, None, None, Y.ptr, None, None, None, 1e-5)
+    assert np.array_equal(Z.get(), Y.get())
+
+
 BP_SIZES = ((1, 1), (1, 5003), (3, 40), (511, 64), (513, 65), (700, 512), (700, 513), (3000, 1024), (300, 4097), (300, 4098), (260, 8195), (260, 8196),
             (257, 16391), (257, 16392), (100, 70001))
 
