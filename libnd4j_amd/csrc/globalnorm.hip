@@ -14,7 +14,7 @@
 // leaves what fits in the last-level cache, the second reads and writes with the streaming one: 60 tensors of 124M floats
 // 245 us, 6.1 TB/s of the 1.49 GB (streaming in the first sweep too took a tenth longer; ordinary loads in the second 6 %,
 // and ordinary stores 14 %; the second sweep from the end of the range is as fast).  20 tensors of 100003 halves in all
-// take 12.5 us, which is two launches.
+// take 12.6 us, which is two launches.
 //
 // Squares are summed in double: the square of any float is finite there, and the order of the sum does not show in the
 // result's type.  (Squares of halves are exact in float; eight of them are added there first.)  Squares of doubles have three

@@ -146,8 +146,9 @@ __global__ void __launch_bounds__(kAcrossThreads) layerNormAcrossKernel(const T 
 // Rows of contiguous elements that a team holds in its registers: a team is LANES lanes of a wave or as many whole waves as
 // the row needs with PACKS vectors of 16 bytes a lane, and the elements behind the last whole vector go one a lane.  One
 // read of x, one write of z, the next row on its way while one is worked on; gain and bias stay in registers over the
-// team's rows (HELD).  [16384, 1024] halves 13.3 us, 5.1 TB/s; what it has beyond the copy's 10.5 are the two sums of a row, one
-// after the other.  Stores have the streaming policy (a tenth longer without it, and with it for the loads too).
+// team's rows (HELD).  [16384, 1024] halves 13.6 us, 4.9 TB/s, where a copy takes 10.5: 24 vector instructions an element hold the
+// SIMDs for 10.1 us of it, and a row has two sums, one after the other.  (The multiplication by s behind the subtraction is 0.3 us of
+// it.)  Stores have the streaming policy (a tenth longer without it, and with it for the loads too).
 // Loads are unconditional (a vector that is not there re-reads the row's first place, see `at`).
 template <typename T, int LANES, int PACKS>
 __global__ void __launch_bounds__(1024)
@@ -329,9 +330,9 @@ __global__ void __launch_bounds__(kAcrossThreads) layerNormBpAcrossKernel(const 
 // which is why there are no more of them, and 16 waves hide the loads of each other.  (Blocks of a single team, which need not
 // wait for others but leave three times the partial sums, took 50 us where these take 35.)
 //
-// [16384, 1024] floats 40 us, 5.0 TB/s of x, dz and dx: bound by memory.  [4097, 5003] halves 34 us, of which the sums of the
-// columns by the kernel below are 5: about 20 vector instructions an element, six rows for every team where 5.3 would be even, and 9 MB of
-// partial sums written and read again.
+// [16384, 1024] floats 39 us, 5.1 TB/s of x, dz and dx: bound by memory.  [4097, 5003] halves 35 us, of which the sums of the
+// columns by the kernel below are 5: 28 vector instructions an element, which hold the SIMDs for 14.5 us, six rows for every team
+// where 5.3 would be even, and 9 MB of partial sums written and read again.
 constexpr int kBpThreads = 1024;
 // the elements from one row of partial sums to the next: vectors of any type begin at a multiple of 16 bytes
 __host__ __device__ inline Long partialPitch(Long length) { return (length + 7) / 8 * 8; }
@@ -610,8 +611,8 @@ int teamWaves(Long vectors, int packs) {
     return (int)(waves < 1 ? 1 : waves);
 }
 // The blocks of the forward kernel.  Halves, and teams of more than eight waves: as many as the 256 compute units hold at once
-// (32 waves a unit at one vector a lane, by registers 20 at two and 16 at four), each going on from row to row: [16384, 1024]
-// halves 14.4 us, 15.4 with 32 waves a unit throughout and 16.4 with a block for every row; [4096, 8192] floats 52 and 68.  Smaller
+// (32 waves a unit at one vector a lane, by registers 20 at two and 16 at four), each going on from row to row: where [16384, 1024]
+// halves took 14.4 us, 32 waves a unit throughout took 15.4 and a block for every row 16.4; [4096, 8192] floats 52 and 68.  Smaller
 // teams of floats and doubles: three times the 32, which spreads what is left at the end: [16384, 1024] floats 21.0 us, 23.5
 // with 32 and 20.8 with a block for every row, [65536, 256] 21.7, 23.4 and 25.5.
 int rowBlocks(int packs, int size, int blockWaves, int teamWaves) {

@@ -80,8 +80,8 @@ void sameShape(const char *op, const char *a, const RowView &x, const char *b, c
 }
 
 // The caller's scratch when it is given one, else the stream's, kept until the call's launches are enqueued.  A stream under
-// capture gets none of the library's: two graphs captured on it would share the block, and a later call that outgrows it would
-// free it under them.
+// capture gets none of the library's: two graphs captured on it would share the block, and releasing the stream would free it
+// under them.
 OperatorScratch scratchFor(const char *op, hipStream_t s, void *given, Long givenBytes, size_t bytes) {
     OperatorScratch scratch;
     if (bytes == 0) return scratch;

@@ -192,6 +192,7 @@ __global__ void __launch_bounds__(kAcrossThreads) tokenProbsAcrossKernel(const T
 //
 // (Keeping the best elements during the sweep, as the first form did, took 118 us over [4096, 32000] floats at k = 5, where
 // the sweep alone takes 81.  This form takes 86, 6.1 TB/s.  One row of 50257 halves takes 11 us, which is two launches.)
+// Short rows pay for the selection, once a row by a whole block: [20000, 5000] halves 115 us at k = 5, 52 without alternatives.
 
 // exp for the sums: the relative error grows with |d| (a rounding of d log2 e), on terms whose share is exp(d)
 __device__ __forceinline__ float expOf(float d) { return __builtin_amdgcn_exp2f(d * 1.44269502162933349609375f); }
@@ -751,7 +752,7 @@ __global__ void __launch_bounds__(kRowThreads) tokenProbsBpAcrossKernel(const T 
 }
 
 // Rows of contiguous elements: a team of a wave or a block takes a stretch of a row, kBpVectors vectors a lane.  Bound by
-// memory: [4096, 50257] halves, whose rows begin anywhere, 141 us, 5.8 TB/s (with four vectors a lane 148).
+// memory: [4096, 50257] halves, whose rows begin anywhere, 140 us, 5.9 TB/s (with four vectors a lane 148).
 constexpr int kBpVectors = 2;
 template <typename T, int TEAM, bool ENTROPY>
 __global__ void __launch_bounds__(kRowThreads) tokenProbsBpRowsKernel(const T *x, RowView xv, const Long *tokens,
