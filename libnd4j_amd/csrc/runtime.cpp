@@ -392,6 +392,7 @@ void releaseStreamResources(hipStream_t s) {
         own->bytes = 0;
     }
     if (w.ptr == nullptr && slots == nullptr && pinned == nullptr && scratch.empty()) return;
+    const OutsideCaptures outside;
     hipError_t e = hipStreamSynchronize(s);  // what is queued on the stream may still use them
     if (e != hipSuccess) throwHip("releaseStreamResources", e);
     if (w.ptr != nullptr) (void)hipFree(w.ptr);

@@ -137,7 +137,8 @@ def test_a_block_grows_without_a_wait(dev):
 
 @pytest.mark.parametrize("mode", (0, 1, 2))  # global, thread-local, relaxed
 def test_eager_calls_beside_a_capture(dev, mode):
-    """a stream that is not captured gets its block, and larger ones, while another one is; the graph replays as it should"""
+    """a stream that is not captured gets its block, and larger ones, and is released, while another one is captured; the graph
+    replays as it should"""
     hip = ctypes.CDLL("libamdhip64.so")
     stream, other = dev.ops.createStream(), dev.ops.createStream()
     captured, twin = Calls(dev, stream, "Float", 37, 300, 300, 7), Calls(dev, stream, "Float", 37, 300, 300, 7)
@@ -148,6 +149,9 @@ def test_eager_calls_beside_a_capture(dev, mode):
     graph, executable = ctypes.c_void_p(), ctypes.c_void_p()
     assert hip.hipStreamBeginCapture(ctypes.c_void_p(stream), mode) == 0
     try:
+        for c in beside:
+            c.run()
+        dev.ops.amd_releaseStream(other)
         for c in beside:
             c.run()
         captured.run()
