@@ -179,6 +179,9 @@ struct OperatorBlocks {
     size_t bytes = 0;            // of that
 };
 std::map<std::pair<int, hipStream_t>, OperatorBlocks> gOperatorBlocks;  // nodes stay, without memory once they are released
+// hipStreamPerThread is one handle for a stream of every thread's own: told apart by where the thread has this byte
+thread_local char tOwnStream;
+hipStream_t operatorStream(hipStream_t s) { return s == hipStreamPerThread ? reinterpret_cast<hipStream_t>(&tOwnStream) : s; }
 }  // namespace
 
 OperatorScratch operatorScratchFor(hipStream_t s, size_t bytes) {
@@ -187,7 +190,7 @@ OperatorScratch operatorScratchFor(hipStream_t s, size_t bytes) {
     OperatorBlocks *own = nullptr;
     {
         std::lock_guard<std::mutex> lock(gMutex);
-        own = &gOperatorBlocks[std::make_pair(dev, s)];
+        own = &gOperatorBlocks[std::make_pair(dev, operatorStream(s))];
     }
     OperatorScratch scratch;
     scratch.held = std::unique_lock<std::mutex>(own->mutex);
@@ -380,7 +383,7 @@ void releaseStreamResources(hipStream_t s) {
         if (wi != gWorkspaces.end()) { w = wi->second; gWorkspaces.erase(wi); }
         auto fi = gFlatSlots.find(key);
         if (fi != gFlatSlots.end()) { slots = fi->second.block; gFlatSlots.erase(fi); }
-        auto bi = gOperatorBlocks.find(key);
+        auto bi = gOperatorBlocks.find(std::make_pair(dev, operatorStream(s)));
         if (bi != gOperatorBlocks.end()) own = &bi->second;
         auto pi = gPinnedSlots.find(key);
         if (pi != gPinnedSlots.end()) { pinned = pi->second.block; gPinnedSlots.erase(pi); }

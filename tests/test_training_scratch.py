@@ -101,6 +101,23 @@ def test_threads_on_one_stream(dev, plain):
     dev.ops.amd_releaseStream(stream)
 
 
+def test_threads_on_the_stream_of_every_thread(dev):
+    """hipStreamPerThread, 2: one handle, and a stream and a block of its own for each thread"""
+    held = [prepared(dev, 2, SIZES[:4][::1 - 2 * (k % 2)], 10 * k) for k in range(4)]
+
+    def work(calls):
+        for _ in range(10):
+            for c in calls:
+                c.run()
+        dev.ops.streamSynchronize(2)
+        dev.ops.amd_releaseStream(2)
+
+    at_once([lambda c=c: work(c) for c, _ in held])
+    for calls, want in held:
+        for c, w in zip(calls, want):
+            assert same(c.results(), w)
+
+
 def test_a_block_grows_without_a_wait(dev):
     """The stream waits for a function of the host's; a call on it that needs a larger block returns all the same, and so does a
     call on another stream.  (The function ends by itself after 20 seconds.)"""
